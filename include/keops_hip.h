@@ -175,6 +175,91 @@ int keops_hip_ranges_status(void* module, unsigned* status);
  */
 int keops_hip_path_status(void* module, unsigned* taken);
 
+/*
+ * Sequence operators (no counterpart in the reference): attention with a bias by buckets of the relative position, linear
+ * attention with a decay for each head, log probabilities of given tokens.  All pointers are device memory of `device`; a
+ * tensor of rows (batch, head, position, component) is a base pointer and three strides in elements, its components are
+ * neighbours and every row starts at a multiple of 16 bytes.  Launches go to hip_stream, nothing is allocated, nothing waits;
+ * workspaces are the caller's, of the size that the *_bytes function names.  dtype: 0 bfloat16, 1 float16, 2 float32.
+ */
+#define KEOPS_HIP_MAX_REACH 2048
+
+typedef struct keops_hip_bucket_attention {
+  int32_t dtype, batch, heads, kv_heads, dim, causal, buckets, reach;
+  int64_t queries, keys, start;   /* start: key position of query 0, where query_start is NULL */
+  float scale, reserved;
+  const void *q, *k, *v;
+  void* out;
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
+  float* lse;                     /* (batch, heads, queries), base 2; may be NULL in the forward pass */
+  const float* bias;              /* (heads, buckets) */
+  const int32_t* bucket_of;       /* (2 reach + 1): bucket of key position - query position, clamped to -reach..reach */
+  const int32_t* bucket_order;    /* (2 reach + 1): the entries of bucket_of by bucket, in increasing order within one */
+  const int32_t* bucket_begin;    /* (buckets + 1): where each bucket begins in bucket_order */
+  const int32_t* key_lengths;     /* (batch) or NULL: keys that exist; what lies behind them is not read */
+  const int32_t* query_start;     /* (batch) or NULL */
+  /* backward pass */
+  const void* grad_out;
+  void *grad_q, *grad_k, *grad_v; /* grad_q may be NULL */
+  int64_t grad_out_stride[3], grad_q_stride[3], grad_k_stride[3], grad_v_stride[3];
+  float* delta;                   /* (batch, heads, queries), written */
+  float* grad_bias;               /* (heads, buckets) or NULL */
+} keops_hip_bucket_attention;
+
+size_t keops_hip_bucket_attention_forward_bytes(const keops_hip_bucket_attention* a);
+size_t keops_hip_bucket_attention_backward_bytes(const keops_hip_bucket_attention* a);
+int keops_hip_bucket_attention_forward(const keops_hip_bucket_attention* a, void* work, size_t work_bytes, int device, void* hip_stream);
+int keops_hip_bucket_attention_backward(const keops_hip_bucket_attention* a, void* work, size_t work_bytes, int device, void* hip_stream);
+
+/*
+ * Linear attention with a decay for each head.  With g = exp(log_decay[h]) and tokens in order (reverse = 0):
+ *   out_i = sum_{j <= i} g^(i-j) product_scale <q_i, k_j> v_j + query_scale g^(i+1) q_i S_0,
+ *   S_T   = g^T S_0 + update_scale sum_j g^(T-1-j) k_j v_j^T.
+ * reverse = 1: the same over the tokens from the last to the first, with g^i in place of g^(i+1) and g^(T-j) in place of
+ * g^(T-1-j): the form of the gradients with respect to keys and values.  q is (batch, heads, tokens, dim), v has dim_v
+ * components; k and v have k_heads and v_heads heads, q has q_heads, each shared by heads / its heads heads.
+ */
+typedef struct keops_hip_decay_attention {
+  int32_t dtype, batch, heads, q_heads, k_heads, v_heads, dim, dim_v, reverse, out_float32;
+  int64_t tokens;
+  float product_scale, query_scale, update_scale, reserved;
+  const void *q, *k, *v;
+  void* out;                      /* the dtype, or float32 where out_float32 is set */
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];
+  const float* log_decay;         /* (heads) */
+  const int32_t* lengths;         /* (batch) or NULL: tokens that exist; outputs behind them are zeros */
+  const float* state_in;          /* (batch, heads) matrices of dim * dim_v contiguous values, or NULL: zeros */
+  float* state_out;               /* the same, or NULL */
+  int64_t state_in_stride[2], state_out_stride[2]; /* strides of a matrix along dim and along dim_v */
+} keops_hip_decay_attention;
+
+size_t keops_hip_decay_attention_bytes(const keops_hip_decay_attention* a);
+int keops_hip_decay_attention_run(const keops_hip_decay_attention* a, void* work, size_t work_bytes, int device, void* hip_stream);
+
+/* One token: state (batch, heads, dim, dim_v) becomes g state + k v^T in place, out = scale q state.  q, k, v, out: strides of
+   (batch, head); rows need not be aligned beyond their elements. */
+int keops_hip_decay_attention_step(int dtype, int batch, int heads, int kv_heads, int dim, int dim_v, float scale,
+                                   const void* q, const int64_t* q_stride, const void* k, const int64_t* k_stride, const void* v,
+                                   const int64_t* v_stride, const float* log_decay, float* state, void* out, int device,
+                                   void* hip_stream);
+
+/*
+ * Rows of logits: logprob[r] = x[r][token[r]] - lse, entropy[r], and the `top` largest x - lse with their indices (equal values:
+ * lowest index first).  token == ignore_index: logprob 0 and no gradient through it; any other token outside 0..vocab-1: NaN.
+ * A row in which nothing is above -inf has logprob and alternatives -inf and entropy 0.
+ */
+#define KEOPS_HIP_MAX_TOP 64
+size_t keops_hip_token_logprobs_bytes(int dtype, int64_t rows, int64_t vocab, int top);
+int keops_hip_token_logprobs(int dtype, int64_t rows, int64_t vocab, int top, const void* logits, int64_t row_stride,
+                             const int64_t* tokens, int64_t ignore_index, float* logprob, float* entropy, float* lse,
+                             float* top_logprob, int64_t* top_index, void* work, size_t work_bytes, int device, void* hip_stream);
+/* Gradient with respect to the logits; grad_* may be NULL (zeros). */
+int keops_hip_token_logprobs_backward(int dtype, int64_t rows, int64_t vocab, int top, const void* logits, int64_t row_stride,
+                                      const int64_t* tokens, int64_t ignore_index, const float* entropy, const float* lse,
+                                      const int64_t* top_index, const float* grad_logprob, const float* grad_entropy,
+                                      const float* grad_top, void* grad_logits, int64_t grad_row_stride, int device,
+                                      void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

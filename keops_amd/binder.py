@@ -12,6 +12,33 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "csrc", "libkeops_hip.so")
 _lib = None
 
+_I32, _I64, _F32, _P, _SIZE = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
+
+
+class BucketAttention(ctypes.Structure):
+    """keops_hip_bucket_attention of include/keops_hip.h."""
+
+    _fields_ = (
+        [(n, _I32) for n in ("dtype", "batch", "heads", "kv_heads", "dim", "causal", "buckets", "reach")]
+        + [(n, _I64) for n in ("queries", "keys", "start")] + [("scale", _F32), ("reserved", _F32)]
+        + [(n, _P) for n in ("q", "k", "v", "out")] + [(n + "_stride", _I64 * 3) for n in ("q", "k", "v", "out")]
+        + [(n, _P) for n in ("lse", "bias", "bucket_of", "bucket_order", "bucket_begin", "key_lengths", "query_start", "grad_out",
+                             "grad_q", "grad_k", "grad_v")]
+        + [(n + "_stride", _I64 * 3) for n in ("grad_out", "grad_q", "grad_k", "grad_v")] + [("delta", _P), ("grad_bias", _P)]
+    )
+
+
+class DecayAttention(ctypes.Structure):
+    """keops_hip_decay_attention of include/keops_hip.h."""
+
+    _fields_ = (
+        [(n, _I32) for n in ("dtype", "batch", "heads", "q_heads", "k_heads", "v_heads", "dim", "dim_v", "reverse", "out_float32")]
+        + [("tokens", _I64)] + [(n, _F32) for n in ("product_scale", "query_scale", "update_scale", "reserved")]
+        + [(n, _P) for n in ("q", "k", "v", "out")] + [(n + "_stride", _I64 * 3) for n in ("q", "k", "v", "out")]
+        + [(n, _P) for n in ("log_decay", "lengths", "state_in", "state_out")]
+        + [("state_in_stride", _I64 * 2), ("state_out_stride", _I64 * 2)]
+    )
+
 
 class KeOpsHipError(RuntimeError):
     pass
@@ -56,6 +83,18 @@ def lib():
         L.keops_hip_noalloc_scratch_bytes.restype = ctypes.c_size_t
         L.keops_hip_ranges_status.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint)]
         L.keops_hip_path_status.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint)]
+        for name, struct in (("bucket_attention", BucketAttention), ("decay_attention", DecayAttention)):
+            passes = ("_forward", "_backward") if struct is BucketAttention else ("",)
+            for p in passes:
+                size = getattr(L, f"keops_hip_{name}{p}_bytes")
+                size.restype, size.argtypes = _SIZE, [ctypes.POINTER(struct)]
+                getattr(L, f"keops_hip_{name}{p or '_run'}").argtypes = [ctypes.POINTER(struct), _P, _SIZE, ctypes.c_int, _P]
+        L.keops_hip_decay_attention_step.argtypes = [ctypes.c_int] * 6 + [_F32] + [_P] * 9 + [ctypes.c_int, _P]
+        L.keops_hip_token_logprobs_bytes.restype = _SIZE
+        L.keops_hip_token_logprobs_bytes.argtypes = [ctypes.c_int, _I64, _I64, ctypes.c_int]
+        L.keops_hip_token_logprobs.argtypes = [ctypes.c_int, _I64, _I64, ctypes.c_int, _P, _I64, _P, _I64] + [_P] * 6 + [_SIZE, ctypes.c_int, _P]
+        L.keops_hip_token_logprobs_backward.argtypes = (
+            [ctypes.c_int, _I64, _I64, ctypes.c_int, _P, _I64, _P, _I64] + [_P] * 7 + [_I64, ctypes.c_int, _P])
         _lib = L
     return _lib
 
@@ -108,6 +147,12 @@ def mfma_probe(a_bits, b_bits, acc0=0.0, device_id=0):
     if rc != 0:
         raise KeOpsHipError(f"matrix-core probe failed (code {rc})")
     return out
+
+
+def check(rc, what):
+    """Raise the library's message when the entry point ``what`` returned an error code."""
+    if rc != 0:
+        raise KeOpsHipError(f"{what} failed (code {rc}): {last_error()}")
 
 
 def last_error():

@@ -2075,3 +2075,12 @@ int keops_hip_ranges_status(void* module, unsigned* status) {
 size_t keops_hip_noalloc_scratch_bytes(void) { return (size_t)KEOPS_STATIC_SCRATCH_BYTES; }
 
 }  // extern "C"
+
+// Message of the sequence operators (csrc/sequence), which report through keops_hip_last_error() too; returns `code`.
+int keops_seq_fail(int code, const char* message) {
+  try {
+    return fail(code, message);
+  } catch (...) {  // no memory for the text: the code alone
+    return code == 0 ? -1 : code;
+  }
+}

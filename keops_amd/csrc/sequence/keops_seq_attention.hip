@@ -1,0 +1,855 @@
+// Softmax attention with a learned bias by buckets of the relative position:
+//
+//   z_ij = scale <q_i, k_j> + bias[h][bucket(j - p_i)],   p_i = query_start + i,   o_i = sum_j softmax_j(z)_ij v_j
+//
+// and its gradients.  bucket() is a table over the clamped distance -reach..reach, so beyond the reach on either side the bias
+// is one number for a head: tiles of pairs that lie there whole take it as a scalar, the others read a table of the head's
+// biases by distance in LDS, in which the four neighbouring keys of a lane's registers are neighbours.
+#include "../../../include/keops_hip.h"
+#include "keops_seq.h"
+
+using namespace kseq;
+
+namespace {
+
+typedef keops_hip_bucket_attention Args;
+
+constexpr int kPad = 96;  // entries of the distance table beyond the reach on each side: a mixed tile of 64 x 32 pairs reads there
+
+__device__ inline int clampi(int x, int lo, int hi) { return x < lo ? lo : (x > hi ? hi : x); }
+
+struct Span {  // what one sequence of the batch sees
+  int klen;    // keys that exist
+  int start;   // key position of query 0
+};
+__device__ inline Span span_of(const Args& A, int b) {
+  Span s;
+  const int n = (int)A.keys;
+  s.klen = A.key_lengths ? clampi(A.key_lengths[b], 0, n) : n;
+  s.start = A.query_start ? clampi(A.query_start[b], -(1 << 29), 1 << 29) : (int)A.start;
+  return s;
+}
+
+// unit (sequence and key/value head) and block within it.  With a multiple of 8 units, the blocks of one unit run on one XCD
+// (workgroups go to the XCDs in turn), which then holds the unit's keys and values in its own L2.
+__device__ inline void block_of(unsigned w, int per_unit, int units, int& unit, int& block) {
+  if (units % 8 == 0) {
+    const int xcd = w & 7, slot = w >> 3;
+    unit = (slot / per_unit) * 8 + xcd;
+    block = slot % per_unit;
+  } else {
+    unit = w / per_unit;
+    block = w % per_unit;
+  }
+}
+
+// biases of head h by distance, times log2(e), padded on both sides
+__device__ inline void fill_table(float* table, const Args& A, int h, int tid, int nthreads) {
+  const int top = 2 * A.reach;
+  for (int i = tid; i <= top + 2 * kPad; i += nthreads) table[i] = A.bias[(long long)h * A.buckets + A.bucket_of[clampi(i - kPad, 0, top)]] * kLog2e;
+}
+
+template <class T> __device__ inline const T* rows_of(const void* p, const int64_t* s, int b, int h) { return (const T*)p + (long long)b * s[0] + (long long)h * s[1]; }
+template <class T> __device__ inline T* rows_of(void* p, const int64_t* s, int b, int h) { return (T*)p + (long long)b * s[0] + (long long)h * s[1]; }
+
+template <class Tc> constexpr int key_tile() { return sizeof(Tc) == 2 ? 64 : 32; }
+
+// logits (base 2) of a 32 x 32 tile in place: rows are keys kb + 8g + 4 half + t, the lane's column is the query at position pos
+__device__ inline void add_bias_by_key(f32x16& s, float scale2, const float* table, int kb, int pos, int half, int kind, float far, int reach) {
+  if (kind == 0) {
+    const float* tp = table + (kb - pos + reach + kPad + 4 * half);
+#pragma unroll
+    for (int r = 0; r < 16; r++) s[r] = fmaf(s[r], scale2, tp[8 * (r / 4) + r % 4]);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; r++) s[r] = fmaf(s[r], scale2, far);
+  }
+}
+
+// ---- forward --------------------------------------------------------------------------------------------------------------
+//
+// One pass over the keys with a running maximum and sum.  A workgroup of four wavefronts has 128 queries of one head, a
+// wavefront 32 of them, one to a lane pair; tiles of 64 keys (32 in float32) are staged in LDS, double buffered, one barrier a
+// tile.  The logits are computed transposed (rows keys, columns queries), so a query's maximum and sum are in-lane reductions
+// and one exchange between the halves, and the probabilities enter the product with the values as they are (keops_seq.h).
+template <class Tin, class Tc, int DP>
+__global__ void __launch_bounds__(256, 2) attention_forward(const Args A) {
+  constexpr int KT = key_tile<Tc>(), ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32, SUB = KT / 32;
+  extern __shared__ __align__(16) unsigned char smem[];
+  Tc* const tiles = (Tc*)smem;  // [2][keys, values][KT][ST]
+  float* const table = (float*)(tiles + 4 * KT * ST);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int group = A.heads / A.kv_heads, M = (int)A.queries, nqb = (M + 127) / 128;
+  int unit, block;
+  block_of(blockIdx.x, group * nqb, A.batch * A.kv_heads, unit, block);
+  const int b = unit / A.kv_heads, kvh = unit % A.kv_heads, h = kvh * group + block / nqb, qb = nqb - 1 - block % nqb;
+  const Span sp = span_of(A, b);
+  fill_table(table, A, h, tid, 256);
+
+  const int row = qb * 128 + wave * 32 + col, pos = sp.start + row;
+  const int pos_lo = sp.start + qb * 128 + wave * 32, pos_hi = pos_lo + 31;
+  const Tin* const K = rows_of<Tin>(A.k, A.k_stride, b, kvh);
+  const Tin* const V = rows_of<Tin>(A.v, A.v_stride, b, kvh);
+  typename Vec<Tc>::x8 qf[NS];
+  {
+    const Tin* q = rows_of<Tin>(A.q, A.q_stride, b, h) + (long long)row * A.q_stride[2];
+#pragma unroll
+    for (int i = 0; i < NS; i++) qf[i] = frag_global<Tin, Tc>(q, row < M, 16 * i, half, A.dim);
+  }
+  int kend = sp.klen;
+  if (A.causal) kend = min(kend, sp.start + min(qb * 128 + 128, M));
+  const int ntiles = kend > 0 ? (kend + KT - 1) / KT : 0;
+  const int lim = A.causal ? min(sp.klen, pos + 1) : sp.klen;
+  const float scale2 = A.scale * kLog2e;
+
+  f32x16 acc[ND];
+#pragma unroll
+  for (int i = 0; i < ND; i++) acc[i] = zero16();
+  float m = -kInf, l = 0.f;
+
+  Staged<Tin, Tc, KT, DP> sk, sv;
+  if (ntiles > 0) {
+    sk.load(K, A.k_stride[2], 0, sp.klen, A.dim, tid);
+    sv.load(V, A.v_stride[2], 0, sp.klen, A.dim, tid);
+    sk.store(tiles, tid);
+    sv.store(tiles + KT * ST, tid);
+    if (ntiles > 1) {
+      sk.load(K, A.k_stride[2], KT, sp.klen, A.dim, tid);
+      sv.load(V, A.v_stride[2], KT, sp.klen, A.dim, tid);
+    }
+  }
+  __syncthreads();
+  const float left = table[0], right = table[2 * A.reach + 2 * kPad];
+  for (int t = 0; t < ntiles; t++) {
+    const Tc* kt = tiles + (t & 1) * 2 * KT * ST;
+    const Tc* vt = kt + KT * ST;
+    if (t + 1 < ntiles) {
+      Tc* nx = tiles + ((t + 1) & 1) * 2 * KT * ST;
+      sk.store(nx, tid);
+      sv.store(nx + KT * ST, tid);
+      if (t + 2 < ntiles) {
+        sk.load(K, A.k_stride[2], (t + 2) * KT, sp.klen, A.dim, tid);
+        sv.load(V, A.v_stride[2], (t + 2) * KT, sp.klen, A.dim, tid);
+      }
+    }
+    const int kb = t * KT;
+    if (!A.causal || kb <= pos_hi) {
+      f32x16 s[SUB];
+#pragma unroll
+      for (int u = 0; u < SUB; u++) {
+        s[u] = zero16();
+#pragma unroll
+        for (int i = 0; i < NS; i++) s[u] = mma(frag_rows(kt + (32 * u + col) * ST, 16 * i, half), qf[i], s[u]);
+      }
+      const int kind = kb - pos_hi >= A.reach ? 1 : (kb + KT - 1 - pos_lo <= -A.reach ? -1 : 0);
+#pragma unroll
+      for (int u = 0; u < SUB; u++) add_bias_by_key(s[u], scale2, table, kb + 32 * u, pos, half, kind, kind > 0 ? right : left, A.reach);
+      if (kb + KT > sp.klen || (A.causal && kb + KT - 1 > pos_lo)) {
+        const int rel = lim - kb - 4 * half;
+#pragma unroll
+        for (int u = 0; u < SUB; u++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) s[u][r] = 32 * u + 8 * (r / 4) + r % 4 < rel ? s[u][r] : -kInf;
+      }
+      float mx = s[0][0];
+#pragma unroll
+      for (int u = 0; u < SUB; u++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[u][r]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      // the reference point moves only when a logit exceeds it by more than 8 (probabilities up to 2^8 lose nothing: the sum is
+      // kept in float32 and 16-bit operands have the same relative step there)
+      if (__any(mx > m + 8.f)) {
+        const float mn = fmaxf(m, mx), alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+#pragma unroll
+        for (int i = 0; i < ND; i++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) acc[i][r] *= alpha;
+        l *= alpha;
+        m = mn;
+      }
+      const float ms = m == -kInf ? 0.f : m;
+#pragma unroll
+      for (int u = 0; u < SUB; u++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          s[u][r] = __builtin_amdgcn_exp2f(s[u][r] - ms);
+          l += s[u][r];
+        }
+      // probabilities rounded to the values' type for the product (2^-9 relative for bf16, as much as the output's own rounding)
+#pragma unroll
+      for (int u = 0; u < SUB; u++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const typename Vec<Tc>::x8 p = pack<Tc>(s[u], k);
+#pragma unroll
+          for (int i = 0; i < ND; i++) acc[i] = mma(frag_cols<Tc>(vt, ST, 32 * u + 16 * k, 32 * i, lane), p, acc[i]);
+        }
+    }
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32);
+  if (row < M) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    Tin* o = rows_of<Tin>(A.out, A.out_stride, b, h) + (long long)row * A.out_stride[2];
+#pragma unroll
+    for (int i = 0; i < ND; i++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int d = 32 * i + 8 * g + 4 * half;
+        if (d < A.dim) store4<Tin>(o + d, acc[i][4 * g] * inv, acc[i][4 * g + 1] * inv, acc[i][4 * g + 2] * inv, acc[i][4 * g + 3] * inv);
+      }
+    // base-2 log of the row's sum; a row that sees nothing gets +inf, with which its probabilities are zeros later
+    if (A.lse && half == 0) A.lse[((long long)b * A.heads + h) * M + row] = l == 0.f ? kInf : m + __builtin_amdgcn_logf(l);
+  }
+}
+
+// ---- few queries ----------------------------------------------------------------------------------------------------------
+//
+// At most 32 rows (queries times heads that share a key/value head): every wavefront holds them all and takes every fourth tile
+// of 32 keys of its share of the sequence; keys go from memory to registers as operands, values through the wavefront's own
+// piece of LDS for the transposing read.  Shares of a long sequence go to different workgroups, which leave their sums for
+// attention_join.
+template <class Tin, class Tc, int DP>
+__global__ void __launch_bounds__(256, 2) attention_rows(const Args A, int splits, float* part) {
+  constexpr int ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32, VE = 16 / (int)sizeof(Tin), PER_ROW = DP / VE, NV = 32 * PER_ROW / 64;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  Tc* const vt = (Tc*)smem + wave * 32 * ST;
+  const int group = A.heads / A.kv_heads, M = (int)A.queries, rows = group * M;
+  const int unit = blockIdx.x / splits, split = blockIdx.x % splits, b = unit / A.kv_heads, kvh = unit % A.kv_heads;
+  const Span sp = span_of(A, b);
+  const int h = kvh * group + col / M, qi = col % M;
+  const bool there = col < rows;
+  const int pos = sp.start + qi;
+  int kend = sp.klen;
+  if (A.causal) kend = min(kend, sp.start + M);
+  if (kend < 0) kend = 0;
+  const int share = ((kend + splits - 1) / splits + 127) / 128 * 128, k0 = min(split * share, kend), k1 = min(k0 + share, kend);
+  const Tin* const K = rows_of<Tin>(A.k, A.k_stride, b, kvh);
+  const Tin* const V = rows_of<Tin>(A.v, A.v_stride, b, kvh);
+  typename Vec<Tc>::x8 qf[NS];
+  {
+    const Tin* q = rows_of<Tin>(A.q, A.q_stride, b, there ? h : 0) + (long long)qi * A.q_stride[2];
+#pragma unroll
+    for (int i = 0; i < NS; i++) qf[i] = frag_global<Tin, Tc>(q, there, 16 * i, half, A.dim);
+  }
+  const float* const bias = A.bias + (long long)(there ? h : 0) * A.buckets;
+  const float left = bias[A.bucket_of[0]] * kLog2e, right = bias[A.bucket_of[2 * A.reach]] * kLog2e;
+  const int lim = A.causal ? min(sp.klen, pos + 1) : sp.klen, pos_lo = sp.start, pos_hi = sp.start + M - 1;
+  const float scale2 = A.scale * kLog2e;
+  f32x16 acc[ND];
+#pragma unroll
+  for (int i = 0; i < ND; i++) acc[i] = zero16();
+  float m = -kInf, l = 0.f;
+
+  typename Vec<Tc>::x8 kf[NS];
+  uint4 vr[NV];
+  auto fetch = [&](int kb) {
+    const int key = kb + col;
+    const Tin* kp = K + (long long)key * A.k_stride[2];
+#pragma unroll
+    for (int i = 0; i < NS; i++) kf[i] = frag_global<Tin, Tc>(kp, key < k1, 16 * i, half, A.dim);
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int c = lane + 64 * i, r = kb + c / PER_ROW, d = (c % PER_ROW) * VE;
+      vr[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < k1 && d < A.dim) vr[i] = *reinterpret_cast<const uint4*>(V + (long long)r * A.v_stride[2] + d);
+    }
+  };
+  const int first = k0 + 32 * wave;
+  if (first < k1) fetch(first);
+  for (int kb = first; kb < k1; kb += 128) {
+    f32x16 s = zero16();
+#pragma unroll
+    for (int i = 0; i < NS; i++) s = mma(kf[i], qf[i], s);
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int c = lane + 64 * i;
+      Tc* dst = vt + (c / PER_ROW) * ST + (c % PER_ROW) * VE;
+      if constexpr (sizeof(Tin) == sizeof(Tc)) {
+        *reinterpret_cast<uint4*>(dst) = vr[i];
+      } else {
+        union { uint4 u; Tin e[VE]; } x;
+        x.u = vr[i];
+#pragma unroll
+        for (int j = 0; j < VE; j++) dst[j] = (Tc)x.e[j];
+      }
+    }
+    if (kb + 128 < k1) fetch(kb + 128);
+    if (kb - pos_hi >= A.reach || kb + 31 - pos_lo <= -A.reach) {
+      const float far = kb - pos_hi >= A.reach ? right : left;
+#pragma unroll
+      for (int r = 0; r < 16; r++) s[r] = fmaf(s[r], scale2, far);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int rel = clampi(kb + c_row(r, half) - pos, -A.reach, A.reach);
+        s[r] = fmaf(s[r], scale2, bias[A.bucket_of[rel + A.reach]] * kLog2e);
+      }
+    }
+    float mx = -kInf;
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      s[r] = kb + c_row(r, half) < min(lim, k1) ? s[r] : -kInf;
+      mx = fmaxf(mx, s[r]);
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    if (__any(mx > m + 8.f)) {
+      const float mn = fmaxf(m, mx), alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+#pragma unroll
+      for (int i = 0; i < ND; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[i][r] *= alpha;
+      l *= alpha;
+      m = mn;
+    }
+    const float ms = m == -kInf ? 0.f : m;
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      s[r] = __builtin_amdgcn_exp2f(s[r] - ms);
+      l += s[r];
+    }
+    // the wavefront's own stores to its piece of LDS come before its reads of it
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const typename Vec<Tc>::x8 p = pack<Tc>(s, k);
+#pragma unroll
+      for (int i = 0; i < ND; i++) acc[i] = mma(frag_cols<Tc>(vt, ST, 16 * k, 32 * i, lane), p, acc[i]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+  l += __shfl_xor(l, 32);
+  // the four wavefronts' sums, joined in their order
+  __syncthreads();
+  float* const o4 = (float*)smem;             // [4][rows][DP]
+  float* const ml = o4 + 4 * rows * DP;       // [4][rows][2]
+  if (there) {
+#pragma unroll
+    for (int i = 0; i < ND; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) o4[(wave * rows + col) * DP + 32 * i + c_row(r, half)] = acc[i][r];
+    if (half == 0) {
+      ml[(wave * rows + col) * 2] = m;
+      ml[(wave * rows + col) * 2 + 1] = l;
+    }
+  }
+  __syncthreads();
+  for (int e = tid; e < rows * DP; e += 256) {
+    const int r = e / DP, d = e % DP;
+    float mm = -kInf, ll = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) mm = fmaxf(mm, ml[(w * rows + r) * 2]);
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float mw = ml[(w * rows + r) * 2], a = mw == mm ? 1.f : __builtin_amdgcn_exp2f(mw - mm);
+      ll += a * ml[(w * rows + r) * 2 + 1];
+      o += a * o4[(w * rows + r) * DP + d];
+    }
+    const int hr = kvh * group + r / M, qr = r % M;
+    if (splits == 1) {
+      if (d < A.dim) rows_of<Tin>(A.out, A.out_stride, b, hr)[(long long)qr * A.out_stride[2] + d] = (Tin)(ll == 0.f ? 0.f : o / ll);
+      if (A.lse && d == 0) A.lse[((long long)b * A.heads + hr) * M + qr] = ll == 0.f ? kInf : mm + __builtin_amdgcn_logf(ll);
+    } else {
+      float* p = part + ((long long)blockIdx.x * rows + r) * (DP + 2);
+      p[2 + d] = o;
+      if (d == 0) {
+        p[0] = mm;
+        p[1] = ll;
+      }
+    }
+  }
+}
+
+// the shares of one row, joined in their order
+template <class Tin> __global__ void __launch_bounds__(128) attention_join(const Args A, int splits, int dp, const float* part) {
+  const int group = A.heads / A.kv_heads, M = (int)A.queries, rows = group * M;
+  const int unit = blockIdx.x / rows, r = blockIdx.x % rows, b = unit / A.kv_heads, h = (unit % A.kv_heads) * group + r / M, qi = r % M;
+  const float* p = part + ((long long)unit * splits * rows + r) * (dp + 2);
+  const long long step = (long long)rows * (dp + 2);
+  float mm = -kInf;
+  for (int s = 0; s < splits; s++) mm = fmaxf(mm, p[s * step]);
+  float ll = 0.f, o = 0.f;
+  const int d = threadIdx.x;
+  for (int s = 0; s < splits; s++) {
+    const float ms = p[s * step], a = ms == mm ? 1.f : __builtin_amdgcn_exp2f(ms - mm);
+    ll += a * p[s * step + 1];
+    if (d < A.dim) o += a * p[s * step + 2 + d];
+  }
+  if (d < A.dim) rows_of<Tin>(A.out, A.out_stride, b, h)[(long long)qi * A.out_stride[2] + d] = (Tin)(ll == 0.f ? 0.f : o / ll);
+  if (A.lse && d == 0) A.lse[((long long)b * A.heads + h) * M + qi] = ll == 0.f ? kInf : mm + __builtin_amdgcn_logf(ll);
+}
+
+// ---- gradient of the queries ------------------------------------------------------------------------------------------------
+//
+// P = exp2(z - lse), dP = dO V^T, dS = P (dP - delta), dq = scale dS K, laid out as in the forward pass.  delta_i = sum_j P_ij dP_ij
+// equals <dO_i, o_i>, but the stored output is rounded and came from rounded probabilities, and the bias gradient sums rows whose
+// exact sum is zero: a delta off by 2^-9 of itself would be most of a far bucket's gradient in a long row.  So dS is formed with
+// <dO_i, o_i>, and the row sums of that dS, which are what delta is off by, are added to the delta that the gradient of keys,
+// values and biases uses.
+template <class Tin, class Tc, int DP>
+__global__ void __launch_bounds__(256, 2) attention_grad_q(const Args A) {
+  constexpr int KT = key_tile<Tc>(), ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32, SUB = KT / 32;
+  extern __shared__ __align__(16) unsigned char smem[];
+  Tc* const tiles = (Tc*)smem;
+  float* const table = (float*)(tiles + 4 * KT * ST);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int group = A.heads / A.kv_heads, M = (int)A.queries, nqb = (M + 127) / 128;
+  int unit, block;
+  block_of(blockIdx.x, group * nqb, A.batch * A.kv_heads, unit, block);
+  const int b = unit / A.kv_heads, kvh = unit % A.kv_heads, h = kvh * group + block / nqb, qb = nqb - 1 - block % nqb;
+  const Span sp = span_of(A, b);
+  fill_table(table, A, h, tid, 256);
+
+  const int row = qb * 128 + wave * 32 + col, pos = sp.start + row;
+  const int pos_lo = sp.start + qb * 128 + wave * 32, pos_hi = pos_lo + 31;
+  const Tin* const K = rows_of<Tin>(A.k, A.k_stride, b, kvh);
+  const Tin* const V = rows_of<Tin>(A.v, A.v_stride, b, kvh);
+  typename Vec<Tc>::x8 qf[NS], gf[NS];
+  float delta = 0.f;
+  {
+    const Tin* q = rows_of<Tin>(A.q, A.q_stride, b, h) + (long long)row * A.q_stride[2];
+    const Tin* g = rows_of<Tin>(A.grad_out, A.grad_out_stride, b, h) + (long long)row * A.grad_out_stride[2];
+    const Tin* o = rows_of<Tin>(A.out, A.out_stride, b, h) + (long long)row * A.out_stride[2];
+#pragma unroll
+    for (int i = 0; i < NS; i++) {
+      qf[i] = frag_global<Tin, Tc>(q, row < M, 16 * i, half, A.dim);
+      gf[i] = frag_global<Tin, Tc>(g, row < M, 16 * i, half, A.dim);
+      const typename Vec<Tc>::x8 of = frag_global<Tin, Tc>(o, row < M, 16 * i, half, A.dim);
+#pragma unroll
+      for (int j = 0; j < 8; j++) delta = fmaf((float)gf[i][j], (float)of[j], delta);
+    }
+    delta += __shfl_xor(delta, 32);
+  }
+  const long long stat = ((long long)b * A.heads + h) * M + row;
+  const float lse = row < M ? A.lse[stat] : kInf;
+  int kend = sp.klen;
+  if (A.causal) kend = min(kend, sp.start + min(qb * 128 + 128, M));
+  const int ntiles = kend > 0 ? (kend + KT - 1) / KT : 0;
+  const int lim = A.causal ? min(sp.klen, pos + 1) : sp.klen;
+  const float scale2 = A.scale * kLog2e;
+
+  f32x16 acc[ND];
+#pragma unroll
+  for (int i = 0; i < ND; i++) acc[i] = zero16();
+  float over = 0.f;
+
+  Staged<Tin, Tc, KT, DP> sk, sv;
+  if (ntiles > 0) {
+    sk.load(K, A.k_stride[2], 0, sp.klen, A.dim, tid);
+    sv.load(V, A.v_stride[2], 0, sp.klen, A.dim, tid);
+    sk.store(tiles, tid);
+    sv.store(tiles + KT * ST, tid);
+    if (ntiles > 1) {
+      sk.load(K, A.k_stride[2], KT, sp.klen, A.dim, tid);
+      sv.load(V, A.v_stride[2], KT, sp.klen, A.dim, tid);
+    }
+  }
+  __syncthreads();
+  const float left = table[0], right = table[2 * A.reach + 2 * kPad];
+  for (int t = 0; t < ntiles; t++) {
+    const Tc* kt = tiles + (t & 1) * 2 * KT * ST;
+    const Tc* vt = kt + KT * ST;
+    if (t + 1 < ntiles) {
+      Tc* nx = tiles + ((t + 1) & 1) * 2 * KT * ST;
+      sk.store(nx, tid);
+      sv.store(nx + KT * ST, tid);
+      if (t + 2 < ntiles) {
+        sk.load(K, A.k_stride[2], (t + 2) * KT, sp.klen, A.dim, tid);
+        sv.load(V, A.v_stride[2], (t + 2) * KT, sp.klen, A.dim, tid);
+      }
+    }
+    const int kb = t * KT;
+    if (!A.causal || kb <= pos_hi) {
+      const int kind = kb - pos_hi >= A.reach ? 1 : (kb + KT - 1 - pos_lo <= -A.reach ? -1 : 0);
+      const bool mask = kb + KT > sp.klen || (A.causal && kb + KT - 1 > pos_lo);
+      const int rel = lim - kb - 4 * half;
+#pragma unroll
+      for (int u = 0; u < SUB; u++) {
+        f32x16 s = zero16(), p = zero16();
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+          s = mma(frag_rows(kt + (32 * u + col) * ST, 16 * i, half), qf[i], s);
+          p = mma(frag_rows(vt + (32 * u + col) * ST, 16 * i, half), gf[i], p);
+        }
+        add_bias_by_key(s, scale2, table, kb + 32 * u, pos, half, kind, kind > 0 ? right : left, A.reach);
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          float e = __builtin_amdgcn_exp2f(s[r] - lse);
+          if (mask) e = 32 * u + 8 * (r / 4) + r % 4 < rel ? e : 0.f;
+          s[r] = e * (p[r] - delta);
+          over += s[r];
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const typename Vec<Tc>::x8 ds = pack<Tc>(s, k);
+#pragma unroll
+          for (int i = 0; i < ND; i++) acc[i] = mma(frag_cols<Tc>(kt, ST, 32 * u + 16 * k, 32 * i, lane), ds, acc[i]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  over += __shfl_xor(over, 32);
+  if (row < M) {
+    if (half == 0) A.delta[stat] = delta + over;
+    if (A.grad_q) {
+      Tin* o = rows_of<Tin>(A.grad_q, A.grad_q_stride, b, h) + (long long)row * A.grad_q_stride[2];
+#pragma unroll
+      for (int i = 0; i < ND; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          const int d = 32 * i + 8 * g + 4 * half;
+          if (d < A.dim)
+            store4<Tin>(o + d, acc[i][4 * g] * A.scale, acc[i][4 * g + 1] * A.scale, acc[i][4 * g + 2] * A.scale, acc[i][4 * g + 3] * A.scale);
+        }
+    }
+  }
+}
+
+// ---- gradients of keys, values and biases -----------------------------------------------------------------------------------
+//
+// A workgroup has 128 keys of one key/value head, a wavefront 32 of them as columns, and walks over the queries of all heads that
+// share them, so nothing is added by two workgroups and no order of additions is left to chance.  Biases: pairs beyond the reach
+// add to one sum a side; a 32 x 32 tile within it is summed along its 63 diagonals (each distance is one: lanes are rotated by the
+// register's row, so that equal distances meet in a lane) into a table by distance that belongs to the wavefront, and the tables
+// become sums by bucket when the head is done.
+template <class Tin, class Tc, int DP>
+__global__ void __launch_bounds__(256, 1) attention_grad_kv(const Args A, float* part) {
+  constexpr int QT = key_tile<Tc>(), ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32, SUB = QT / 32;
+  extern __shared__ __align__(16) unsigned char smem[];
+  Tc* const tiles = (Tc*)smem;                          // [2][queries, output gradients][QT][ST]
+  float* const stats = (float*)(tiles + 4 * QT * ST);   // [2][lse, delta][QT]
+  const int tlen = 2 * A.reach + 1 + 2 * kPad;
+  float* const table = stats + 4 * QT;
+  float* const sums = table + tlen;                     // [4][tlen]
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int group = A.heads / A.kv_heads, M = (int)A.queries, N = (int)A.keys, nkb = (N + 127) / 128;
+  int unit, kblock;
+  block_of(blockIdx.x, nkb, A.batch * A.kv_heads, unit, kblock);
+  const int b = unit / A.kv_heads, kvh = unit % A.kv_heads;
+  const Span sp = span_of(A, b);
+  const int kb = kblock * 128 + wave * 32, key = kb + col;
+  const bool want_bias = part != nullptr;
+  typename Vec<Tc>::x8 kf[NS], vf[NS];
+  {
+    const Tin* k = rows_of<Tin>(A.k, A.k_stride, b, kvh) + (long long)key * A.k_stride[2];
+    const Tin* v = rows_of<Tin>(A.v, A.v_stride, b, kvh) + (long long)key * A.v_stride[2];
+#pragma unroll
+    for (int i = 0; i < NS; i++) {
+      kf[i] = frag_global<Tin, Tc>(k, key < sp.klen, 16 * i, half, A.dim);
+      vf[i] = frag_global<Tin, Tc>(v, key < sp.klen, 16 * i, half, A.dim);
+    }
+  }
+  f32x16 dk[ND], dv[ND];
+#pragma unroll
+  for (int i = 0; i < ND; i++) {
+    dk[i] = zero16();
+    dv[i] = zero16();
+  }
+  const float scale2 = A.scale * kLog2e;
+  // first query tile that can see a key of this workgroup
+  int q_first = 0;
+  if (A.causal) q_first = max(0, kblock * 128 - sp.start) / QT * QT;
+  const int q_end = kblock * 128 < sp.klen ? M : 0;
+  const int ntiles = q_end > q_first ? (q_end - q_first + QT - 1) / QT : 0;
+
+  for (int g = 0; g < group; g++) {
+    const int h = kvh * group + g;
+    const Tin* const Q = rows_of<Tin>(A.q, A.q_stride, b, h);
+    const Tin* const G = rows_of<Tin>(A.grad_out, A.grad_out_stride, b, h);
+    const float* const lse = A.lse + ((long long)b * A.heads + h) * M;
+    const float* const del = A.delta + ((long long)b * A.heads + h) * M;
+    float far_left = 0.f, far_right = 0.f;
+    Staged<Tin, Tc, QT, DP> sq, sg;
+    float s_lse = kInf, s_del = 0.f;
+    auto fetch = [&](int q0) {
+      sq.load(Q, A.q_stride[2], q0, M, A.dim, tid);
+      sg.load(G, A.grad_out_stride[2], q0, M, A.dim, tid);
+      if (tid < QT) {
+        s_lse = q0 + tid < M ? lse[q0 + tid] : kInf;
+        s_del = q0 + tid < M ? del[q0 + tid] : 0.f;
+      }
+    };
+    auto put = [&](int buf) {
+      sq.store(tiles + buf * 2 * QT * ST, tid);
+      sg.store(tiles + buf * 2 * QT * ST + QT * ST, tid);
+      if (tid < QT) {
+        stats[buf * 2 * QT + tid] = s_lse;
+        stats[buf * 2 * QT + QT + tid] = s_del;
+      }
+    };
+    fill_table(table, A, h, tid, 256);
+    if (want_bias)
+      for (int i = tid; i < 4 * tlen; i += 256) sums[i] = 0.f;
+    if (ntiles > 0) {
+      fetch(q_first);
+      put(0);
+      if (ntiles > 1) fetch(q_first + QT);
+    }
+    __syncthreads();
+    const float left = table[0], right = table[tlen - 1];
+    for (int t = 0; t < ntiles; t++) {
+      const Tc* qt = tiles + (t & 1) * 2 * QT * ST;
+      const Tc* gt = qt + QT * ST;
+      const float* st = stats + (t & 1) * 2 * QT;
+      if (t + 1 < ntiles) {
+        put((t + 1) & 1);
+        if (t + 2 < ntiles) fetch(q_first + (t + 2) * QT);
+      }
+#pragma unroll
+      for (int u = 0; u < SUB; u++) {
+        const int q0 = q_first + t * QT + 32 * u, pos0 = sp.start + q0;  // position of the tile's first query
+        if (kb >= sp.klen || (A.causal && kb > pos0 + 31)) continue;     // nothing in this wavefront's tile
+        f32x16 s = zero16(), p = zero16();
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+          s = mma(frag_rows(qt + (32 * u + col) * ST, 16 * i, half), kf[i], s);
+          p = mma(frag_rows(gt + (32 * u + col) * ST, 16 * i, half), vf[i], p);
+        }
+        const int kind = kb - (pos0 + 31) >= A.reach ? 1 : (kb + 31 - pos0 <= -A.reach ? -1 : 0);
+        f32x16 e;
+        if (kind == 0) {
+          const float* tp = table + (key - pos0 - 4 * half + A.reach + kPad);
+#pragma unroll
+          for (int r = 0; r < 16; r++) e[r] = fmaf(s[r], scale2, tp[-(8 * (r / 4) + r % 4)]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; r++) e[r] = fmaf(s[r], scale2, kind > 0 ? right : left);
+        }
+#pragma unroll
+        for (int g4 = 0; g4 < 4; g4++) {
+          const f32x4 ls = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * g4 + 4 * half);
+          const f32x4 de = *reinterpret_cast<const f32x4*>(st + QT + 32 * u + 8 * g4 + 4 * half);
+#pragma unroll
+          for (int t4 = 0; t4 < 4; t4++) {
+            const int r = 4 * g4 + t4;
+            float x = __builtin_amdgcn_exp2f(e[r] - ls[t4]);
+            const int qpos = pos0 + 8 * g4 + 4 * half + t4;
+            if (key >= sp.klen || (A.causal && key > qpos)) x = 0.f;
+            e[r] = x;
+            s[r] = x * (p[r] - de[t4]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const typename Vec<Tc>::x8 pf = pack<Tc>(e, k), df = pack<Tc>(s, k);
+#pragma unroll
+          for (int i = 0; i < ND; i++) {
+            dv[i] = mma(frag_cols<Tc>(gt, ST, 32 * u + 16 * k, 32 * i, lane), pf, dv[i]);
+            dk[i] = mma(frag_cols<Tc>(qt, ST, 32 * u + 16 * k, 32 * i, lane), df, dk[i]);
+          }
+        }
+        if (want_bias) {
+          if (kind != 0) {
+            float x = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; r++) x += s[r];
+            if (kind > 0) far_right += x; else far_left += x;
+          } else {
+            // distance of (query row r, key col) is col - row + (kb - pos0): lane c of a half takes the value of key (c + row) % 32
+            float up = 0.f, down = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+              const int from = col + c_row(r, half);
+              const float x = __shfl(s[r], (from & 31) | (half << 5));
+              if (from < 32) up += x; else down += x;  // distance c, or c - 32
+            }
+            const float other = __shfl_xor(half ? up : down, 32);
+            const float mine = (half ? down : up) + other;
+            float* d = sums + wave * tlen + (kb - pos0 + A.reach + kPad + col - 32 * half);
+            *d += mine;
+          }
+        }
+      }
+      __syncthreads();
+    }
+    if (want_bias) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) {
+        far_left += __shfl_xor(far_left, o);
+        far_right += __shfl_xor(far_right, o);
+      }
+      __syncthreads();
+      if (lane == 0) {
+        sums[wave * tlen] += far_left;
+        sums[wave * tlen + tlen - 1] += far_right;
+      }
+      __syncthreads();
+      for (int i = tid; i < tlen; i += 256) table[i] = (sums[i] + sums[tlen + i]) + (sums[2 * tlen + i] + sums[3 * tlen + i]);
+      __syncthreads();
+      float* out = part + ((long long)(b * nkb + kblock) * A.heads + h) * A.buckets;
+      for (int bu = wave; bu < A.buckets; bu += 4) {
+        float x = 0.f;
+        for (int e = A.bucket_begin[bu] + lane; e < A.bucket_begin[bu + 1]; e += 64) {
+          const int d = A.bucket_order[e];  // 0 .. 2 reach
+          x += table[d + kPad];
+          if (d == 0)
+            for (int i = 0; i < kPad; i++) x += table[i];
+          if (d == 2 * A.reach)
+            for (int i = 0; i < kPad; i++) x += table[d + kPad + 1 + i];
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+        if (lane == 0) out[bu] = x;
+      }
+    }
+    __syncthreads();
+  }
+  if (key < N) {
+    Tin* ok = rows_of<Tin>(A.grad_k, A.grad_k_stride, b, kvh) + (long long)key * A.grad_k_stride[2];
+    Tin* ov = rows_of<Tin>(A.grad_v, A.grad_v_stride, b, kvh) + (long long)key * A.grad_v_stride[2];
+#pragma unroll
+    for (int i = 0; i < ND; i++)
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const int d = 32 * i + 8 * g + 4 * half;
+        if (d < A.dim) {
+          store4<Tin>(ok + d, dk[i][4 * g] * A.scale, dk[i][4 * g + 1] * A.scale, dk[i][4 * g + 2] * A.scale, dk[i][4 * g + 3] * A.scale);
+          store4<Tin>(ov + d, dv[i][4 * g], dv[i][4 * g + 1], dv[i][4 * g + 2], dv[i][4 * g + 3]);
+        }
+      }
+  }
+}
+
+// gradient of one bias: the workgroups' sums in their order
+__global__ void __launch_bounds__(256) attention_grad_bias(const float* part, float* out, int parts, int total) {
+  __shared__ double red[256];
+  double x = 0.0;
+  for (int i = threadIdx.x; i < parts; i += 256) x += (double)part[(long long)i * total + blockIdx.x];
+  red[threadIdx.x] = x;
+  __syncthreads();
+  for (int o = 128; o > 0; o >>= 1) {
+    if ((int)threadIdx.x < o) red[threadIdx.x] += red[threadIdx.x + o];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) out[blockIdx.x] = (float)red[0];
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------
+
+int padded_dim(int dim) { return dim <= 32 ? 32 : (dim <= 64 ? 64 : (dim <= 96 ? 96 : 128)); }
+
+const char* check(const Args* a) {
+  if (!a) return "bucket attention: null arguments";
+  if (a->dtype < 0 || a->dtype > 2) return "bucket attention: dtype must be 0 (bfloat16), 1 (float16) or 2 (float32)";
+  const int ve = a->dtype == 2 ? 4 : 8;
+  if (a->batch < 1 || a->heads < 1 || a->kv_heads < 1 || a->heads % a->kv_heads) return "bucket attention: heads must be a multiple of kv_heads";
+  if (a->dim < ve || a->dim > 128 || a->dim % ve) return "bucket attention: dim must be a multiple of 16 bytes, at most 128";
+  if (a->queries < 1 || a->queries > (1 << 29) || a->keys < 0 || a->keys > (1 << 29)) return "bucket attention: queries or keys out of range";
+  if (a->reach < 1 || a->reach > KEOPS_HIP_MAX_REACH || a->buckets < 1 || a->buckets > 2 * a->reach + 1) return "bucket attention: reach or number of buckets out of range";
+  if (a->start < -(1 << 29) || a->start > (1 << 29)) return "bucket attention: query_start out of range";
+  if (!a->q || !a->out || !a->bias || !a->bucket_of || (a->keys > 0 && (!a->k || !a->v))) return "bucket attention: null data";
+  const int64_t units = (int64_t)a->batch * a->heads;
+  if (units * ((a->queries + 127) / 128) > 0x7fffffff || units * ((a->keys + 127) / 128) > 0x7fffffff) return "bucket attention: too many workgroups";
+  return nullptr;
+}
+
+bool few_rows(const Args* a) { return a->queries * (a->heads / a->kv_heads) <= 32; }
+
+// Shares of the keys for few rows: enough workgroups for four on every CU, at least 256 keys to a share (two tiles a wavefront).
+int splits_of(const Args* a) {
+  const int64_t units = (int64_t)a->batch * a->kv_heads;
+  int64_t s = 1024 / units, most = a->keys / 256;
+  s = s < most ? s : most;
+  return (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
+}
+
+int tile_bytes(int dtype_bytes, int dp) {
+  const int kt = dtype_bytes == 2 ? 64 : 32;
+  return 4 * kt * (dp + 16 / dtype_bytes) * dtype_bytes;
+}
+int table_entries(const Args* a) { return 2 * a->reach + 1 + 2 * kPad; }
+
+template <class K> int prepare_lds(K kernel, size_t bytes) {
+  if (bytes <= 64 * 1024) return 0;
+  const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  return e == hipSuccess ? 0 : keops_seq_fail((int)e, "bucket attention: shared memory");
+}
+
+// fp16 in the gradients: dS is a product of small numbers that would fall below fp16's normal range, so these two passes compute
+// in float32
+template <class Tin, class Tc, class Tg, int DP> struct Passes {
+  static int forward(const Args& a, float* work, hipStream_t st) {
+    const int group = a.heads / a.kv_heads;
+    if (few_rows(&a)) {
+      const int rows = group * (int)a.queries, splits = splits_of(&a);
+      const size_t v = 4 * 32 * (size_t)tile_stride<Tc, DP>() * sizeof(Tc), o = 4 * (size_t)rows * (DP + 2) * 4, lds = v > o ? v : o;
+      if (int e = prepare_lds(attention_rows<Tin, Tc, DP>, lds)) return e;
+      attention_rows<Tin, Tc, DP><<<a.batch * a.kv_heads * splits, 256, lds, st>>>(a, splits, work);
+      if (splits > 1) attention_join<Tin><<<a.batch * a.kv_heads * rows, 128, 0, st>>>(a, splits, DP, work);
+    } else {
+      const size_t lds = tile_bytes(sizeof(Tc), DP) + 4 * (size_t)table_entries(&a);
+      if (int e = prepare_lds(attention_forward<Tin, Tc, DP>, lds)) return e;
+      const int nqb = (int)((a.queries + 127) / 128);
+      attention_forward<Tin, Tc, DP><<<a.batch * a.heads * nqb, 256, lds, st>>>(a);
+    }
+    return seq_launched("bucket attention: launch");
+  }
+  static int backward(const Args& a, float* work, hipStream_t st) {
+    const int nqb = (int)((a.queries + 127) / 128), nkb = (int)((a.keys + 127) / 128);
+    const size_t tb = tile_bytes(sizeof(Tg), DP), te = 4 * (size_t)table_entries(&a);
+    if (int e = prepare_lds(attention_grad_q<Tin, Tg, DP>, tb + te)) return e;
+    attention_grad_q<Tin, Tg, DP><<<a.batch * a.heads * nqb, 256, tb + te, st>>>(a);
+    if (nkb > 0) {
+      float* part = a.grad_bias ? work : nullptr;
+      const size_t lds = tb + 4 * key_tile<Tg>() * 4 + 5 * te;
+      if (int e = prepare_lds(attention_grad_kv<Tin, Tg, DP>, lds)) return e;
+      attention_grad_kv<Tin, Tg, DP><<<a.batch * a.kv_heads * nkb, 256, lds, st>>>(a, part);
+    }
+    if (a.grad_bias) attention_grad_bias<<<a.heads * a.buckets, 256, 0, st>>>(work, a.grad_bias, a.batch * nkb, a.heads * a.buckets);
+    return seq_launched("bucket attention: launch of the backward pass");
+  }
+};
+
+template <class Tin, class Tc, class Tg> int dispatch(const Args& a, bool backward, float* work, hipStream_t st) {
+  switch (padded_dim(a.dim)) {
+    case 32: return backward ? Passes<Tin, Tc, Tg, 32>::backward(a, work, st) : Passes<Tin, Tc, Tg, 32>::forward(a, work, st);
+    case 64: return backward ? Passes<Tin, Tc, Tg, 64>::backward(a, work, st) : Passes<Tin, Tc, Tg, 64>::forward(a, work, st);
+    case 96: return backward ? Passes<Tin, Tc, Tg, 96>::backward(a, work, st) : Passes<Tin, Tc, Tg, 96>::forward(a, work, st);
+    default: return backward ? Passes<Tin, Tc, Tg, 128>::backward(a, work, st) : Passes<Tin, Tc, Tg, 128>::forward(a, work, st);
+  }
+}
+
+int enter(const Args* a, bool backward, void* work, size_t work_bytes, int device, void* stream) {
+  if (const char* why = check(a)) return keops_seq_fail(-1, why);
+  if (backward && (!a->grad_out || !a->lse || !a->delta || (a->keys > 0 && (!a->grad_k || !a->grad_v)) || (a->grad_bias && (!a->bucket_order || !a->bucket_begin))))
+    return keops_seq_fail(-1, "bucket attention: null data for the backward pass");
+  const size_t need = backward ? keops_hip_bucket_attention_backward_bytes(a) : keops_hip_bucket_attention_forward_bytes(a);
+  if (need > work_bytes || (need > 0 && !work)) return keops_seq_fail(-1, "bucket attention: workspace too small");
+  SeqDevice on(device);
+  hipStream_t st = (hipStream_t)stream;
+  if (a->dtype == 0) return dispatch<bf16, bf16, bf16>(*a, backward, (float*)work, st);
+  if (a->dtype == 1) return dispatch<f16, f16, float>(*a, backward, (float*)work, st);
+  return dispatch<float, float, float>(*a, backward, (float*)work, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t keops_hip_bucket_attention_forward_bytes(const keops_hip_bucket_attention* a) {
+  if (check(a) || !few_rows(a) || splits_of(a) == 1) return 0;
+  const size_t rows = (size_t)(a->heads / a->kv_heads) * a->queries;
+  return (size_t)a->batch * a->kv_heads * splits_of(a) * rows * (padded_dim(a->dim) + 2) * sizeof(float);
+}
+
+size_t keops_hip_bucket_attention_backward_bytes(const keops_hip_bucket_attention* a) {
+  if (check(a) || !a->grad_bias) return 0;
+  return (size_t)a->batch * ((a->keys + 127) / 128) * a->heads * a->buckets * sizeof(float);
+}
+
+int keops_hip_bucket_attention_forward(const keops_hip_bucket_attention* a, void* work, size_t work_bytes, int device, void* hip_stream) {
+  return enter(a, false, work, work_bytes, device, hip_stream);
+}
+
+int keops_hip_bucket_attention_backward(const keops_hip_bucket_attention* a, void* work, size_t work_bytes, int device, void* hip_stream) {
+  return enter(a, true, work, work_bytes, device, hip_stream);
+}
+
+}  // extern "C"

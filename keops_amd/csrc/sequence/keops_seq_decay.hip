@@ -1,0 +1,450 @@
+// Linear attention with a decay for each head:  S_t = g S_{t-1} + k_t v_t^T,  o_t = scale q_t S_t,  and its gradients, which are
+// the same sum with the roles of the inputs exchanged (d = gradient of o):
+//   dq = A(d, v, k; S_0^T),   dk = A^rev(v, d, q; dS_T^T),   dv = A^rev(k, q, d; dS_T),   dS_0 = final state of the last one,
+// where A^rev walks from the last token to the first.  One kernel serves all of them.
+//
+// Chunks of 64 tokens: within a chunk the masked product (q k^T) o g^(i-j) times v, across chunks the state, so a token costs
+// 4 dim dim_v flop and 64 (dim + dim_v) more.  The state stays in the registers of the wavefronts, each of which has 32 of its
+// columns, as a C tile (keops_seq.h) that serves as an operand as it is.
+#include "../../../include/keops_hip.h"
+#include "keops_seq.h"
+
+using namespace kseq;
+
+namespace {
+
+typedef keops_hip_decay_attention Args;
+
+constexpr int C = 64;  // tokens of a chunk
+
+// x as a sum of NT terms of the operand's type; bf16: two terms hold 16 bits, three all 24 of a float32
+template <class T, int NT> struct Terms {
+  typename Vec<T>::x8 t[NT];
+  __device__ inline void set(const float (&x)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      float rest = x[j];
+#pragma unroll
+      for (int n = 0; n < NT; n++) {
+        const T e = (T)rest;
+        t[n][j] = e;
+        rest -= (float)e;
+      }
+    }
+  }
+};
+template <class Tc> constexpr int state_terms() { return sizeof(Tc) == 2 ? 2 : 1; }   // the state as an operand for the output
+template <class Tc> constexpr int update_terms() { return sizeof(Tc) == 2 ? 3 : 1; }  // decayed values as an operand for the state
+
+// powers of the decay in LDS: entry kZero + n holds g^n for n = 0..C, zeros before and behind
+constexpr int kZero = 64, kPowers = kZero + C + 8;
+__device__ inline float power(float log_decay, long long n) { return n == 0 ? 1.f : (float)exp((double)log_decay * (double)n); }
+__device__ inline void fill_powers(float* pw, float log_decay, int tid, int nt) {
+  for (int i = tid; i < kPowers; i += nt) pw[i] = i < kZero || i > kZero + C ? 0.f : power(log_decay, i - kZero);
+}
+
+template <class T> __device__ inline const T* rows_of(const void* p, const int64_t* s, int b, int h) { return (const T*)p + (long long)b * s[0] + (long long)h * s[1]; }
+
+__device__ inline int length_of(const Args& A, int b) {
+  const int t = (int)A.tokens;
+  if (!A.lengths) return t;
+  const int n = A.lengths[b];
+  return n < 0 ? 0 : (n > t ? t : n);
+}
+
+// S = g^n S + sum_j weight_j k_j v_j^T of the chunk in LDS (n tokens); wavefront's 32 columns of v
+template <class Tc, int DK, int DV>
+__device__ inline void update_state(f32x16 (&S)[DK / 32], const Tc* kt, const Tc* vt, const float* pw, int n, int shift, float scale, int wave, int lane) {
+  constexpr int SK = tile_stride<Tc, DK>(), SV = tile_stride<Tc, DV>(), NT = update_terms<Tc>();
+  const int half = lane >> 5;
+  const float all = pw[kZero + n];
+#pragma unroll
+  for (int i = 0; i < DK / 32; i++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) S[i][r] *= all;
+  const float* w = pw + kZero + n - 1 + shift - 4 * half;  // weight of token j is w[-j], zero behind the chunk's end
+#pragma unroll
+  for (int s = 0; s < C / 16; s++) {
+    const typename Vec<Tc>::x8 v = frag_cols<Tc>(vt, SV, 16 * s, 32 * wave, lane);
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) x[j] = (float)v[j] * (w[-(16 * s + (j & 3) + 2 * (j & 4))] * scale);
+    Terms<Tc, NT> t;
+    t.set(x);
+#pragma unroll
+    for (int i = 0; i < DK / 32; i++) {
+      const typename Vec<Tc>::x8 k = frag_cols<Tc>(kt, SK, 16 * s, 32 * i, lane);
+#pragma unroll
+      for (int m = 0; m < NT; m++) S[i] = mma(k, t.t[m], S[i]);
+    }
+  }
+}
+
+// ---- states at the ends of segments -------------------------------------------------------------------------------------------
+//
+// Few sequences and heads do not fill the chip, so a long sequence is cut into segments: their own states first (this kernel),
+// then decay_scan carries them on, then decay_outputs starts every segment from its state.
+template <class Tin, class Tc, int DK, int DV>
+__global__ void __launch_bounds__(2 * DV, 1) decay_states(const Args A, int segments, int seg_tokens, float* states) {
+  constexpr int NT = 2 * DV, SK = tile_stride<Tc, DK>(), SV = tile_stride<Tc, DV>();
+  extern __shared__ __align__(16) unsigned char smem[];
+  Tc* const kt = (Tc*)smem;
+  Tc* const vt = kt + C * SK;
+  float* const pw = (float*)(vt + C * SV);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int unit = blockIdx.x / segments, seg = blockIdx.x % segments, b = unit / A.heads, h = unit % A.heads;
+  const int len = length_of(A, b), t0 = seg * seg_tokens, t1 = min(len, t0 + seg_tokens);
+  fill_powers(pw, A.log_decay[h], tid, NT);
+  const Tin* k = rows_of<Tin>(A.k, A.k_stride, b, h / (A.heads / A.k_heads));
+  const Tin* v = rows_of<Tin>(A.v, A.v_stride, b, h / (A.heads / A.v_heads));
+  long long ks = A.k_stride[2], vs = A.v_stride[2];
+  if (A.reverse && len > 0) {
+    k += (long long)(len - 1) * ks; ks = -ks;
+    v += (long long)(len - 1) * vs; vs = -vs;
+  }
+  f32x16 S[DK / 32];
+#pragma unroll
+  for (int i = 0; i < DK / 32; i++) S[i] = zero16();
+  Staged<Tin, Tc, C, DK, NT> sk;
+  Staged<Tin, Tc, C, DV, NT> sv;
+  if (t0 < t1) {
+    sk.load(k, ks, t0, t1, A.dim, tid);
+    sv.load(v, vs, t0, t1, A.dim_v, tid);
+  }
+  for (int t = t0; t < t1; t += C) {
+    __syncthreads();
+    sk.store(kt, tid);
+    sv.store(vt, tid);
+    __syncthreads();
+    if (t + C < t1) {
+      sk.load(k, ks, t + C, t1, A.dim, tid);
+      sv.load(v, vs, t + C, t1, A.dim_v, tid);
+    }
+    update_state<Tc, DK, DV>(S, kt, vt, pw, min(C, t1 - t), A.reverse, A.update_scale, wave, lane);
+  }
+  float* out = states + (long long)blockIdx.x * A.dim * A.dim_v;
+  const int c = 32 * wave + col;
+#pragma unroll
+  for (int i = 0; i < DK / 32; i++)
+#pragma unroll
+    for (int r = 0; r < 16; r++) {
+      const int d = 32 * i + c_row(r, half);
+      if (d < A.dim && c < A.dim_v) out[(long long)d * A.dim_v + c] = S[i][r];
+    }
+}
+
+// states before the segments in place of the segments' own, and the final state
+__global__ void __launch_bounds__(256) decay_scan(const Args A, int segments, int seg_tokens, float* states) {
+  const int unit = blockIdx.y, b = unit / A.heads, h = unit % A.heads, size = A.dim * A.dim_v;
+  const int e = blockIdx.x * 256 + threadIdx.x;
+  if (e >= size) return;
+  const int d = e / A.dim_v, c = e % A.dim_v, len = length_of(A, b);
+  const float lg = A.log_decay[h], whole = power(lg, seg_tokens);
+  float x = A.state_in ? A.state_in[(long long)unit * size + d * A.state_in_stride[0] + c * A.state_in_stride[1]] : 0.f;
+  float* s = states + (long long)unit * segments * size + e;
+  for (int g = 0; g < segments; g++) {
+    const int n = min(max(len - g * seg_tokens, 0), seg_tokens);
+    const float own = s[(long long)g * size];
+    s[(long long)g * size] = x;
+    x = (n == seg_tokens ? whole : power(lg, n)) * x + own;
+  }
+  if (A.state_out) A.state_out[(long long)unit * size + d * A.state_out_stride[0] + c * A.state_out_stride[1]] = x;
+}
+
+// ---- outputs --------------------------------------------------------------------------------------------------------------------
+template <class Tin, class Tc, int DK, int DV>
+__global__ void __launch_bounds__(2 * DV, 1) decay_outputs(const Args A, int segments, int seg_tokens, const float* states) {
+  constexpr int NT = 2 * DV, NW = DV / 32, SK = tile_stride<Tc, DK>(), SV = tile_stride<Tc, DV>(), SP = tile_stride<Tc, C>();
+  extern __shared__ __align__(16) unsigned char smem[];
+  Tc* const qt = (Tc*)smem;
+  Tc* const kt = qt + C * SK;
+  Tc* const vt = kt + C * SK;
+  Tc* const pt = vt + C * SV;
+  float* const pw = (float*)(pt + C * SP);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int unit = blockIdx.x / segments, seg = blockIdx.x % segments, b = unit / A.heads, h = unit % A.heads;
+  const int len = length_of(A, b), t0 = seg * seg_tokens, t1 = min(len, t0 + seg_tokens);
+  const int c = 32 * wave + col, shift = A.reverse ? 0 : 1;
+  fill_powers(pw, A.log_decay[h], tid, NT);
+  const Tin* q = rows_of<Tin>(A.q, A.q_stride, b, h / (A.heads / A.q_heads));
+  const Tin* k = rows_of<Tin>(A.k, A.k_stride, b, h / (A.heads / A.k_heads));
+  const Tin* v = rows_of<Tin>(A.v, A.v_stride, b, h / (A.heads / A.v_heads));
+  long long qs = A.q_stride[2], ks = A.k_stride[2], vs = A.v_stride[2];
+  if (A.reverse && len > 0) {
+    q += (long long)(len - 1) * qs; qs = -qs;
+    k += (long long)(len - 1) * ks; ks = -ks;
+    v += (long long)(len - 1) * vs; vs = -vs;
+  }
+  const long long out0 = (long long)b * A.out_stride[0] + (long long)h * A.out_stride[1];
+  auto put = [&](int t, int d, float x) {  // component d of token t (in the order of the walk)
+    const long long at = out0 + (long long)(A.reverse && t < len ? len - 1 - t : t) * A.out_stride[2] + d;
+    if (A.out_float32) ((float*)A.out)[at] = x; else ((Tin*)A.out)[at] = (Tin)x;
+  };
+
+  f32x16 S[DK / 32];
+  {
+    const float* from = segments > 1 ? states + (long long)blockIdx.x * A.dim * A.dim_v : (A.state_in ? A.state_in + (long long)unit * A.dim * A.dim_v : nullptr);
+    const long long s0 = segments > 1 ? A.dim_v : A.state_in_stride[0], s1 = segments > 1 ? 1 : A.state_in_stride[1];
+#pragma unroll
+    for (int i = 0; i < DK / 32; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int d = 32 * i + c_row(r, half);
+        S[i][r] = from && d < A.dim && c < A.dim_v ? from[d * s0 + c * s1] : 0.f;
+      }
+  }
+  Staged<Tin, Tc, C, DK, NT> sq, sk;
+  Staged<Tin, Tc, C, DV, NT> sv;
+  if (t0 < t1) {
+    sq.load(q, qs, t0, t1, A.dim, tid);
+    sk.load(k, ks, t0, t1, A.dim, tid);
+    sv.load(v, vs, t0, t1, A.dim_v, tid);
+  }
+  for (int t = t0; t < t1; t += C) {
+    __syncthreads();
+    sq.store(qt, tid);
+    sk.store(kt, tid);
+    sv.store(vt, tid);
+    __syncthreads();
+    if (t + C < t1) {
+      sq.load(q, qs, t + C, t1, A.dim, tid);
+      sk.load(k, ks, t + C, t1, A.dim, tid);
+      sv.load(v, vs, t + C, t1, A.dim_v, tid);
+    }
+    // decayed products within the chunk: three 32 x 32 tiles (rows tokens j, columns tokens i >= j), shared through LDS
+    for (int tile = wave; tile < 3; tile += NW) {
+      const int i0 = tile == 0 ? 0 : 32, j0 = tile == 2 ? 32 : 0;
+      f32x16 a = zero16();
+#pragma unroll
+      for (int s = 0; s < DK / 16; s++) a = mma(frag_rows(kt + (j0 + col) * SK, 16 * s, half), frag_rows(qt + (i0 + col) * SK, 16 * s, half), a);
+      const float* w = pw + kZero + i0 + col - j0 - 4 * half;
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        float x[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) x[u] = i0 + col >= j0 + 8 * g + 4 * half + u ? a[4 * g + u] * (w[-(8 * g + u)] * A.product_scale) : 0.f;
+        store4<Tc>(pt + (i0 + col) * SP + j0 + 8 * g + 4 * half, x[0], x[1], x[2], x[3]);
+      }
+    }
+    __syncthreads();
+    // outputs: the state's part first, decayed to each row in float32, then the chunk's own
+    f32x16 o[2] = {zero16(), zero16()};
+#pragma unroll
+    for (int i = 0; i < DK / 32; i++)
+#pragma unroll
+      for (int s = 0; s < 2; s++) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) x[j] = S[i][8 * s + j];
+        Terms<Tc, state_terms<Tc>()> st;
+        st.set(x);
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+          const typename Vec<Tc>::x8 qf = frag_rows_split(qt + (32 * u + col) * SK, 32 * i + 16 * s, half);
+#pragma unroll
+          for (int m = 0; m < state_terms<Tc>(); m++) o[u] = mma(qf, st.t[m], o[u]);
+        }
+      }
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+#pragma unroll
+      for (int r = 0; r < 16; r++) o[u][r] *= pw[kZero + 32 * u + c_row(r, half) + shift] * A.query_scale;
+#pragma unroll
+      for (int s = 0; s < 2 * (u + 1); s++) o[u] = mma(frag_rows_split(pt + (32 * u + col) * SP, 16 * s, half), frag_cols<Tc>(vt, SV, 16 * s, 32 * wave, lane), o[u]);
+    }
+    if (c < A.dim_v) {
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          const int row = t + 32 * u + c_row(r, half);
+          if (row < t1) put(row, c, o[u][r]);
+        }
+    }
+    if (segments == 1 ? (A.state_out || t + C < t1) : t + C < t1)
+      update_state<Tc, DK, DV>(S, kt, vt, pw, min(C, t1 - t), A.reverse, A.update_scale, wave, lane);
+  }
+  // tokens behind the sequence
+  for (int t = max(t0, len); t < min((int)A.tokens, t0 + seg_tokens); t++)
+    for (int d = tid; d < A.dim_v; d += NT) put(t, d, 0.f);
+  if (segments == 1 && A.state_out) {
+    float* to = A.state_out + (long long)unit * A.dim * A.dim_v;
+#pragma unroll
+    for (int i = 0; i < DK / 32; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) {
+        const int d = 32 * i + c_row(r, half);
+        if (d < A.dim && c < A.dim_v) to[d * A.state_out_stride[0] + c * A.state_out_stride[1]] = S[i][r];
+      }
+  }
+}
+
+// ---- one token ----------------------------------------------------------------------------------------------------------------
+//
+// One read and one write of the state, float32.  A workgroup has `slice` columns of one head's state, 16 bytes of a row to a
+// thread; the sum over the rows is joined in LDS.
+struct Strides2 { long long batch, head; };
+
+template <class T>
+__global__ void __launch_bounds__(256) decay_step(int heads, int group, int dim, int dim_v, int slice, float scale, const T* q, Strides2 qs, const T* k,
+                                                  Strides2 ks, const T* v, Strides2 vs, const float* log_decay, float* state, T* out) {
+  __shared__ float qk[2][128];
+  __shared__ f32x4 red[256];
+  const int unit = blockIdx.x, b = unit / heads, h = unit % heads, tid = threadIdx.x;
+  for (int d = tid; d < dim; d += 256) {
+    qk[0][d] = (float)q[b * qs.batch + h * qs.head + d] * scale;
+    qk[1][d] = (float)k[b * ks.batch + (h / group) * ks.head + d];
+  }
+  const float g = expf(log_decay[h]);
+  const int quads = slice / 4, c = blockIdx.y * slice + 4 * (tid % quads), r0 = tid / quads, step = 256 / quads;
+  f32x4 vv = {0.f, 0.f, 0.f, 0.f}, acc = vv;
+  const bool there = c < dim_v;
+  if (there) {
+    const T* vp = v + b * vs.batch + (h / group) * vs.head + c;
+#pragma unroll
+    for (int j = 0; j < 4; j++) vv[j] = (float)vp[j];
+  }
+  __syncthreads();
+  float* s = state + (long long)unit * dim * dim_v + c;
+  if (there) {
+    constexpr int U = 8;  // rows of a thread in flight
+    for (int d0 = r0; d0 < dim; d0 += U * step) {
+      f32x4 x[U];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (d0 + u * step < dim) x[u] = *reinterpret_cast<const f32x4*>(s + (long long)(d0 + u * step) * dim_v);
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int d = d0 + u * step;
+        if (d < dim) {
+          const float kk = qk[1][d], qq = qk[0][d];
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            x[u][j] = fmaf(g, x[u][j], kk * vv[j]);
+            acc[j] = fmaf(qq, x[u][j], acc[j]);
+          }
+          *reinterpret_cast<f32x4*>(s + (long long)d * dim_v) = x[u];
+        }
+      }
+    }
+  }
+  red[tid] = acc;
+  __syncthreads();
+  for (int o = 128; o >= quads; o >>= 1) {
+    if (tid < o) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) red[tid][j] += red[tid + o][j];
+    }
+    __syncthreads();
+  }
+  if (tid < quads && there) {
+    T* op = out + (long long)unit * dim_v + c;
+#pragma unroll
+    for (int j = 0; j < 4; j++) op[j] = (T)red[tid][j];
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------------------
+
+const char* check(const Args* a) {
+  if (!a) return "decay attention: null arguments";
+  if (a->dtype < 0 || a->dtype > 2) return "decay attention: dtype must be 0 (bfloat16), 1 (float16) or 2 (float32)";
+  const int ve = a->dtype == 2 ? 4 : 8;
+  if (a->batch < 1 || a->heads < 1 || a->q_heads < 1 || a->k_heads < 1 || a->v_heads < 1 || a->heads % a->q_heads || a->heads % a->k_heads || a->heads % a->v_heads)
+    return "decay attention: heads must be a multiple of the heads of q, k and v";
+  if (a->dim < ve || a->dim > 128 || a->dim % ve || a->dim_v < ve || a->dim_v > 128 || a->dim_v % ve)
+    return "decay attention: dim and dim_v must be multiples of 16 bytes, at most 128";
+  if (a->tokens < 0 || a->tokens > (1 << 29)) return "decay attention: tokens out of range";
+  if (!a->log_decay || (a->tokens > 0 && (!a->q || !a->k || !a->v || !a->out))) return "decay attention: null data";
+  if ((int64_t)a->batch * a->heads > 65535) return "decay attention: more than 65535 sequences times heads";
+  return nullptr;
+}
+
+// Segments of a sequence: enough workgroups to fill the chip, whole chunks each.
+void segments_of(const Args* a, int& segments, int& seg_tokens) {
+  const int64_t units = (int64_t)a->batch * a->heads, chunks = (a->tokens + C - 1) / C;
+  int64_t want = (512 + units - 1) / units;
+  if (want > chunks) want = chunks;
+  if (want < 1) want = 1;
+  const int64_t per = chunks < 1 ? 1 : (chunks + want - 1) / want;
+  segments = (int)(chunks < 1 ? 1 : (chunks + per - 1) / per);
+  seg_tokens = (int)(per * C);
+}
+
+template <class K> int prepare_lds(K kernel, size_t bytes) {
+  if (bytes <= 64 * 1024) return 0;
+  const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  return e == hipSuccess ? 0 : keops_seq_fail((int)e, "decay attention: shared memory");
+}
+
+template <class Tin, class Tc, int DK, int DV> int run(const Args& a, float* work, hipStream_t st) {
+  int segments, seg_tokens;
+  segments_of(&a, segments, seg_tokens);
+  const int units = a.batch * a.heads;
+  const size_t kv = (size_t)C * (tile_stride<Tc, DK>() + tile_stride<Tc, DV>()) * sizeof(Tc), pw = kPowers * sizeof(float);
+  const size_t all = kv + (size_t)C * (tile_stride<Tc, DK>() + tile_stride<Tc, C>()) * sizeof(Tc) + pw;
+  if (segments > 1) {
+    if (int e = prepare_lds(decay_states<Tin, Tc, DK, DV>, kv + pw)) return e;
+    decay_states<Tin, Tc, DK, DV><<<units * segments, 2 * DV, kv + pw, st>>>(a, segments, seg_tokens, work);
+    decay_scan<<<dim3((a.dim * a.dim_v + 255) / 256, units), 256, 0, st>>>(a, segments, seg_tokens, work);
+  }
+  if (int e = prepare_lds(decay_outputs<Tin, Tc, DK, DV>, all)) return e;
+  decay_outputs<Tin, Tc, DK, DV><<<units * segments, 2 * DV, all, st>>>(a, segments, seg_tokens, work);
+  return seq_launched("decay attention: launch");
+}
+
+template <class Tin, class Tc> int dispatch(const Args& a, float* work, hipStream_t st) {
+  if (a.dim <= 64) return a.dim_v <= 64 ? run<Tin, Tc, 64, 64>(a, work, st) : run<Tin, Tc, 64, 128>(a, work, st);
+  return a.dim_v <= 64 ? run<Tin, Tc, 128, 64>(a, work, st) : run<Tin, Tc, 128, 128>(a, work, st);
+}
+
+template <class T>
+int step(int batch, int heads, int group, int dim, int dim_v, float scale, const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v,
+         const int64_t* vs, const float* log_decay, float* state, void* out, hipStream_t st) {
+  // narrow slices while whole heads would not give two workgroups to a CU
+  const int units = batch * heads, slice = units >= 512 ? 128 : 32;
+  decay_step<T><<<dim3(units, (dim_v + slice - 1) / slice), 256, 0, st>>>(heads, group, dim, dim_v, slice, scale, (const T*)q, Strides2{qs[0], qs[1]},
+                                                                          (const T*)k, Strides2{ks[0], ks[1]}, (const T*)v, Strides2{vs[0], vs[1]}, log_decay,
+                                                                          state, (T*)out);
+  return seq_launched("decay attention step: launch");
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t keops_hip_decay_attention_bytes(const keops_hip_decay_attention* a) {
+  if (check(a)) return 0;
+  int segments, seg_tokens;
+  segments_of(a, segments, seg_tokens);
+  return segments > 1 ? (size_t)a->batch * a->heads * segments * a->dim * a->dim_v * sizeof(float) : 0;
+}
+
+int keops_hip_decay_attention_run(const keops_hip_decay_attention* a, void* work, size_t work_bytes, int device, void* hip_stream) {
+  if (const char* why = check(a)) return keops_seq_fail(-1, why);
+  const size_t need = keops_hip_decay_attention_bytes(a);
+  if (need > work_bytes || (need > 0 && !work)) return keops_seq_fail(-1, "decay attention: workspace too small");
+  SeqDevice on(device);
+  hipStream_t st = (hipStream_t)hip_stream;
+  if (a->dtype == 0) return dispatch<bf16, bf16>(*a, (float*)work, st);
+  if (a->dtype == 1) return dispatch<f16, float>(*a, (float*)work, st);
+  return dispatch<float, float>(*a, (float*)work, st);
+}
+
+int keops_hip_decay_attention_step(int dtype, int batch, int heads, int kv_heads, int dim, int dim_v, float scale, const void* q, const int64_t* q_stride,
+                                   const void* k, const int64_t* k_stride, const void* v, const int64_t* v_stride, const float* log_decay, float* state,
+                                   void* out, int device, void* hip_stream) {
+  if (dtype < 0 || dtype > 2) return keops_seq_fail(-1, "decay attention step: dtype must be 0 (bfloat16), 1 (float16) or 2 (float32)");
+  if (batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads) return keops_seq_fail(-1, "decay attention step: heads must be a multiple of kv_heads");
+  if (dim < 1 || dim > 128 || dim_v < 4 || dim_v > 128 || dim_v % 4) return keops_seq_fail(-1, "decay attention step: dim at most 128, dim_v a multiple of 4, at most 128");
+  if ((int64_t)batch * heads > 0x7fffffff) return keops_seq_fail(-1, "decay attention step: too many workgroups");
+  if (!q || !q_stride || !k || !k_stride || !v || !v_stride || !log_decay || !state || !out) return keops_seq_fail(-1, "decay attention step: null data");
+  SeqDevice on(device);
+  hipStream_t st = (hipStream_t)hip_stream;
+  const int group = heads / kv_heads;
+  if (dtype == 0) return step<bf16>(batch, heads, group, dim, dim_v, scale, q, q_stride, k, k_stride, v, v_stride, log_decay, state, out, st);
+  if (dtype == 1) return step<f16>(batch, heads, group, dim, dim_v, scale, q, q_stride, k, k_stride, v, v_stride, log_decay, state, out, st);
+  return step<float>(batch, heads, group, dim, dim_v, scale, q, q_stride, k, k_stride, v, v_stride, log_decay, state, out, st);
+}
+
+}  // extern "C"

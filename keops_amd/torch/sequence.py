@@ -1,0 +1,568 @@
+"""Sequence operators: three of the engine's reductions in the form in which models of token sequences use them, where no
+formula can express them (a table looked up by position, a causal bound, shared heads, 16-bit types).
+
+=========================  =====================================================  ==============================
+:func:`bucket_attention`   softmax-weighted sum over keys (``SumSoftMaxWeight``)  learned bias by position bucket
+:func:`decay_attention`    sum over past tokens (``Sum``) in linear time          decay for each head, carried state
+:func:`token_logprobs`     ``LogSumExp`` and K largest values of rows of logits   log probability, entropy, alternatives
+=========================  =====================================================  ==============================
+
+Tensors live on one HIP device, in bfloat16, float16 or float32; sums, softmax statistics and states are float32.  Launches go to
+the current stream of that device and can be captured in a HIP graph (for :class:`PositionBuckets`, after a first use on the
+device outside the capture).  Results do not depend on the order in which workgroups run.  Gradients are of first order.
+"""
+import ctypes
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import binder
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _check_data(what, **tensors):
+    """All on one HIP device, all of one supported type; returns them in order."""
+    device = dtype = None
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"[KeOps] {what}: {name} must be a torch tensor, got {type(t)}.")
+        if not t.is_cuda:
+            raise ValueError(f"[KeOps] {what}: {name} must be on a HIP device, it is on {t.device}.")
+        if device is not None and t.device != device:
+            raise ValueError("[KeOps] Input arrays must be all located on the same device.")
+        if t.dtype not in _DTYPES:
+            raise ValueError(f"[KeOps] {what}: {name} must be bfloat16, float16 or float32, it is {t.dtype}.")
+        if dtype is not None and t.dtype != dtype:
+            raise ValueError(f"[KeOps] {what}: {', '.join(tensors)} must be of one type, got {dtype} and {t.dtype}.")
+        device, dtype = t.device, t.dtype
+    return device, dtype
+
+
+def _check_whole(what, name, t, shape, device):
+    """An int32 / int64 tensor of this shape on this device, as int32."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"[KeOps] {what}: {name} must be an int32 or int64 tensor.")
+    if t.device != device:
+        raise ValueError("[KeOps] Input arrays must be all located on the same device.")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"[KeOps] {what}: {name} must be of shape {shape}, got {tuple(t.shape)}.")
+    return t.to(torch.int32).contiguous()
+
+
+def _rows(x):
+    """x with rows as the kernels read them: neighbouring components, every row at a multiple of 16 bytes (a copy if not)."""
+    size = x.element_size()
+    if x.numel() == 0 or (
+        x.stride(-1) == 1 and x.data_ptr() % 16 == 0
+        and all(s * size % 16 == 0 for s, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1)
+    ):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _like(x):
+    """Uninitialised tensor of x's shape, in x's order of dimensions where x is dense, with rows as the kernels write them."""
+    y = torch.empty_like(x)
+    return y if _rows(y) is y else torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
+def _pad(x, *multiples):
+    """x with zeros behind its last dimensions, up to multiples (given from the last dimension on)."""
+    pad = []
+    for k, m in enumerate(multiples):
+        pad += [0, -x.shape[-1 - k] % m]
+    return torch.nn.functional.pad(x, pad) if any(pad) else x
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stride(t):
+    return t.stride()[:3]
+
+
+def _needs_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _call(name, args, size, device):
+    """Run an entry point of the library on the device's current stream, with the workspace that it asks for."""
+    lib = binder.lib()
+    nbytes = getattr(lib, size)(ctypes.byref(args))
+    work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    stream = torch.cuda.current_stream(device).cuda_stream
+    binder.check(getattr(lib, name)(ctypes.byref(args), _ptr(work), nbytes, device.index, stream), name)
+
+
+# --------------------------------------------------------------------------------------------------- position buckets
+class PositionBuckets:
+    """Buckets of relative positions ``key - query``, for :func:`bucket_attention`.
+
+    One bucket for each of the first distances, then buckets in equal steps of the logarithm up to ``max_distance``; everything
+    farther shares the last one.  With ``bidirectional`` half of the buckets are for keys after the query, otherwise those share
+    the bucket of distance 0.  The borders are whole numbers found without rounding: with n buckets for a direction, m = n // 2
+    and t > 0, bucket m + t begins at the smallest distance d with (d / m)^(n - m) >= (max_distance / m)^t.
+
+    ``PositionBuckets.from_map`` takes any other map.  Objects are immutable; their device copies are made at first use on a
+    device.
+    """
+
+    MAX_REACH = 2048  # KEOPS_HIP_MAX_REACH
+
+    def __init__(self, num_buckets=32, max_distance=128, bidirectional=True):
+        count = num_buckets // 2 if bidirectional else num_buckets
+        near = count // 2
+        if num_buckets < (4 if bidirectional else 2) or (bidirectional and num_buckets % 2):
+            raise ValueError("[KeOps] PositionBuckets: num_buckets must be at least 2 (bidirectional: an even number, at least 4).")
+        if not near < max_distance <= self.MAX_REACH:
+            raise ValueError(f"[KeOps] PositionBuckets: max_distance must be above {near} (the distances with a bucket of their "
+                             f"own) and at most {self.MAX_REACH}.")
+        if num_buckets > 2 * max_distance + 1:
+            raise ValueError("[KeOps] PositionBuckets: more buckets than positions within max_distance.")
+        steps, t, by_distance = count - near, 0, []
+        for d in range(max_distance + 1):
+            while d >= near and t + 1 < steps and d ** steps >= near ** (steps - t - 1) * max_distance ** (t + 1):
+                t += 1
+            by_distance.append(d if d < near else near + t)
+        reach = max(by_distance.index(by_distance[-1]), num_buckets // 2)  # the tables hold at least one entry a bucket
+        before = [by_distance[d] for d in range(reach, -1, -1)]
+        after = [count + by_distance[d] for d in range(1, reach + 1)] if bidirectional else [0] * reach
+        self._set(before + after, num_buckets)
+
+    @classmethod
+    def from_map(cls, bucket_of, num_buckets=None):
+        """Buckets from a sequence of 2 * reach + 1 whole numbers: the bucket of each relative position ``key - query`` from
+        ``-reach`` to ``reach``; positions beyond take that of the nearer end."""
+        bucket_of = [int(b) for b in (bucket_of.tolist() if isinstance(bucket_of, torch.Tensor) else bucket_of)]
+        if len(bucket_of) % 2 == 0 or len(bucket_of) < 3 or len(bucket_of) // 2 > cls.MAX_REACH:
+            raise ValueError(f"[KeOps] PositionBuckets: the map must have 2 * reach + 1 entries, with reach from 1 to {cls.MAX_REACH}.")
+        count = max(bucket_of) + 1 if num_buckets is None else int(num_buckets)
+        if min(bucket_of) < 0 or max(bucket_of) >= count or count > len(bucket_of):
+            raise ValueError("[KeOps] PositionBuckets: the map's entries must be from 0 to num_buckets - 1, and num_buckets at most "
+                             "the number of entries.")
+        self = cls.__new__(cls)
+        self._set(bucket_of, count)
+        return self
+
+    def _set(self, bucket_of, num_buckets):
+        self.num_buckets, self.reach = num_buckets, len(bucket_of) // 2
+        order = sorted(range(len(bucket_of)), key=lambda i: (bucket_of[i], i))
+        begin = [sum(b < k for b in bucket_of) for k in range(num_buckets + 1)]
+        self._host = tuple(torch.tensor(x, dtype=torch.int32) for x in (bucket_of, order, begin))
+        self._device = {}
+
+    def __call__(self, relative_position):
+        """Bucket of each entry of an integer tensor of relative positions ``key - query``."""
+        table = self._host[0].to(device=relative_position.device, dtype=torch.int64)
+        return table[relative_position.clamp(-self.reach, self.reach).long() + self.reach]
+
+    def on(self, device):
+        """The tables on a device: bucket of each distance, distances by bucket, begin of each bucket."""
+        device = torch.device(device)
+        if device not in self._device:
+            self._device[device] = tuple(t.to(device) for t in self._host)
+        return self._device[device]
+
+
+# --------------------------------------------------------------------------------------------------- bucket attention
+def _bucket_args(q, k, v, bias, buckets, causal, key_lengths, query_start, scale):
+    a = binder.BucketAttention()
+    a.dtype, a.batch, a.heads, a.kv_heads, a.dim = _DTYPES[q.dtype], q.shape[0], q.shape[1], k.shape[1], q.shape[3]
+    a.queries, a.keys, a.causal, a.scale = q.shape[2], k.shape[2], int(causal), scale
+    a.buckets, a.reach = buckets.num_buckets, buckets.reach
+    a.q, a.k, a.v, a.bias = _ptr(q), _ptr(k), _ptr(v), _ptr(bias)
+    a.q_stride[:], a.k_stride[:], a.v_stride[:] = _stride(q), _stride(k), _stride(v)
+    a.bucket_of, a.bucket_order, a.bucket_begin = (t.data_ptr() for t in buckets.on(q.device))
+    a.key_lengths = _ptr(key_lengths)
+    if isinstance(query_start, torch.Tensor):
+        a.query_start = _ptr(query_start)
+    else:
+        a.start = query_start
+    return a
+
+
+def _bucket_forward(q, k, v, bias, options, want_lse):
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    out = _like(q)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
+    if out.numel():
+        a = _bucket_args(q, k, v, bias, *options)
+        a.out, a.out_stride[:], a.lse = _ptr(out), _stride(out), _ptr(lse)
+        _call("keops_hip_bucket_attention_forward", a, "keops_hip_bucket_attention_forward_bytes", q.device)
+    return q, k, v, out, lse
+
+
+class _BucketAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, bias, options):
+        q, k, v, out, lse = _bucket_forward(q, k, v, bias, options, True)
+        tensors = [t for t in options if isinstance(t, torch.Tensor)]
+        ctx.places = [i for i, t in enumerate(options) if isinstance(t, torch.Tensor)]
+        ctx.options = [None if isinstance(t, torch.Tensor) else t for t in options]
+        ctx.save_for_backward(q, k, v, bias, out, lse, *tensors)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        q, k, v, bias, out, lse, *tensors = ctx.saved_tensors
+        options = list(ctx.options)
+        for i, t in zip(ctx.places, tensors):
+            options[i] = t
+        if out.numel() == 0:
+            return (*(torch.zeros_like(t) for t in (q, k, v, bias)), None)
+        grad = _rows(grad)
+        dq, dk, dv = (_like(q) if ctx.needs_input_grad[0] else None), _like(k), _like(v)
+        db = torch.empty_like(bias) if ctx.needs_input_grad[3] else None
+        delta = torch.empty_like(lse)
+        a = _bucket_args(q, k, v, bias, *options)
+        a.out, a.out_stride[:], a.lse, a.delta = _ptr(out), _stride(out), _ptr(lse), _ptr(delta)
+        a.grad_out, a.grad_out_stride[:] = _ptr(grad), _stride(grad)
+        if dq is not None:
+            a.grad_q, a.grad_q_stride[:] = _ptr(dq), _stride(dq)
+        a.grad_k, a.grad_k_stride[:], a.grad_v, a.grad_v_stride[:] = _ptr(dk), _stride(dk), _ptr(dv), _stride(dv)
+        a.grad_bias = _ptr(db)
+        _call("keops_hip_bucket_attention_backward", a, "keops_hip_bucket_attention_backward_bytes", q.device)
+        return dq, dk, dv, db, None
+
+
+def bucket_attention(q, k, v, bias, buckets, *, causal=False, key_lengths=None, query_start=0, scale=None):
+    r"""Softmax attention with a learned bias for each bucket of the relative position:
+
+    ``out_i = sum_j softmax_j(scale * <q_i, k_j> + bias[h, buckets(j - query_start - i)]) v_j``
+
+    Args:
+        q: (batch, heads, queries, dim).
+        k, v: (batch, kv_heads, keys, dim); ``heads`` is a multiple of ``kv_heads``, neighbouring heads share.  dim is at most
+            128.  Any strides (rows that do not start at multiples of 16 bytes are copied first).
+        bias: (heads, buckets.num_buckets), float32 or the type of q.
+        buckets: a :class:`PositionBuckets`.
+        causal: keys after the query's position do not count.
+        key_lengths: (batch,) whole numbers: keys from there on do not exist; what is stored there is not read.
+        query_start: position of the first query among the keys: a number, or (batch,) whole numbers, of absolute value at most
+            2**29.  For one new token against a cache that already holds its key: ``key_lengths - 1``.
+        scale: default ``dim ** -0.5``.
+
+    A query that sees no key has output 0 and gives no gradient.  Keys that are only hidden by ``causal`` are read with their
+    tile: a value that is not finite there can reach earlier queries.
+
+    Returns (batch, heads, queries, dim) in the type and order of dimensions of q.  Differentiable with respect to q, k, v and
+    bias.  Up to 32 queries x shared heads use a form of their own that splits the keys over the chip (token generation).
+    """
+    what = "bucket_attention"
+    device, dtype = _check_data(what, q=q, k=k, v=v)
+    if not isinstance(buckets, PositionBuckets):
+        raise TypeError("[KeOps] bucket_attention: buckets must be a PositionBuckets.")
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError("[KeOps] bucket_attention: q must be (batch, heads, queries, dim), k and v (batch, kv_heads, keys, dim).")
+    b, h, m, d = q.shape
+    if k.shape[0] != b or k.shape[3] != d or k.shape[1] < 1 or h % k.shape[1]:
+        raise ValueError(f"[KeOps] bucket_attention: q {tuple(q.shape)} and k {tuple(k.shape)} do not fit: same batch and dim, heads a "
+                         "multiple of kv_heads.")
+    if not 1 <= d <= 128:
+        raise ValueError(f"[KeOps] bucket_attention: dim must be from 1 to 128, it is {d}.")
+    if max(m, k.shape[2]) > 1 << 29:
+        raise ValueError("[KeOps] bucket_attention: at most 2**29 queries and keys.")
+    _check_data(what, bias=bias)
+    if bias.device != device:
+        raise ValueError("[KeOps] Input arrays must be all located on the same device.")
+    if bias.dtype not in (torch.float32, dtype) or tuple(bias.shape) != (h, buckets.num_buckets):
+        raise ValueError(f"[KeOps] bucket_attention: bias must be ({h}, {buckets.num_buckets}), float32 or {dtype}; got "
+                         f"{tuple(bias.shape)}, {bias.dtype}.")
+    if key_lengths is not None:
+        key_lengths = _check_whole(what, "key_lengths", key_lengths, (b,), device)
+    if isinstance(query_start, torch.Tensor):
+        query_start = _check_whole(what, "query_start", query_start, (b,), device)
+    elif isinstance(query_start, bool) or not isinstance(query_start, int) or abs(query_start) > 1 << 29:
+        raise ValueError("[KeOps] bucket_attention: query_start must be a whole number of absolute value at most 2**29, or a tensor.")
+    scale = d ** -0.5 if scale is None else float(scale)
+    align = 16 // q.element_size()
+    q, k, v, bias = _pad(q, align), _pad(k, align), _pad(v, align), bias.float().contiguous()
+    options = (buckets, bool(causal), key_lengths, query_start, scale)
+    if _needs_grad(q, k, v, bias):
+        out = _BucketAttention.apply(q, k, v, bias, options)
+    else:
+        out = _bucket_forward(q, k, v, bias, options, False)[3]
+    return out if out.shape[3] == d else out[..., :d].contiguous()
+
+
+# --------------------------------------------------------------------------------------------------- decay attention
+def _decay_run(q, k, v, log_decay, lengths, heads, *, reverse=False, product_scale=1.0, query_scale=1.0, update_scale=1.0, state=None,
+               transposed=False, out=None, float32=False, want_state=False):
+    """One walk over the tokens (keops_hip_decay_attention of include/keops_hip.h); ``transposed``: ``state`` holds the transpose
+    of the matrices that the walk starts from.  Returns the outputs and the final state (or None)."""
+    b, t, d, dv = q.shape[0], q.shape[2], q.shape[3], v.shape[3]
+    if out is None:
+        out = torch.empty(b, heads, t, dv, dtype=torch.float32 if float32 else q.dtype, device=q.device)
+    last = torch.empty(b, heads, d, dv, dtype=torch.float32, device=q.device) if want_state else None
+    if b == 0 or heads == 0:
+        return out, last
+    a = binder.DecayAttention()
+    a.dtype, a.batch, a.heads, a.dim, a.dim_v, a.tokens = _DTYPES[q.dtype], b, heads, d, dv, t
+    a.q_heads, a.k_heads, a.v_heads = q.shape[1], k.shape[1], v.shape[1]
+    a.reverse, a.out_float32 = int(reverse), int(out.dtype == torch.float32)
+    a.product_scale, a.query_scale, a.update_scale = product_scale, query_scale, update_scale
+    a.q, a.k, a.v, a.out = _ptr(q), _ptr(k), _ptr(v), _ptr(out)
+    a.q_stride[:], a.k_stride[:], a.v_stride[:], a.out_stride[:] = _stride(q), _stride(k), _stride(v), _stride(out)
+    a.log_decay, a.lengths, a.state_in, a.state_out = _ptr(log_decay), _ptr(lengths), _ptr(state), _ptr(last)
+    a.state_in_stride[:] = (1, d) if transposed else (dv, 1)
+    a.state_out_stride[:] = (dv, 1)
+    _call("keops_hip_decay_attention_run", a, "keops_hip_decay_attention_bytes", q.device)
+    return out, last
+
+
+def _decay_out(q, v):
+    """Outputs: q's order of dimensions, v's components."""
+    if q.shape[3] == v.shape[3]:
+        return _like(q)
+    if q.dim() == 4 and q.stride(1) < q.stride(2):  # (batch, tokens, heads, dim) in memory
+        return torch.empty(q.shape[0], q.shape[2], q.shape[1], v.shape[3], dtype=q.dtype, device=q.device).transpose(1, 2)
+    return torch.empty(*q.shape[:3], v.shape[3], dtype=q.dtype, device=q.device)
+
+
+def _decay_forward(q, k, v, log_decay, state, lengths, scale):
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    out, last = _decay_run(q, k, v, log_decay, lengths, q.shape[1], product_scale=scale, query_scale=scale, state=state,
+                           out=_decay_out(q, v), want_state=True)
+    return q, k, v, out, last
+
+
+class _DecayAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, state, log_decay, lengths, scale):
+        ctx.set_materialize_grads(False)
+        q, k, v, out, last = _decay_forward(q, k, v, log_decay, state, lengths, scale)
+        ctx.scale = scale
+        ctx.save_for_backward(q, k, v, state, log_decay, lengths)
+        return out, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, grad_last):
+        # gradients are walks of the same kind (csrc/sequence/keops_seq_decay.hip)
+        q, k, v, state, log_decay, lengths = ctx.saved_tensors
+        (b, h, t, d), dv, scale, shared = q.shape, v.shape[3], ctx.scale, k.shape[1]
+        grad = torch.zeros(b, h, t, dv, dtype=q.dtype, device=q.device) if grad is None else _rows(grad)
+        grad_last = None if grad_last is None else grad_last.contiguous()
+
+        def walk(*data, want_state=False, like=None, **options):
+            # a shared head's gradient is the sum over the heads that share it, rounded once
+            out = None if like is not None and like.shape[1] != h else _like(like)
+            out, last = _decay_run(*data, log_decay, lengths, h, product_scale=scale, out=out, float32=True, want_state=want_state, **options)
+            if like is not None and like.shape[1] != h:
+                out = out.view(b, shared, h // shared, t, -1).sum(2).to(like.dtype)
+            return out, last
+
+        dq = dk = dv_ = ds = None
+        if ctx.needs_input_grad[0]:
+            dq, _ = walk(grad, v, k, like=q, query_scale=scale, state=state, transposed=True)
+        if ctx.needs_input_grad[1]:
+            dk, _ = walk(v, grad, q, like=k, reverse=True, update_scale=scale, state=grad_last, transposed=True)
+        if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
+            dv_, ds = walk(k, q, grad, like=v, reverse=True, update_scale=scale, state=grad_last, want_state=ctx.needs_input_grad[3])
+        return dq, dk, dv_, ds, None, None, None
+
+
+def _check_decay(what, q, k, v, log_decay, state, dims):
+    device, dtype = _check_data(what, q=q, k=k, v=v)
+    if any(x.dim() != dims for x in (q, k, v)):
+        raise ValueError(f"[KeOps] {what}: q, k and v must have {dims} dimensions.")
+    b, h, d, dv = q.shape[0], q.shape[1], q.shape[-1], v.shape[-1]
+    if k.shape[:-1] != v.shape[:-1] or k.shape[0] != b or k.shape[-1] != d or k.shape[2:-1] != q.shape[2:-1] or k.shape[1] < 1 or h % k.shape[1]:
+        raise ValueError(f"[KeOps] {what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit: same batch and tokens, k "
+                         "as wide as q, heads a multiple of kv_heads.")
+    if not (1 <= d <= 128 and 1 <= dv <= 128):
+        raise ValueError(f"[KeOps] {what}: dim and dim_v must be from 1 to 128, they are {d} and {dv}.")
+    if b * h > 65535:
+        raise ValueError(f"[KeOps] {what}: at most 65535 sequences times heads.")
+    for name, t, shape in (("log_decay", log_decay, (h,)), ("state", state, (b, h, d, dv))):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or tuple(t.shape) != shape:
+            raise ValueError(f"[KeOps] {what}: {name} must be a float32 tensor of shape {shape}.")
+        if t.device != device:
+            raise ValueError("[KeOps] Input arrays must be all located on the same device.")
+    if log_decay is None:
+        raise ValueError(f"[KeOps] {what}: log_decay must be a float32 tensor of shape ({h},).")
+    if log_decay.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"[KeOps] {what}: log_decay is a constant of the layer, no gradient with respect to it is computed; detach it.")
+    return device
+
+
+def decay_attention(q, k, v, log_decay, *, initial_state=None, lengths=None, scale=None):
+    r"""Linear attention with a decay for each head, over whole sequences.  With ``g = exp(log_decay[h])``:
+
+    ``S_t = g * S_(t-1) + k_t v_t^T,   out_t = scale * q_t S_t,   S_(-1) = initial_state``
+
+    Args:
+        q: (batch, heads, tokens, dim).
+        k: (batch, kv_heads, tokens, dim), v: (batch, kv_heads, tokens, dim_v); ``heads`` is a multiple of ``kv_heads``,
+            neighbouring heads share.  dim and dim_v are at most 128.  Any strides.
+        log_decay: (heads,), float32: logarithms of the decays, usually negative; ``-inf`` forgets everything but the token itself.
+        initial_state: (batch, heads, dim, dim_v), float32, or None for zeros.
+        lengths: (batch,) whole numbers: tokens from there on do not exist; they are not read, their outputs and gradients are
+            zeros, and the state stops before them.
+        scale: default ``dim ** -0.5``.
+
+    Returns ``(out, state)``: (batch, heads, tokens, dim_v) in the type of q, and the state behind the last token, float32, from
+    which :func:`decay_attention_step` or another call goes on.  Differentiable with respect to q, k, v and initial_state, through
+    both results.  Tokens are worked on in chunks of 64; a value that is not finite can reach earlier tokens of its chunk.
+    """
+    what = "decay_attention"
+    device = _check_decay(what, q, k, v, log_decay, initial_state, 4)
+    d, dv = q.shape[3], v.shape[3]
+    if q.shape[2] > 1 << 29:
+        raise ValueError("[KeOps] decay_attention: at most 2**29 tokens.")
+    if lengths is not None:
+        lengths = _check_whole(what, "lengths", lengths, (q.shape[0],), device)
+    scale = d ** -0.5 if scale is None else float(scale)
+    align = 16 // q.element_size()
+    q, k, v = _pad(q, align), _pad(k, align), _pad(v, align)
+    state = None if initial_state is None else _pad(initial_state, align, align).contiguous()
+    log_decay = log_decay.contiguous()
+    if _needs_grad(q, k, v, state):
+        out, last = _DecayAttention.apply(q, k, v, state, log_decay, lengths, scale)
+    else:
+        out, last = _decay_forward(q, k, v, log_decay, state, lengths, scale)[3:]
+    if out.shape[3] != dv:
+        out = out[..., :dv].contiguous()
+    if last.shape[2:] != (d, dv):
+        last = last[:, :, :d, :dv].contiguous()
+    return out, last
+
+
+def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
+    r"""One token of :func:`decay_attention` for every sequence: ``state`` becomes ``g * state + k v^T`` in place, the result is
+    ``scale * q state``.
+
+    Args:
+        q: (batch, heads, dim), k: (batch, kv_heads, dim), v: (batch, kv_heads, dim_v), dim_v a multiple of 4.
+        log_decay: (heads,), float32.
+        state: (batch, heads, dim, dim_v), float32, contiguous; overwritten.
+        scale: default ``dim ** -0.5``.
+
+    Returns (batch, heads, dim_v) in the type of q.  No gradients.
+    """
+    what = "decay_attention_step"
+    if state is None:
+        raise ValueError("[KeOps] decay_attention_step: state must be a float32 tensor of shape (batch, heads, dim, dim_v).")
+    device = _check_decay(what, q, k, v, log_decay, state, 3)
+    if _needs_grad(q, k, v, state):
+        raise ValueError("[KeOps] decay_attention_step overwrites the state and has no gradient: use decay_attention, or torch.no_grad().")
+    if v.shape[2] % 4:
+        raise ValueError(f"[KeOps] decay_attention_step: dim_v must be a multiple of 4, it is {v.shape[2]}.")
+    if not state.is_contiguous() or state.data_ptr() % 16:
+        raise ValueError("[KeOps] decay_attention_step: state must be contiguous and aligned to 16 bytes, it is overwritten.")
+    b, h, d = q.shape
+    q, k, v = (x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous() for x in (q, k, v))
+    out = torch.empty(b, h, v.shape[2], dtype=q.dtype, device=device)
+    if out.numel() == 0:
+        return out
+    pair = ctypes.c_int64 * 2
+    log_decay = log_decay.contiguous()
+    rc = binder.lib().keops_hip_decay_attention_step(
+        _DTYPES[q.dtype], b, h, k.shape[1], d, v.shape[2], d ** -0.5 if scale is None else float(scale), _ptr(q), pair(*q.stride()[:2]),
+        _ptr(k), pair(*k.stride()[:2]), _ptr(v), pair(*v.stride()[:2]), _ptr(log_decay), _ptr(state), _ptr(out), device.index,
+        torch.cuda.current_stream(device).cuda_stream)
+    binder.check(rc, "keops_hip_decay_attention_step")
+    return out
+
+
+# --------------------------------------------------------------------------------------------------- log probabilities
+class TokenLogprobs(NamedTuple):
+    """Result of :func:`token_logprobs`."""
+
+    logprob: torch.Tensor      # (...,) float32
+    entropy: torch.Tensor      # (...,) float32
+    top_logprob: torch.Tensor  # (..., top) float32
+    top_index: torch.Tensor    # (..., top) int64
+
+
+def _logprobs_forward(logits, tokens, top, ignore_index):
+    rows, vocab = logits.shape
+    f32 = dict(dtype=torch.float32, device=logits.device)
+    logprob, entropy, lse = torch.empty(rows, **f32), torch.empty(rows, **f32), torch.empty(rows, **f32)
+    top_logprob = torch.empty(rows, top, **f32)
+    top_index = torch.empty(rows, top, dtype=torch.int64, device=logits.device)
+    if rows:
+        lib = binder.lib()
+        dt = _DTYPES[logits.dtype]
+        nbytes = lib.keops_hip_token_logprobs_bytes(dt, rows, vocab, top)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
+        rc = lib.keops_hip_token_logprobs(
+            dt, rows, vocab, top, _ptr(logits), logits.stride(0), _ptr(tokens), ignore_index, _ptr(logprob), _ptr(entropy), _ptr(lse),
+            _ptr(top_logprob), _ptr(top_index), _ptr(work), nbytes, logits.device.index,
+            torch.cuda.current_stream(logits.device).cuda_stream)
+        binder.check(rc, "keops_hip_token_logprobs")
+    return logprob, entropy, lse, top_logprob, top_index
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top, ignore_index):
+        ctx.set_materialize_grads(False)
+        logprob, entropy, lse, top_logprob, top_index = _logprobs_forward(logits, tokens, top, ignore_index)
+        ctx.save_for_backward(logits, tokens, entropy, lse, top_index)
+        ctx.top, ctx.ignore_index = top, ignore_index
+        ctx.mark_non_differentiable(top_index)
+        return logprob, entropy, top_logprob, top_index
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_logprob, g_entropy, g_top, _):
+        logits, tokens, entropy, lse, top_index = ctx.saved_tensors
+        rows, vocab = logits.shape
+        grad = torch.empty(rows, vocab, dtype=logits.dtype, device=logits.device)
+        if rows:
+            g_logprob, g_entropy, g_top = (None if g is None else g.contiguous() for g in (g_logprob, g_entropy, g_top))
+            rc = binder.lib().keops_hip_token_logprobs_backward(
+                _DTYPES[logits.dtype], rows, vocab, ctx.top, _ptr(logits), logits.stride(0), _ptr(tokens), ctx.ignore_index,
+                _ptr(entropy), _ptr(lse), _ptr(top_index), _ptr(g_logprob), _ptr(g_entropy), _ptr(g_top), _ptr(grad), vocab,
+                logits.device.index, torch.cuda.current_stream(logits.device).cuda_stream)
+            binder.check(rc, "keops_hip_token_logprobs_backward")
+        return grad, None, None, None
+
+
+def token_logprobs(logits, tokens, *, top=0, ignore_index=-100):
+    r"""Log probabilities of given tokens under ``softmax(logits)``, the entropies of the distributions and their ``top`` largest
+    log probabilities, in one sweep over the logits.
+
+    Args:
+        logits: (..., vocab).
+        tokens: (...), int64 or int32.
+        top: number of alternatives, at most 64 and at most vocab; equal values: the lowest index first.
+        ignore_index: rows with this token have log probability 0, without gradient; their entropy and alternatives are those of
+            the row.  Any other token outside 0..vocab-1 gives NaN.
+
+    Logits of ``-inf`` have probability 0; a row of nothing else has log probability and alternatives ``-inf`` and entropy 0, and
+    gradient 0.  A NaN or ``+inf`` makes its row's results NaN.
+
+    Returns a :class:`TokenLogprobs`, float32.  Differentiable with respect to the logits through ``logprob``, ``entropy`` and
+    ``top_logprob``.
+    """
+    what = "token_logprobs"
+    device, _ = _check_data(what, logits=logits)
+    if not isinstance(tokens, torch.Tensor) or tokens.dtype not in (torch.int64, torch.int32):
+        raise TypeError("[KeOps] token_logprobs: tokens must be an int64 or int32 tensor.")
+    if tokens.device != device:
+        raise ValueError("[KeOps] Input arrays must be all located on the same device.")
+    if logits.dim() < 1 or tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"[KeOps] token_logprobs: logits must be (..., vocab) and tokens (...); got {tuple(logits.shape)} and {tuple(tokens.shape)}.")
+    vocab = logits.shape[-1]
+    if not 1 <= vocab <= 2**31 - 1:
+        raise ValueError("[KeOps] token_logprobs: the vocabulary must have from 1 to 2**31 - 1 entries.")
+    if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= min(64, vocab):
+        raise ValueError(f"[KeOps] token_logprobs: top must be a whole number from 0 to {min(64, vocab)}, got {top}.")
+    shape = tokens.shape
+    flat = logits.reshape(-1, vocab)
+    if flat.stride(1) != 1 and vocab > 1:
+        flat = flat.contiguous()
+    tokens = tokens.reshape(-1).long().contiguous()
+    if _needs_grad(logits):
+        logprob, entropy, top_logprob, top_index = _TokenLogprobs.apply(flat, tokens, top, int(ignore_index))
+    else:
+        logprob, entropy, _, top_logprob, top_index = _logprobs_forward(flat, tokens, top, int(ignore_index))
+    return TokenLogprobs(logprob.view(shape), entropy.view(shape), top_logprob.view(*shape, top), top_index.view(*shape, top))
