@@ -56,43 +56,57 @@ __device__ inline f32x16 mma(const f32x8& a, const f32x8& b, f32x16 c) {
 // row of register r of a C tile
 __device__ inline constexpr int c_row(int r, int half) { return 8 * (r / 4) + 4 * half + r % 4; }
 
-// Tiles in LDS: rows of DP elements, padded by 16 bytes, so that the 16-byte row reads of eight neighbouring lanes fall into
-// different banks.
-template <class Tc, int DP> constexpr int tile_stride() { return DP + 16 / (int)sizeof(Tc); }
+// Tiles in LDS: rows of DP elements.  Two-byte elements: no padding, the 16-byte piece c of row r lies at place c ^ swizzle(r).
+// LDS has 64 banks (256 bytes): a row read takes the same piece of 16 rows at a time, a transposing read 64 neighbouring bytes of
+// four rows; the exclusive-or spreads both over all banks.  float32: rows padded by 16 bytes, no exclusive-or.
+template <class T, int DP> constexpr int tile_stride() { return sizeof(T) == 2 ? DP : DP + 4; }
+template <class T, int DP> __device__ inline int swizzle(int row) {
+  if constexpr (sizeof(T) != 2) return 0;
+  else if constexpr (DP == 128) return ((row & 3) << 2) | ((row >> 2) & 3);           // 256-byte rows: 16 pieces
+  else if constexpr (DP == 64) return ((row & 2) << 1) | ((row >> 2) & 3);            // two rows to 256 bytes: 8 pieces
+  else return (row >> 2) & 3;                                                         // 64 and 192 bytes: rows begin 64 bytes apart, 4 pieces
+}
+// offset of element `col` of row `row` (col: a multiple of 16 bytes, or within a piece)
+template <class T, int DP> __device__ inline int tile_at(int row, int col) {
+  if constexpr (sizeof(T) != 2) return row * tile_stride<T, DP>() + col;
+  else return row * DP + ((((col >> 3) ^ swizzle<T, DP>(row)) << 3) | (col & 7));
+}
 
 // contraction steps k0 + 8*half + (0..7) of one row
-template <class T> __device__ inline typename Vec<T>::x8 frag_rows(const T* row, int k0, int half) {
-  return *reinterpret_cast<const typename Vec<T>::x8*>(row + k0 + 8 * half);
+template <class T, int DP> __device__ inline typename Vec<T>::x8 frag_rows(const T* tile, int row, int k0, int half) {
+  return *reinterpret_cast<const typename Vec<T>::x8*>(tile + tile_at<T, DP>(row, k0 + 8 * half));
 }
 // contraction steps k0 + 4*half + (0..3), k0 + 8 + 4*half + (0..3) of one row: the order of a C tile's registers
-template <class T> __device__ inline typename Vec<T>::x8 frag_rows_split(const T* row, int k0, int half) {
+template <class T, int DP> __device__ inline typename Vec<T>::x8 frag_rows_split(const T* tile, int row, int k0, int half) {
   typedef typename Vec<T>::x4 x4;
-  const x4 a = *reinterpret_cast<const x4*>(row + k0 + 4 * half), b = *reinterpret_cast<const x4*>(row + k0 + 8 + 4 * half);
+  const x4 a = *reinterpret_cast<const x4*>(tile + tile_at<T, DP>(row, k0 + 4 * half));
+  const x4 b = *reinterpret_cast<const x4*>(tile + tile_at<T, DP>(row, k0 + 8 + 4 * half));
   return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
 // The transpose: column c0 + col of rows r0 + 4*half + (0..3) and r0 + 8 + 4*half + (0..3) of a tile in LDS.  Two-byte elements
 // come through the transposing LDS read: of each 16 lanes, lane i addresses four neighbouring elements of row i / 4 and
 // receives column i of the four rows.
-template <class T> __device__ inline typename Vec<T>::x8 frag_cols(const T* tile, int stride, int r0, int c0, int lane) {
-  typedef __attribute__((address_space(3))) s16x4 lds4;
-  const int half = lane >> 5, sub = (lane >> 4) & 1, i = lane & 15;
-  const T* p = tile + (r0 + 4 * half + (i >> 2)) * stride + c0 + 16 * sub + 4 * (i & 3);
-  union { s16x4 v[2]; typename Vec<T>::x8 x; } u;
-  u.v[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p));
-  u.v[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 8 * stride));
-  return u.x;
-}
-template <> __device__ inline f32x8 frag_cols<float>(const float* tile, int stride, int r0, int c0, int lane) {
-  const int half = lane >> 5, col = lane & 31;
-  const float* p = tile + (r0 + 4 * half) * stride + c0 + col;
-  f32x8 x;
+template <class T, int DP> __device__ inline typename Vec<T>::x8 frag_cols(const T* tile, int r0, int c0, int lane) {
+  const int half = lane >> 5;
+  if constexpr (sizeof(T) == 2) {
+    typedef __attribute__((address_space(3))) s16x4 lds4;
+    const int i = lane & 15, row = r0 + 4 * half + (i >> 2), col = c0 + (lane & 16) + 4 * (i & 3);
+    union { s16x4 v[2]; typename Vec<T>::x8 x; } u;
+    u.v[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + tile_at<T, DP>(row, col)));
+    u.v[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + tile_at<T, DP>(row + 8, col)));
+    return u.x;
+  } else {
+    constexpr int ST = tile_stride<T, DP>();
+    const T* p = tile + (r0 + 4 * half) * ST + c0 + (lane & 31);
+    typename Vec<T>::x8 x;
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    x[j] = p[j * stride];
-    x[4 + j] = p[(8 + j) * stride];
+    for (int j = 0; j < 4; j++) {
+      x[j] = p[j * ST];
+      x[4 + j] = p[(8 + j) * ST];
+    }
+    return x;
   }
-  return x;
 }
 
 // registers 8s..8s+7 of a C tile as an operand, rounded to the operand's type
@@ -104,17 +118,27 @@ template <class T> __device__ inline typename Vec<T>::x8 pack(const f32x16& c, i
 }
 
 // A tile of ROWS x DP elements on its way from memory to LDS, held in the registers of a workgroup of NT threads: rows from
-// `limit` on and columns from `dim` on are zeros and are not read, so what lies behind them never enters a product.
-template <class Tin, class Tc, int ROWS, int DP, int NT = 256> struct Staged {
+// `left` on and columns from `dim` on are zeros and are not read, so what lies behind them never enters a product.  `base` is the
+// tile's first row, the same for all threads; a thread's offset to it is 32 bits (rows are at most kMaxRowStride apart).
+// REVERSE: row r lies r rows before `base`.
+constexpr long long kMaxRowStride = 1ll << 23;  // elements: 64 rows of 4 bytes span 2^31 bytes
+
+template <class Tin, class Tc, int ROWS, int DP, int NT = 256, bool REVERSE = false> struct Staged {
   static constexpr int VE = 16 / (int)sizeof(Tin), PER_ROW = DP / VE, TOTAL = ROWS * PER_ROW, N = (TOTAL + NT - 1) / NT;
   uint4 r[N];
-  __device__ inline void load(const Tin* base, long long stride, long long row0, long long limit, int dim, int tid) {
+  __device__ inline void load(const Tin* base, long long stride, int left, int dim, int tid) {
+    const char* lowest = (const char*)(REVERSE ? base - (ROWS - 1) * stride : base);
+    const bool whole = left >= ROWS && dim == DP && TOTAL % NT == 0;
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const int c = tid + NT * i, row = c / PER_ROW, col = (c % PER_ROW) * VE;
-      r[i] = make_uint4(0u, 0u, 0u, 0u);
-      if ((TOTAL % NT == 0 || c < TOTAL) && row0 + row < limit && col < dim)
-        r[i] = *reinterpret_cast<const uint4*>(base + (row0 + row) * stride + col);
+      const unsigned off = ((unsigned)(REVERSE ? ROWS - 1 - row : row) * (unsigned)stride + (unsigned)col) * (unsigned)sizeof(Tin);
+      if (whole) {
+        r[i] = *reinterpret_cast<const uint4*>(lowest + off);
+      } else {
+        r[i] = make_uint4(0u, 0u, 0u, 0u);
+        if ((TOTAL % NT == 0 || c < TOTAL) && row < left && col < dim) r[i] = *reinterpret_cast<const uint4*>(lowest + off);
+      }
     }
   }
   __device__ inline void store(Tc* tile, int tid) const {
@@ -122,7 +146,7 @@ template <class Tin, class Tc, int ROWS, int DP, int NT = 256> struct Staged {
     for (int i = 0; i < N; i++) {
       const int c = tid + NT * i, row = c / PER_ROW, col = (c % PER_ROW) * VE;
       if (TOTAL % NT != 0 && c >= TOTAL) break;
-      Tc* dst = tile + row * tile_stride<Tc, DP>() + col;
+      Tc* dst = tile + tile_at<Tc, DP>(row, col);
       if constexpr (sizeof(Tin) == sizeof(Tc)) {
         *reinterpret_cast<uint4*>(dst) = r[i];
       } else {

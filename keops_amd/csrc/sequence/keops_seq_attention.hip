@@ -30,74 +30,98 @@ __device__ inline Span span_of(const Args& A, int b) {
   return s;
 }
 
-// unit (sequence and key/value head) and block within it.  With a multiple of 8 units, the blocks of one unit run on one XCD
-// (workgroups go to the XCDs in turn), which then holds the unit's keys and values in its own L2.
+// Unit (sequence and key/value head) and block within it of a workgroup.  With a multiple of 8 units, the blocks of one unit run
+// on one XCD (workgroups go to the XCDs in turn), which then holds the unit's keys and values in its own L2.  Block by block over
+// the units: with a causal bound the blocks are of very different length, and the longest of all units come first.
 __device__ inline void block_of(unsigned w, int per_unit, int units, int& unit, int& block) {
   if (units % 8 == 0) {
-    const int xcd = w & 7, slot = w >> 3;
-    unit = (slot / per_unit) * 8 + xcd;
-    block = slot % per_unit;
+    const int xcd = w & 7, slot = w >> 3, here = units / 8;
+    unit = (slot % here) * 8 + xcd;
+    block = slot / here;
   } else {
-    unit = w / per_unit;
-    block = w % per_unit;
+    unit = w % units;
+    block = w / units;
   }
 }
+
+// A bias of -6e4 or less (the lowest fp16 is -65504; masks of the type's lowest value) hides its pairs as -inf does: next to such a
+// number a float32 logit keeps nothing of the product, and a row of nothing else would be an average of what was masked.
+__device__ inline float bias_of(float x) { return x <= -6e4f ? -kInf : x * kLog2e; }
 
 // biases of head h by distance, times log2(e), padded on both sides
 __device__ inline void fill_table(float* table, const Args& A, int h, int tid, int nthreads) {
   const int top = 2 * A.reach;
-  for (int i = tid; i <= top + 2 * kPad; i += nthreads) table[i] = A.bias[(long long)h * A.buckets + A.bucket_of[clampi(i - kPad, 0, top)]] * kLog2e;
+  for (int i = tid; i <= top + 2 * kPad; i += nthreads) table[i] = bias_of(A.bias[(long long)h * A.buckets + A.bucket_of[clampi(i - kPad, 0, top)]]);
 }
 
 template <class T> __device__ inline const T* rows_of(const void* p, const int64_t* s, int b, int h) { return (const T*)p + (long long)b * s[0] + (long long)h * s[1]; }
 template <class T> __device__ inline T* rows_of(void* p, const int64_t* s, int b, int h) { return (T*)p + (long long)b * s[0] + (long long)h * s[1]; }
 
-template <class Tc> constexpr int key_tile() { return sizeof(Tc) == 2 ? 64 : 32; }
+// keys of a staged tile: 32 where 64 would not leave the rows in flight, the logits and the sums in 256 registers
+template <int DP> constexpr int key_tile() { return DP <= 64 ? 64 : 32; }
+template <class Tc> constexpr int query_tile() { return sizeof(Tc) == 2 ? 64 : 32; }  // queries of one, where keys are in registers
 
-// logits (base 2) of a 32 x 32 tile in place: rows are keys kb + 8g + 4 half + t, the lane's column is the query at position pos
-__device__ inline void add_bias_by_key(f32x16& s, float scale2, const float* table, int kb, int pos, int half, int kind, float far, int reach) {
+// wavefronts a SIMD: wide float32 rows need more than 256 registers
+template <class Tc, int DP> constexpr int waves() { return sizeof(Tc) == 4 && DP > 64 ? 1 : 2; }
+
+// logits (base 2, less `less`) of a 32 x 32 tile in place: rows are keys kb + 8g + 4 half + t, the lane's column is the query at
+// position pos.  kind: 0 within the reach of the buckets, otherwise the bias is `far`; keys from `lim` on do not count (mask).
+__device__ inline void logits_by_key(f32x16& s, float scale2, const float* table, float less, float far, int kind, bool mask, int lim, int kb, int pos,
+                                     int half, int reach) {
   if (kind == 0) {
     const float* tp = table + (kb - pos + reach + kPad + 4 * half);
 #pragma unroll
-    for (int r = 0; r < 16; r++) s[r] = fmaf(s[r], scale2, tp[8 * (r / 4) + r % 4]);
+    for (int r = 0; r < 16; r++) s[r] = fmaf(s[r], scale2, tp[8 * (r / 4) + r % 4]) - less;
   } else {
+    const float c = far - less;
 #pragma unroll
-    for (int r = 0; r < 16; r++) s[r] = fmaf(s[r], scale2, far);
+    for (int r = 0; r < 16; r++) s[r] = fmaf(s[r], scale2, c);
+  }
+  if (mask) {
+    const int rel = lim - kb - 4 * half;
+#pragma unroll
+    for (int r = 0; r < 16; r++) s[r] = 8 * (r / 4) + r % 4 < rel ? s[r] : -kInf;
   }
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------------
 //
-// One pass over the keys with a running maximum and sum.  A workgroup of four wavefronts has 128 queries of one head, a
-// wavefront 32 of them, one to a lane pair; tiles of 64 keys (32 in float32) are staged in LDS, double buffered, one barrier a
-// tile.  The logits are computed transposed (rows keys, columns queries), so a query's maximum and sum are in-lane reductions
-// and one exchange between the halves, and the probabilities enter the product with the values as they are (keops_seq.h).
+// One pass over the keys with a running reference point and sum.  A workgroup of four wavefronts has 128 queries of one head, a
+// wavefront 32 of them, one to a lane pair; tiles of 64 keys are staged in LDS, double buffered, one barrier a tile.  The logits
+// are computed transposed (rows keys, columns queries), so a query's sum is an in-lane reduction, and the probabilities enter the
+// product with the values as they are (keops_seq.h).
+//
+// Logits are formed less the reference point, so probabilities are exp2 of one multiply-add.  The point moves only when a logit
+// exceeds it by more than 8 (probabilities up to 2^8 lose nothing: the sum is kept in float32 and 16-bit operands have the same
+// relative step there).
 template <class Tin, class Tc, int DP>
-__global__ void __launch_bounds__(256, 2) attention_forward(const Args A) {
-  constexpr int KT = key_tile<Tc>(), ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32, SUB = KT / 32;
+__global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_forward(const Args A) {
+  constexpr int KT = key_tile<DP>(), SUB = KT / 32, ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32;
+  typedef typename Vec<Tc>::x8 frag;
   extern __shared__ __align__(16) unsigned char smem[];
-  Tc* const tiles = (Tc*)smem;  // [2][keys, values][KT][ST]
-  float* const table = (float*)(tiles + 4 * KT * ST);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  Tc* const ktiles = (Tc*)smem;  // [2][KT][ST]
+  Tc* const vtiles = ktiles + 2 * KT * ST;
+  float* const table = (float*)(vtiles + 2 * KT * ST);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
   const int group = A.heads / A.kv_heads, M = (int)A.queries, nqb = (M + 127) / 128;
   int unit, block;
   block_of(blockIdx.x, group * nqb, A.batch * A.kv_heads, unit, block);
-  const int b = unit / A.kv_heads, kvh = unit % A.kv_heads, h = kvh * group + block / nqb, qb = nqb - 1 - block % nqb;
+  const int b = unit / A.kv_heads, kvh = unit % A.kv_heads, h = kvh * group + block % group, qb = nqb - 1 - block / group;
   const Span sp = span_of(A, b);
   fill_table(table, A, h, tid, 256);
 
-  const int row = qb * 128 + wave * 32 + col, pos = sp.start + row;
-  const int pos_lo = sp.start + qb * 128 + wave * 32, pos_hi = pos_lo + 31;
+  const int pos_lo = sp.start + qb * 128 + wave * 32, pos_hi = pos_lo + 31, row = qb * 128 + wave * 32 + col, pos = pos_lo + col;
   const Tin* const K = rows_of<Tin>(A.k, A.k_stride, b, kvh);
   const Tin* const V = rows_of<Tin>(A.v, A.v_stride, b, kvh);
-  typename Vec<Tc>::x8 qf[NS];
+  const long long ks = A.k_stride[2], vs = A.v_stride[2];
+  frag qf[NS];
   {
     const Tin* q = rows_of<Tin>(A.q, A.q_stride, b, h) + (long long)row * A.q_stride[2];
 #pragma unroll
     for (int i = 0; i < NS; i++) qf[i] = frag_global<Tin, Tc>(q, row < M, 16 * i, half, A.dim);
   }
-  int kend = sp.klen;
-  if (A.causal) kend = min(kend, sp.start + min(qb * 128 + 128, M));
+  const int kend = A.causal ? min(sp.klen, sp.start + min(qb * 128 + 128, M)) : sp.klen;  // keys that the workgroup sees
+  const int wend = A.causal ? min(kend, pos_hi + 1) : kend;                                // and this wavefront
   const int ntiles = kend > 0 ? (kend + KT - 1) / KT : 0;
   const int lim = A.causal ? min(sp.klen, pos + 1) : sp.klen;
   const float scale2 = A.scale * kLog2e;
@@ -105,75 +129,86 @@ __global__ void __launch_bounds__(256, 2) attention_forward(const Args A) {
   f32x16 acc[ND];
 #pragma unroll
   for (int i = 0; i < ND; i++) acc[i] = zero16();
-  float m = -kInf, l = 0.f;
+  float m = 0.f, l = 0.f, above = -kInf;  // reference point, sum, by what a logit may exceed the reference (-inf: none yet)
 
   Staged<Tin, Tc, KT, DP> sk, sv;
   if (ntiles > 0) {
-    sk.load(K, A.k_stride[2], 0, sp.klen, A.dim, tid);
-    sv.load(V, A.v_stride[2], 0, sp.klen, A.dim, tid);
-    sk.store(tiles, tid);
-    sv.store(tiles + KT * ST, tid);
+    sk.load(K, ks, sp.klen, A.dim, tid);
+    sv.load(V, vs, sp.klen, A.dim, tid);
+    sk.store(ktiles, tid);
+    sv.store(vtiles, tid);
     if (ntiles > 1) {
-      sk.load(K, A.k_stride[2], KT, sp.klen, A.dim, tid);
-      sv.load(V, A.v_stride[2], KT, sp.klen, A.dim, tid);
+      sk.load(K + KT * ks, ks, sp.klen - KT, A.dim, tid);
+      sv.load(V + KT * vs, vs, sp.klen - KT, A.dim, tid);
     }
   }
   __syncthreads();
   const float left = table[0], right = table[2 * A.reach + 2 * kPad];
   for (int t = 0; t < ntiles; t++) {
-    const Tc* kt = tiles + (t & 1) * 2 * KT * ST;
-    const Tc* vt = kt + KT * ST;
+    const Tc* kt = ktiles + (t & 1) * KT * ST;
+    const Tc* vt = vtiles + (t & 1) * KT * ST;
     if (t + 1 < ntiles) {
-      Tc* nx = tiles + ((t + 1) & 1) * 2 * KT * ST;
-      sk.store(nx, tid);
-      sv.store(nx + KT * ST, tid);
+      sk.store(ktiles + ((t + 1) & 1) * KT * ST, tid);
+      sv.store(vtiles + ((t + 1) & 1) * KT * ST, tid);
       if (t + 2 < ntiles) {
-        sk.load(K, A.k_stride[2], (t + 2) * KT, sp.klen, A.dim, tid);
-        sv.load(V, A.v_stride[2], (t + 2) * KT, sp.klen, A.dim, tid);
+        sk.load(K + (long long)(t + 2) * KT * ks, ks, sp.klen - (t + 2) * KT, A.dim, tid);
+        sv.load(V + (long long)(t + 2) * KT * vs, vs, sp.klen - (t + 2) * KT, A.dim, tid);
       }
     }
     const int kb = t * KT;
-    if (!A.causal || kb <= pos_hi) {
+    if (kb < wend) {
       f32x16 s[SUB];
-#pragma unroll
-      for (int u = 0; u < SUB; u++) {
-        s[u] = zero16();
-#pragma unroll
-        for (int i = 0; i < NS; i++) s[u] = mma(frag_rows(kt + (32 * u + col) * ST, 16 * i, half), qf[i], s[u]);
-      }
+      float mx;
       const int kind = kb - pos_hi >= A.reach ? 1 : (kb + KT - 1 - pos_lo <= -A.reach ? -1 : 0);
+      const bool mask = kb + KT > sp.klen || (A.causal && kb + KT - 1 > pos_lo);
+      const auto logits = [&]() __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < SUB; u++) add_bias_by_key(s[u], scale2, table, kb + 32 * u, pos, half, kind, kind > 0 ? right : left, A.reach);
-      if (kb + KT > sp.klen || (A.causal && kb + KT - 1 > pos_lo)) {
-        const int rel = lim - kb - 4 * half;
+        for (int u = 0; u < SUB; u++) {
+          s[u] = zero16();
+#pragma unroll
+          for (int i = 0; i < NS; i++) s[u] = mma(frag_rows<Tc, DP>(kt, 32 * u + col, 16 * i, half), qf[i], s[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < SUB; u++) logits_by_key(s[u], scale2, table, m, kind > 0 ? right : left, kind, mask, lim, kb + 32 * u, pos, half, A.reach);
+        mx = s[0][0];
 #pragma unroll
         for (int u = 0; u < SUB; u++)
 #pragma unroll
-          for (int r = 0; r < 16; r++) s[u][r] = 32 * u + 8 * (r / 4) + r % 4 < rel ? s[u][r] : -kInf;
+          for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[u][r]);
+      };
+      logits();
+      if (__any(mx > above)) {
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        if (__any(mx > 192.f && above > 0.f)) {
+          // so far beyond the reference that nothing before counts, and that the difference may have lost what the logit was made
+          // of: such rows begin again, from the products
+          if (mx > 192.f && above > 0.f) {
+            m = l = 0.f;
+            above = -kInf;
+#pragma unroll
+            for (int k = 0; k < ND; k++) acc[k] = zero16();
+          }
+          logits();
+          mx = fmaxf(mx, __shfl_xor(mx, 32));
+        }
+        const float d = mx > above ? mx : 0.f, f = above == -kInf ? 0.f : __builtin_amdgcn_exp2f(-d);
+        above = mx > above ? 8.f : above;
+        m += d;
+        l *= f;
+#pragma unroll
+        for (int u = 0; u < SUB; u++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) s[u][r] -= d;
+#pragma unroll
+        for (int k = 0; k < ND; k++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) acc[k][r] *= f;
       }
-      float mx = s[0][0];
-#pragma unroll
-      for (int u = 0; u < SUB; u++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[u][r]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
-      // the reference point moves only when a logit exceeds it by more than 8 (probabilities up to 2^8 lose nothing: the sum is
-      // kept in float32 and 16-bit operands have the same relative step there)
-      if (__any(mx > m + 8.f)) {
-        const float mn = fmaxf(m, mx), alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-#pragma unroll
-        for (int i = 0; i < ND; i++)
-#pragma unroll
-          for (int r = 0; r < 16; r++) acc[i][r] *= alpha;
-        l *= alpha;
-        m = mn;
-      }
-      const float ms = m == -kInf ? 0.f : m;
 #pragma unroll
       for (int u = 0; u < SUB; u++)
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-          s[u][r] = __builtin_amdgcn_exp2f(s[u][r] - ms);
+          s[u][r] = __builtin_amdgcn_exp2f(s[u][r]);
           l += s[u][r];
         }
       // probabilities rounded to the values' type for the product (2^-9 relative for bf16, as much as the output's own rounding)
@@ -181,9 +216,9 @@ __global__ void __launch_bounds__(256, 2) attention_forward(const Args A) {
       for (int u = 0; u < SUB; u++)
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-          const typename Vec<Tc>::x8 p = pack<Tc>(s[u], k);
+          const frag p = pack<Tc>(s[u], k);
 #pragma unroll
-          for (int i = 0; i < ND; i++) acc[i] = mma(frag_cols<Tc>(vt, ST, 32 * u + 16 * k, 32 * i, lane), p, acc[i]);
+          for (int i = 0; i < ND; i++) acc[i] = mma(frag_cols<Tc, DP>(vt, 32 * u + 16 * k, 32 * i, lane), p, acc[i]);
         }
     }
     __syncthreads();
@@ -211,7 +246,7 @@ __global__ void __launch_bounds__(256, 2) attention_forward(const Args A) {
 // piece of LDS for the transposing read.  Shares of a long sequence go to different workgroups, which leave their sums for
 // attention_join.
 template <class Tin, class Tc, int DP>
-__global__ void __launch_bounds__(256, 2) attention_rows(const Args A, int splits, float* part) {
+__global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_rows(const Args A, int splits, float* part) {
   constexpr int ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32, VE = 16 / (int)sizeof(Tin), PER_ROW = DP / VE, NV = 32 * PER_ROW / 64;
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
@@ -235,7 +270,7 @@ __global__ void __launch_bounds__(256, 2) attention_rows(const Args A, int split
     for (int i = 0; i < NS; i++) qf[i] = frag_global<Tin, Tc>(q, there, 16 * i, half, A.dim);
   }
   const float* const bias = A.bias + (long long)(there ? h : 0) * A.buckets;
-  const float left = bias[A.bucket_of[0]] * kLog2e, right = bias[A.bucket_of[2 * A.reach]] * kLog2e;
+  const float left = bias_of(bias[A.bucket_of[0]]), right = bias_of(bias[A.bucket_of[2 * A.reach]]);
   const int lim = A.causal ? min(sp.klen, pos + 1) : sp.klen, pos_lo = sp.start, pos_hi = sp.start + M - 1;
   const float scale2 = A.scale * kLog2e;
   f32x16 acc[ND];
@@ -266,7 +301,7 @@ __global__ void __launch_bounds__(256, 2) attention_rows(const Args A, int split
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       const int c = lane + 64 * i;
-      Tc* dst = vt + (c / PER_ROW) * ST + (c % PER_ROW) * VE;
+      Tc* dst = vt + tile_at<Tc, DP>(c / PER_ROW, (c % PER_ROW) * VE);
       if constexpr (sizeof(Tin) == sizeof(Tc)) {
         *reinterpret_cast<uint4*>(dst) = vr[i];
       } else {
@@ -285,7 +320,7 @@ __global__ void __launch_bounds__(256, 2) attention_rows(const Args A, int split
 #pragma unroll
       for (int r = 0; r < 16; r++) {
         const int rel = clampi(kb + c_row(r, half) - pos, -A.reach, A.reach);
-        s[r] = fmaf(s[r], scale2, bias[A.bucket_of[rel + A.reach]] * kLog2e);
+        s[r] = fmaf(s[r], scale2, bias_of(bias[A.bucket_of[rel + A.reach]]));
       }
     }
     float mx = -kInf;
@@ -318,7 +353,7 @@ __global__ void __launch_bounds__(256, 2) attention_rows(const Args A, int split
     for (int k = 0; k < 2; k++) {
       const typename Vec<Tc>::x8 p = pack<Tc>(s, k);
 #pragma unroll
-      for (int i = 0; i < ND; i++) acc[i] = mma(frag_cols<Tc>(vt, ST, 16 * k, 32 * i, lane), p, acc[i]);
+      for (int i = 0; i < ND; i++) acc[i] = mma(frag_cols<Tc, DP>(vt, 16 * k, 32 * i, lane), p, acc[i]);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -393,24 +428,26 @@ template <class Tin> __global__ void __launch_bounds__(128) attention_join(const
 // <dO_i, o_i>, and the row sums of that dS, which are what delta is off by, are added to the delta that the gradient of keys,
 // values and biases uses.
 template <class Tin, class Tc, int DP>
-__global__ void __launch_bounds__(256, 2) attention_grad_q(const Args A) {
-  constexpr int KT = key_tile<Tc>(), ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32, SUB = KT / 32;
+__global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_grad_q(const Args A) {
+  constexpr int KT = key_tile<DP>(), SUB = KT / 32, ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32;
+  typedef typename Vec<Tc>::x8 frag;
   extern __shared__ __align__(16) unsigned char smem[];
-  Tc* const tiles = (Tc*)smem;
-  float* const table = (float*)(tiles + 4 * KT * ST);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  Tc* const ktiles = (Tc*)smem;
+  Tc* const vtiles = ktiles + 2 * KT * ST;
+  float* const table = (float*)(vtiles + 2 * KT * ST);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
   const int group = A.heads / A.kv_heads, M = (int)A.queries, nqb = (M + 127) / 128;
   int unit, block;
   block_of(blockIdx.x, group * nqb, A.batch * A.kv_heads, unit, block);
-  const int b = unit / A.kv_heads, kvh = unit % A.kv_heads, h = kvh * group + block / nqb, qb = nqb - 1 - block % nqb;
+  const int b = unit / A.kv_heads, kvh = unit % A.kv_heads, h = kvh * group + block % group, qb = nqb - 1 - block / group;
   const Span sp = span_of(A, b);
   fill_table(table, A, h, tid, 256);
 
-  const int row = qb * 128 + wave * 32 + col, pos = sp.start + row;
-  const int pos_lo = sp.start + qb * 128 + wave * 32, pos_hi = pos_lo + 31;
+  const int pos_lo = sp.start + qb * 128 + wave * 32, pos_hi = pos_lo + 31, row = qb * 128 + wave * 32 + col, pos = pos_lo + col;
   const Tin* const K = rows_of<Tin>(A.k, A.k_stride, b, kvh);
   const Tin* const V = rows_of<Tin>(A.v, A.v_stride, b, kvh);
-  typename Vec<Tc>::x8 qf[NS], gf[NS];
+  const long long ks = A.k_stride[2], vs = A.v_stride[2];
+  frag qf[NS], gf[NS];
   float delta = 0.f;
   {
     const Tin* q = rows_of<Tin>(A.q, A.q_stride, b, h) + (long long)row * A.q_stride[2];
@@ -420,7 +457,7 @@ __global__ void __launch_bounds__(256, 2) attention_grad_q(const Args A) {
     for (int i = 0; i < NS; i++) {
       qf[i] = frag_global<Tin, Tc>(q, row < M, 16 * i, half, A.dim);
       gf[i] = frag_global<Tin, Tc>(g, row < M, 16 * i, half, A.dim);
-      const typename Vec<Tc>::x8 of = frag_global<Tin, Tc>(o, row < M, 16 * i, half, A.dim);
+      const frag of = frag_global<Tin, Tc>(o, row < M, 16 * i, half, A.dim);
 #pragma unroll
       for (int j = 0; j < 8; j++) delta = fmaf((float)gf[i][j], (float)of[j], delta);
     }
@@ -428,9 +465,9 @@ __global__ void __launch_bounds__(256, 2) attention_grad_q(const Args A) {
   }
   const long long stat = ((long long)b * A.heads + h) * M + row;
   const float lse = row < M ? A.lse[stat] : kInf;
-  int kend = sp.klen;
-  if (A.causal) kend = min(kend, sp.start + min(qb * 128 + 128, M));
-  const int ntiles = kend > 0 ? (kend + KT - 1) / KT : 0;
+  const int kend = A.causal ? min(sp.klen, sp.start + min(qb * 128 + 128, M)) : sp.klen;
+  const int wend = A.causal ? min(kend, pos_hi + 1) : kend;
+  const int ntiles = kend > 0 ? (kend + KT - 1) / KT : 0, nsub = wend > 0 ? (wend + 31) / 32 : 0;
   const int lim = A.causal ? min(sp.klen, pos + 1) : sp.klen;
   const float scale2 = A.scale * kLog2e;
 
@@ -441,56 +478,52 @@ __global__ void __launch_bounds__(256, 2) attention_grad_q(const Args A) {
 
   Staged<Tin, Tc, KT, DP> sk, sv;
   if (ntiles > 0) {
-    sk.load(K, A.k_stride[2], 0, sp.klen, A.dim, tid);
-    sv.load(V, A.v_stride[2], 0, sp.klen, A.dim, tid);
-    sk.store(tiles, tid);
-    sv.store(tiles + KT * ST, tid);
+    sk.load(K, ks, sp.klen, A.dim, tid);
+    sv.load(V, vs, sp.klen, A.dim, tid);
+    sk.store(ktiles, tid);
+    sv.store(vtiles, tid);
     if (ntiles > 1) {
-      sk.load(K, A.k_stride[2], KT, sp.klen, A.dim, tid);
-      sv.load(V, A.v_stride[2], KT, sp.klen, A.dim, tid);
+      sk.load(K + KT * ks, ks, sp.klen - KT, A.dim, tid);
+      sv.load(V + KT * vs, vs, sp.klen - KT, A.dim, tid);
     }
   }
   __syncthreads();
   const float left = table[0], right = table[2 * A.reach + 2 * kPad];
   for (int t = 0; t < ntiles; t++) {
-    const Tc* kt = tiles + (t & 1) * 2 * KT * ST;
-    const Tc* vt = kt + KT * ST;
+    const Tc* kt = ktiles + (t & 1) * KT * ST;
+    const Tc* vt = vtiles + (t & 1) * KT * ST;
     if (t + 1 < ntiles) {
-      Tc* nx = tiles + ((t + 1) & 1) * 2 * KT * ST;
-      sk.store(nx, tid);
-      sv.store(nx + KT * ST, tid);
+      sk.store(ktiles + ((t + 1) & 1) * KT * ST, tid);
+      sv.store(vtiles + ((t + 1) & 1) * KT * ST, tid);
       if (t + 2 < ntiles) {
-        sk.load(K, A.k_stride[2], (t + 2) * KT, sp.klen, A.dim, tid);
-        sv.load(V, A.v_stride[2], (t + 2) * KT, sp.klen, A.dim, tid);
+        sk.load(K + (long long)(t + 2) * KT * ks, ks, sp.klen - (t + 2) * KT, A.dim, tid);
+        sv.load(V + (long long)(t + 2) * KT * vs, vs, sp.klen - (t + 2) * KT, A.dim, tid);
       }
     }
-    const int kb = t * KT;
-    if (!A.causal || kb <= pos_hi) {
-      const int kind = kb - pos_hi >= A.reach ? 1 : (kb + KT - 1 - pos_lo <= -A.reach ? -1 : 0);
-      const bool mask = kb + KT > sp.klen || (A.causal && kb + KT - 1 > pos_lo);
-      const int rel = lim - kb - 4 * half;
 #pragma unroll
-      for (int u = 0; u < SUB; u++) {
-        f32x16 s = zero16(), p = zero16();
+    for (int u = 0; u < SUB; u++) {
+      const int kb = t * KT + 32 * u;
+      if (SUB * t + u >= nsub) continue;
+      f32x16 s = zero16(), p;
 #pragma unroll
-        for (int i = 0; i < NS; i++) {
-          s = mma(frag_rows(kt + (32 * u + col) * ST, 16 * i, half), qf[i], s);
-          p = mma(frag_rows(vt + (32 * u + col) * ST, 16 * i, half), gf[i], p);
-        }
-        add_bias_by_key(s, scale2, table, kb + 32 * u, pos, half, kind, kind > 0 ? right : left, A.reach);
+      for (int r = 0; r < 16; r++) p[r] = -delta;
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-          float e = __builtin_amdgcn_exp2f(s[r] - lse);
-          if (mask) e = 32 * u + 8 * (r / 4) + r % 4 < rel ? e : 0.f;
-          s[r] = e * (p[r] - delta);
-          over += s[r];
-        }
+      for (int i = 0; i < NS; i++) {
+        s = mma(frag_rows<Tc, DP>(kt, 32 * u + col, 16 * i, half), qf[i], s);
+        p = mma(frag_rows<Tc, DP>(vt, 32 * u + col, 16 * i, half), gf[i], p);
+      }
+      const int kind = kb - pos_hi >= A.reach ? 1 : (kb + 31 - pos_lo <= -A.reach ? -1 : 0);
+      logits_by_key(s, scale2, table, lse, kind > 0 ? right : left, kind, kb + 32 > sp.klen || (A.causal && kb + 31 > pos_lo), lim, kb, pos, half, A.reach);
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-          const typename Vec<Tc>::x8 ds = pack<Tc>(s, k);
+      for (int r = 0; r < 16; r++) {
+        s[r] = __builtin_amdgcn_exp2f(s[r]) * p[r];
+        over += s[r];
+      }
 #pragma unroll
-          for (int i = 0; i < ND; i++) acc[i] = mma(frag_cols<Tc>(kt, ST, 32 * u + 16 * k, 32 * i, lane), ds, acc[i]);
-        }
+      for (int k = 0; k < 2; k++) {
+        const frag ds = pack<Tc>(s, k);
+#pragma unroll
+        for (int i = 0; i < ND; i++) acc[i] = mma(frag_cols<Tc, DP>(kt, 32 * u + 16 * k, 32 * i, lane), ds, acc[i]);
       }
     }
     __syncthreads();
@@ -520,8 +553,8 @@ __global__ void __launch_bounds__(256, 2) attention_grad_q(const Args A) {
 // register's row, so that equal distances meet in a lane) into a table by distance that belongs to the wavefront, and the tables
 // become sums by bucket when the head is done.
 template <class Tin, class Tc, int DP>
-__global__ void __launch_bounds__(256, 1) attention_grad_kv(const Args A, float* part) {
-  constexpr int QT = key_tile<Tc>(), ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32, SUB = QT / 32;
+__global__ void __launch_bounds__(256, sizeof(Tc) == 2 && DP <= 64 ? 2 : 1) attention_grad_kv(const Args A, float* part) {
+  constexpr int QT = query_tile<Tc>(), ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32, SUB = QT / 32;
   extern __shared__ __align__(16) unsigned char smem[];
   Tc* const tiles = (Tc*)smem;                          // [2][queries, output gradients][QT][ST]
   float* const stats = (float*)(tiles + 4 * QT * ST);   // [2][lse, delta][QT]
@@ -567,13 +600,13 @@ __global__ void __launch_bounds__(256, 1) attention_grad_kv(const Args A, float*
     const float* const del = A.delta + ((long long)b * A.heads + h) * M;
     float far_left = 0.f, far_right = 0.f;
     Staged<Tin, Tc, QT, DP> sq, sg;
-    float s_lse = kInf, s_del = 0.f;
+    float s_lse = -kInf, s_del = 0.f;
     auto fetch = [&](int q0) {
-      sq.load(Q, A.q_stride[2], q0, M, A.dim, tid);
-      sg.load(G, A.grad_out_stride[2], q0, M, A.dim, tid);
-      if (tid < QT) {
-        s_lse = q0 + tid < M ? lse[q0 + tid] : kInf;
-        s_del = q0 + tid < M ? del[q0 + tid] : 0.f;
+      sq.load(Q + (long long)q0 * A.q_stride[2], A.q_stride[2], M - q0, A.dim, tid);
+      sg.load(G + (long long)q0 * A.grad_out_stride[2], A.grad_out_stride[2], M - q0, A.dim, tid);
+      if (tid < QT) {  // the negatives, as they are added
+        s_lse = q0 + tid < M ? -lse[q0 + tid] : -kInf;
+        s_del = q0 + tid < M ? -del[q0 + tid] : 0.f;
       }
     };
     auto put = [&](int buf) {
@@ -606,43 +639,51 @@ __global__ void __launch_bounds__(256, 1) attention_grad_kv(const Args A, float*
       for (int u = 0; u < SUB; u++) {
         const int q0 = q_first + t * QT + 32 * u, pos0 = sp.start + q0;  // position of the tile's first query
         if (kb >= sp.klen || (A.causal && kb > pos0 + 31)) continue;     // nothing in this wavefront's tile
-        f32x16 s = zero16(), p = zero16();
+        f32x16 s = zero16(), p, e;
+#pragma unroll
+        for (int g4 = 0; g4 < 4; g4++) {
+          const f32x4 de = *reinterpret_cast<const f32x4*>(st + QT + 32 * u + 8 * g4 + 4 * half);
+#pragma unroll
+          for (int t4 = 0; t4 < 4; t4++) p[4 * g4 + t4] = de[t4];
+        }
 #pragma unroll
         for (int i = 0; i < NS; i++) {
-          s = mma(frag_rows(qt + (32 * u + col) * ST, 16 * i, half), kf[i], s);
-          p = mma(frag_rows(gt + (32 * u + col) * ST, 16 * i, half), vf[i], p);
+          s = mma(frag_rows<Tc, DP>(qt, 32 * u + col, 16 * i, half), kf[i], s);
+          p = mma(frag_rows<Tc, DP>(gt, 32 * u + col, 16 * i, half), vf[i], p);
         }
         const int kind = kb - (pos0 + 31) >= A.reach ? 1 : (kb + 31 - pos0 <= -A.reach ? -1 : 0);
-        f32x16 e;
-        if (kind == 0) {
-          const float* tp = table + (key - pos0 - 4 * half + A.reach + kPad);
-#pragma unroll
-          for (int r = 0; r < 16; r++) e[r] = fmaf(s[r], scale2, tp[-(8 * (r / 4) + r % 4)]);
-        } else {
-#pragma unroll
-          for (int r = 0; r < 16; r++) e[r] = fmaf(s[r], scale2, kind > 0 ? right : left);
-        }
 #pragma unroll
         for (int g4 = 0; g4 < 4; g4++) {
           const f32x4 ls = *reinterpret_cast<const f32x4*>(st + 32 * u + 8 * g4 + 4 * half);
-          const f32x4 de = *reinterpret_cast<const f32x4*>(st + QT + 32 * u + 8 * g4 + 4 * half);
 #pragma unroll
-          for (int t4 = 0; t4 < 4; t4++) {
-            const int r = 4 * g4 + t4;
-            float x = __builtin_amdgcn_exp2f(e[r] - ls[t4]);
-            const int qpos = pos0 + 8 * g4 + 4 * half + t4;
-            if (key >= sp.klen || (A.causal && key > qpos)) x = 0.f;
-            e[r] = x;
-            s[r] = x * (p[r] - de[t4]);
-          }
+          for (int t4 = 0; t4 < 4; t4++) e[4 * g4 + t4] = fmaf(s[4 * g4 + t4], scale2, ls[t4]);
+        }
+        if (kind == 0) {
+          const float* tp = table + (key - pos0 - 4 * half + A.reach + kPad);
+#pragma unroll
+          for (int r = 0; r < 16; r++) e[r] += tp[-(8 * (r / 4) + r % 4)];
+        } else {
+          const float far = kind > 0 ? right : left;
+#pragma unroll
+          for (int r = 0; r < 16; r++) e[r] += far;
+        }
+        if (kb + 31 >= sp.klen || (A.causal && kb + 31 > pos0)) {
+          const int first = key >= sp.klen ? 32 : (A.causal ? key - pos0 - 4 * half : -64);  // first row of the tile that sees the key
+#pragma unroll
+          for (int r = 0; r < 16; r++) e[r] = 8 * (r / 4) + r % 4 >= first ? e[r] : -kInf;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          e[r] = __builtin_amdgcn_exp2f(e[r]);
+          s[r] = e[r] * p[r];
         }
 #pragma unroll
         for (int k = 0; k < 2; k++) {
           const typename Vec<Tc>::x8 pf = pack<Tc>(e, k), df = pack<Tc>(s, k);
 #pragma unroll
           for (int i = 0; i < ND; i++) {
-            dv[i] = mma(frag_cols<Tc>(gt, ST, 32 * u + 16 * k, 32 * i, lane), pf, dv[i]);
-            dk[i] = mma(frag_cols<Tc>(qt, ST, 32 * u + 16 * k, 32 * i, lane), df, dk[i]);
+            dv[i] = mma(frag_cols<Tc, DP>(gt, 32 * u + 16 * k, 32 * i, lane), pf, dv[i]);
+            dk[i] = mma(frag_cols<Tc, DP>(qt, 32 * u + 16 * k, 32 * i, lane), df, dk[i]);
           }
         }
         if (want_bias) {
@@ -744,6 +785,8 @@ const char* check(const Args* a) {
   if (a->queries < 1 || a->queries > (1 << 29) || a->keys < 0 || a->keys > (1 << 29)) return "bucket attention: queries or keys out of range";
   if (a->reach < 1 || a->reach > KEOPS_HIP_MAX_REACH || a->buckets < 1 || a->buckets > 2 * a->reach + 1) return "bucket attention: reach or number of buckets out of range";
   if (a->start < -(1 << 29) || a->start > (1 << 29)) return "bucket attention: query_start out of range";
+  for (const int64_t* x : {a->q_stride, a->k_stride, a->v_stride, a->grad_out_stride})
+    if (x[2] < 0 || x[2] > kMaxRowStride) return "bucket attention: rows too far apart";
   if (!a->q || !a->out || !a->bias || !a->bucket_of || (a->keys > 0 && (!a->k || !a->v))) return "bucket attention: null data";
   const int64_t units = (int64_t)a->batch * a->heads;
   if (units * ((a->queries + 127) / 128) > 0x7fffffff || units * ((a->keys + 127) / 128) > 0x7fffffff) return "bucket attention: too many workgroups";
@@ -760,10 +803,7 @@ int splits_of(const Args* a) {
   return (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
 }
 
-int tile_bytes(int dtype_bytes, int dp) {
-  const int kt = dtype_bytes == 2 ? 64 : 32;
-  return 4 * kt * (dp + 16 / dtype_bytes) * dtype_bytes;
-}
+template <class Tc, int DP> constexpr size_t tile_bytes(int rows) { return 4 * (size_t)rows * tile_stride<Tc, DP>() * sizeof(Tc); }  // two tensors, two buffers
 int table_entries(const Args* a) { return 2 * a->reach + 1 + 2 * kPad; }
 
 template <class K> int prepare_lds(K kernel, size_t bytes) {
@@ -784,7 +824,7 @@ template <class Tin, class Tc, class Tg, int DP> struct Passes {
       attention_rows<Tin, Tc, DP><<<a.batch * a.kv_heads * splits, 256, lds, st>>>(a, splits, work);
       if (splits > 1) attention_join<Tin><<<a.batch * a.kv_heads * rows, 128, 0, st>>>(a, splits, DP, work);
     } else {
-      const size_t lds = tile_bytes(sizeof(Tc), DP) + 4 * (size_t)table_entries(&a);
+      const size_t lds = tile_bytes<Tc, DP>(key_tile<DP>()) + 4 * (size_t)table_entries(&a);
       if (int e = prepare_lds(attention_forward<Tin, Tc, DP>, lds)) return e;
       const int nqb = (int)((a.queries + 127) / 128);
       attention_forward<Tin, Tc, DP><<<a.batch * a.heads * nqb, 256, lds, st>>>(a);
@@ -793,12 +833,12 @@ template <class Tin, class Tc, class Tg, int DP> struct Passes {
   }
   static int backward(const Args& a, float* work, hipStream_t st) {
     const int nqb = (int)((a.queries + 127) / 128), nkb = (int)((a.keys + 127) / 128);
-    const size_t tb = tile_bytes(sizeof(Tg), DP), te = 4 * (size_t)table_entries(&a);
+    const size_t tb = tile_bytes<Tg, DP>(key_tile<DP>()), te = 4 * (size_t)table_entries(&a);
     if (int e = prepare_lds(attention_grad_q<Tin, Tg, DP>, tb + te)) return e;
     attention_grad_q<Tin, Tg, DP><<<a.batch * a.heads * nqb, 256, tb + te, st>>>(a);
     if (nkb > 0) {
       float* part = a.grad_bias ? work : nullptr;
-      const size_t lds = tb + 4 * key_tile<Tg>() * 4 + 5 * te;
+      const size_t lds = tile_bytes<Tg, DP>(query_tile<Tg>()) + 4 * query_tile<Tg>() * sizeof(float) + 5 * te;
       if (int e = prepare_lds(attention_grad_kv<Tin, Tg, DP>, lds)) return e;
       attention_grad_kv<Tin, Tg, DP><<<a.batch * a.kv_heads * nkb, 256, lds, st>>>(a, part);
     }

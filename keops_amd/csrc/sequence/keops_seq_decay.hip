@@ -55,7 +55,7 @@ __device__ inline int length_of(const Args& A, int b) {
 // S = g^n S + sum_j weight_j k_j v_j^T of the chunk in LDS (n tokens); wavefront's 32 columns of v
 template <class Tc, int DK, int DV>
 __device__ inline void update_state(f32x16 (&S)[DK / 32], const Tc* kt, const Tc* vt, const float* pw, int n, int shift, float scale, int wave, int lane) {
-  constexpr int SK = tile_stride<Tc, DK>(), SV = tile_stride<Tc, DV>(), NT = update_terms<Tc>();
+  constexpr int NT = update_terms<Tc>();
   const int half = lane >> 5;
   const float all = pw[kZero + n];
 #pragma unroll
@@ -65,7 +65,7 @@ __device__ inline void update_state(f32x16 (&S)[DK / 32], const Tc* kt, const Tc
   const float* w = pw + kZero + n - 1 + shift - 4 * half;  // weight of token j is w[-j], zero behind the chunk's end
 #pragma unroll
   for (int s = 0; s < C / 16; s++) {
-    const typename Vec<Tc>::x8 v = frag_cols<Tc>(vt, SV, 16 * s, 32 * wave, lane);
+    const typename Vec<Tc>::x8 v = frag_cols<Tc, DV>(vt, 16 * s, 32 * wave, lane);
     float x[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) x[j] = (float)v[j] * (w[-(16 * s + (j & 3) + 2 * (j & 4))] * scale);
@@ -73,7 +73,7 @@ __device__ inline void update_state(f32x16 (&S)[DK / 32], const Tc* kt, const Tc
     t.set(x);
 #pragma unroll
     for (int i = 0; i < DK / 32; i++) {
-      const typename Vec<Tc>::x8 k = frag_cols<Tc>(kt, SK, 16 * s, 32 * i, lane);
+      const typename Vec<Tc>::x8 k = frag_cols<Tc, DK>(kt, 16 * s, 32 * i, lane);
 #pragma unroll
       for (int m = 0; m < NT; m++) S[i] = mma(k, t.t[m], S[i]);
     }
@@ -84,7 +84,7 @@ __device__ inline void update_state(f32x16 (&S)[DK / 32], const Tc* kt, const Tc
 //
 // Few sequences and heads do not fill the chip, so a long sequence is cut into segments: their own states first (this kernel),
 // then decay_scan carries them on, then decay_outputs starts every segment from its state.
-template <class Tin, class Tc, int DK, int DV>
+template <class Tin, class Tc, int DK, int DV, bool REV>
 __global__ void __launch_bounds__(2 * DV, 1) decay_states(const Args A, int segments, int seg_tokens, float* states) {
   constexpr int NT = 2 * DV, SK = tile_stride<Tc, DK>(), SV = tile_stride<Tc, DV>();
   extern __shared__ __align__(16) unsigned char smem[];
@@ -95,21 +95,18 @@ __global__ void __launch_bounds__(2 * DV, 1) decay_states(const Args A, int segm
   const int unit = blockIdx.x / segments, seg = blockIdx.x % segments, b = unit / A.heads, h = unit % A.heads;
   const int len = length_of(A, b), t0 = seg * seg_tokens, t1 = min(len, t0 + seg_tokens);
   fill_powers(pw, A.log_decay[h], tid, NT);
-  const Tin* k = rows_of<Tin>(A.k, A.k_stride, b, h / (A.heads / A.k_heads));
-  const Tin* v = rows_of<Tin>(A.v, A.v_stride, b, h / (A.heads / A.v_heads));
-  long long ks = A.k_stride[2], vs = A.v_stride[2];
-  if (A.reverse && len > 0) {
-    k += (long long)(len - 1) * ks; ks = -ks;
-    v += (long long)(len - 1) * vs; vs = -vs;
-  }
+  const Tin* const k = rows_of<Tin>(A.k, A.k_stride, b, h / (A.heads / A.k_heads));
+  const Tin* const v = rows_of<Tin>(A.v, A.v_stride, b, h / (A.heads / A.v_heads));
+  const long long ks = A.k_stride[2], vs = A.v_stride[2];
+  const auto at = [&](int t) -> long long { return REV ? len - 1 - t : t; };  // row of the t-th token of the walk
   f32x16 S[DK / 32];
 #pragma unroll
   for (int i = 0; i < DK / 32; i++) S[i] = zero16();
-  Staged<Tin, Tc, C, DK, NT> sk;
-  Staged<Tin, Tc, C, DV, NT> sv;
+  Staged<Tin, Tc, C, DK, NT, REV> sk;
+  Staged<Tin, Tc, C, DV, NT, REV> sv;
   if (t0 < t1) {
-    sk.load(k, ks, t0, t1, A.dim, tid);
-    sv.load(v, vs, t0, t1, A.dim_v, tid);
+    sk.load(k + at(t0) * ks, ks, t1 - t0, A.dim, tid);
+    sv.load(v + at(t0) * vs, vs, t1 - t0, A.dim_v, tid);
   }
   for (int t = t0; t < t1; t += C) {
     __syncthreads();
@@ -117,10 +114,10 @@ __global__ void __launch_bounds__(2 * DV, 1) decay_states(const Args A, int segm
     sv.store(vt, tid);
     __syncthreads();
     if (t + C < t1) {
-      sk.load(k, ks, t + C, t1, A.dim, tid);
-      sv.load(v, vs, t + C, t1, A.dim_v, tid);
+      sk.load(k + at(t + C) * ks, ks, t1 - t - C, A.dim, tid);
+      sv.load(v + at(t + C) * vs, vs, t1 - t - C, A.dim_v, tid);
     }
-    update_state<Tc, DK, DV>(S, kt, vt, pw, min(C, t1 - t), A.reverse, A.update_scale, wave, lane);
+    update_state<Tc, DK, DV>(S, kt, vt, pw, min(C, t1 - t), REV ? 1 : 0, A.update_scale, wave, lane);
   }
   float* out = states + (long long)blockIdx.x * A.dim * A.dim_v;
   const int c = 32 * wave + col;
@@ -152,7 +149,7 @@ __global__ void __launch_bounds__(256) decay_scan(const Args A, int segments, in
 }
 
 // ---- outputs --------------------------------------------------------------------------------------------------------------------
-template <class Tin, class Tc, int DK, int DV>
+template <class Tin, class Tc, int DK, int DV, bool REV>
 __global__ void __launch_bounds__(2 * DV, 1) decay_outputs(const Args A, int segments, int seg_tokens, const float* states) {
   constexpr int NT = 2 * DV, NW = DV / 32, SK = tile_stride<Tc, DK>(), SV = tile_stride<Tc, DV>(), SP = tile_stride<Tc, C>();
   extern __shared__ __align__(16) unsigned char smem[];
@@ -164,21 +161,17 @@ __global__ void __launch_bounds__(2 * DV, 1) decay_outputs(const Args A, int seg
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
   const int unit = blockIdx.x / segments, seg = blockIdx.x % segments, b = unit / A.heads, h = unit % A.heads;
   const int len = length_of(A, b), t0 = seg * seg_tokens, t1 = min(len, t0 + seg_tokens);
-  const int c = 32 * wave + col, shift = A.reverse ? 0 : 1;
+  const int c = 32 * wave + col, shift = REV ? 0 : 1;
   fill_powers(pw, A.log_decay[h], tid, NT);
-  const Tin* q = rows_of<Tin>(A.q, A.q_stride, b, h / (A.heads / A.q_heads));
-  const Tin* k = rows_of<Tin>(A.k, A.k_stride, b, h / (A.heads / A.k_heads));
-  const Tin* v = rows_of<Tin>(A.v, A.v_stride, b, h / (A.heads / A.v_heads));
-  long long qs = A.q_stride[2], ks = A.k_stride[2], vs = A.v_stride[2];
-  if (A.reverse && len > 0) {
-    q += (long long)(len - 1) * qs; qs = -qs;
-    k += (long long)(len - 1) * ks; ks = -ks;
-    v += (long long)(len - 1) * vs; vs = -vs;
-  }
+  const Tin* const q = rows_of<Tin>(A.q, A.q_stride, b, h / (A.heads / A.q_heads));
+  const Tin* const k = rows_of<Tin>(A.k, A.k_stride, b, h / (A.heads / A.k_heads));
+  const Tin* const v = rows_of<Tin>(A.v, A.v_stride, b, h / (A.heads / A.v_heads));
+  const long long qs = A.q_stride[2], ks = A.k_stride[2], vs = A.v_stride[2];
+  const auto at = [&](int t) -> long long { return REV ? len - 1 - t : t; };  // row of the t-th token of the walk
   const long long out0 = (long long)b * A.out_stride[0] + (long long)h * A.out_stride[1];
   auto put = [&](int t, int d, float x) {  // component d of token t (in the order of the walk)
-    const long long at = out0 + (long long)(A.reverse && t < len ? len - 1 - t : t) * A.out_stride[2] + d;
-    if (A.out_float32) ((float*)A.out)[at] = x; else ((Tin*)A.out)[at] = (Tin)x;
+    const long long place = out0 + (t < len ? at(t) : t) * A.out_stride[2] + d;
+    if (A.out_float32) ((float*)A.out)[place] = x; else ((Tin*)A.out)[place] = (Tin)x;
   };
 
   f32x16 S[DK / 32];
@@ -193,12 +186,12 @@ __global__ void __launch_bounds__(2 * DV, 1) decay_outputs(const Args A, int seg
         S[i][r] = from && d < A.dim && c < A.dim_v ? from[d * s0 + c * s1] : 0.f;
       }
   }
-  Staged<Tin, Tc, C, DK, NT> sq, sk;
-  Staged<Tin, Tc, C, DV, NT> sv;
+  Staged<Tin, Tc, C, DK, NT, REV> sq, sk;
+  Staged<Tin, Tc, C, DV, NT, REV> sv;
   if (t0 < t1) {
-    sq.load(q, qs, t0, t1, A.dim, tid);
-    sk.load(k, ks, t0, t1, A.dim, tid);
-    sv.load(v, vs, t0, t1, A.dim_v, tid);
+    sq.load(q + at(t0) * qs, qs, t1 - t0, A.dim, tid);
+    sk.load(k + at(t0) * ks, ks, t1 - t0, A.dim, tid);
+    sv.load(v + at(t0) * vs, vs, t1 - t0, A.dim_v, tid);
   }
   for (int t = t0; t < t1; t += C) {
     __syncthreads();
@@ -207,23 +200,23 @@ __global__ void __launch_bounds__(2 * DV, 1) decay_outputs(const Args A, int seg
     sv.store(vt, tid);
     __syncthreads();
     if (t + C < t1) {
-      sq.load(q, qs, t + C, t1, A.dim, tid);
-      sk.load(k, ks, t + C, t1, A.dim, tid);
-      sv.load(v, vs, t + C, t1, A.dim_v, tid);
+      sq.load(q + at(t + C) * qs, qs, t1 - t - C, A.dim, tid);
+      sk.load(k + at(t + C) * ks, ks, t1 - t - C, A.dim, tid);
+      sv.load(v + at(t + C) * vs, vs, t1 - t - C, A.dim_v, tid);
     }
     // decayed products within the chunk: three 32 x 32 tiles (rows tokens j, columns tokens i >= j), shared through LDS
     for (int tile = wave; tile < 3; tile += NW) {
       const int i0 = tile == 0 ? 0 : 32, j0 = tile == 2 ? 32 : 0;
       f32x16 a = zero16();
 #pragma unroll
-      for (int s = 0; s < DK / 16; s++) a = mma(frag_rows(kt + (j0 + col) * SK, 16 * s, half), frag_rows(qt + (i0 + col) * SK, 16 * s, half), a);
+      for (int s = 0; s < DK / 16; s++) a = mma(frag_rows<Tc, DK>(kt, j0 + col, 16 * s, half), frag_rows<Tc, DK>(qt, i0 + col, 16 * s, half), a);
       const float* w = pw + kZero + i0 + col - j0 - 4 * half;
 #pragma unroll
       for (int g = 0; g < 4; g++) {
         float x[4];
 #pragma unroll
         for (int u = 0; u < 4; u++) x[u] = i0 + col >= j0 + 8 * g + 4 * half + u ? a[4 * g + u] * (w[-(8 * g + u)] * A.product_scale) : 0.f;
-        store4<Tc>(pt + (i0 + col) * SP + j0 + 8 * g + 4 * half, x[0], x[1], x[2], x[3]);
+        store4<Tc>(pt + tile_at<Tc, C>(i0 + col, j0 + 8 * g + 4 * half), x[0], x[1], x[2], x[3]);
       }
     }
     __syncthreads();
@@ -240,7 +233,7 @@ __global__ void __launch_bounds__(2 * DV, 1) decay_outputs(const Args A, int seg
         st.set(x);
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-          const typename Vec<Tc>::x8 qf = frag_rows_split(qt + (32 * u + col) * SK, 32 * i + 16 * s, half);
+          const typename Vec<Tc>::x8 qf = frag_rows_split<Tc, DK>(qt, 32 * u + col, 32 * i + 16 * s, half);
 #pragma unroll
           for (int m = 0; m < state_terms<Tc>(); m++) o[u] = mma(qf, st.t[m], o[u]);
         }
@@ -250,7 +243,7 @@ __global__ void __launch_bounds__(2 * DV, 1) decay_outputs(const Args A, int seg
 #pragma unroll
       for (int r = 0; r < 16; r++) o[u][r] *= pw[kZero + 32 * u + c_row(r, half) + shift] * A.query_scale;
 #pragma unroll
-      for (int s = 0; s < 2 * (u + 1); s++) o[u] = mma(frag_rows_split(pt + (32 * u + col) * SP, 16 * s, half), frag_cols<Tc>(vt, SV, 16 * s, 32 * wave, lane), o[u]);
+      for (int s = 0; s < 2 * (u + 1); s++) o[u] = mma(frag_rows_split<Tc, C>(pt, 32 * u + col, 16 * s, half), frag_cols<Tc, DV>(vt, 16 * s, 32 * wave, lane), o[u]);
     }
     if (c < A.dim_v) {
 #pragma unroll
@@ -262,7 +255,7 @@ __global__ void __launch_bounds__(2 * DV, 1) decay_outputs(const Args A, int seg
         }
     }
     if (segments == 1 ? (A.state_out || t + C < t1) : t + C < t1)
-      update_state<Tc, DK, DV>(S, kt, vt, pw, min(C, t1 - t), A.reverse, A.update_scale, wave, lane);
+      update_state<Tc, DK, DV>(S, kt, vt, pw, min(C, t1 - t), REV ? 1 : 0, A.update_scale, wave, lane);
   }
   // tokens behind the sequence
   for (int t = max(t0, len); t < min((int)A.tokens, t0 + seg_tokens); t++)
@@ -355,6 +348,8 @@ const char* check(const Args* a) {
   if (a->dim < ve || a->dim > 128 || a->dim % ve || a->dim_v < ve || a->dim_v > 128 || a->dim_v % ve)
     return "decay attention: dim and dim_v must be multiples of 16 bytes, at most 128";
   if (a->tokens < 0 || a->tokens > (1 << 29)) return "decay attention: tokens out of range";
+  for (const int64_t* x : {a->q_stride, a->k_stride, a->v_stride})
+    if (x[2] < 0 || x[2] > kMaxRowStride) return "decay attention: rows too far apart";
   if (!a->log_decay || (a->tokens > 0 && (!a->q || !a->k || !a->v || !a->out))) return "decay attention: null data";
   if ((int64_t)a->batch * a->heads > 65535) return "decay attention: more than 65535 sequences times heads";
   return nullptr;
@@ -377,25 +372,29 @@ template <class K> int prepare_lds(K kernel, size_t bytes) {
   return e == hipSuccess ? 0 : keops_seq_fail((int)e, "decay attention: shared memory");
 }
 
-template <class Tin, class Tc, int DK, int DV> int run(const Args& a, float* work, hipStream_t st) {
+template <class Tin, class Tc, int DK, int DV, bool REV> int run(const Args& a, float* work, hipStream_t st) {
   int segments, seg_tokens;
   segments_of(&a, segments, seg_tokens);
   const int units = a.batch * a.heads;
   const size_t kv = (size_t)C * (tile_stride<Tc, DK>() + tile_stride<Tc, DV>()) * sizeof(Tc), pw = kPowers * sizeof(float);
   const size_t all = kv + (size_t)C * (tile_stride<Tc, DK>() + tile_stride<Tc, C>()) * sizeof(Tc) + pw;
   if (segments > 1) {
-    if (int e = prepare_lds(decay_states<Tin, Tc, DK, DV>, kv + pw)) return e;
-    decay_states<Tin, Tc, DK, DV><<<units * segments, 2 * DV, kv + pw, st>>>(a, segments, seg_tokens, work);
+    if (int e = prepare_lds(decay_states<Tin, Tc, DK, DV, REV>, kv + pw)) return e;
+    decay_states<Tin, Tc, DK, DV, REV><<<units * segments, 2 * DV, kv + pw, st>>>(a, segments, seg_tokens, work);
     decay_scan<<<dim3((a.dim * a.dim_v + 255) / 256, units), 256, 0, st>>>(a, segments, seg_tokens, work);
   }
-  if (int e = prepare_lds(decay_outputs<Tin, Tc, DK, DV>, all)) return e;
-  decay_outputs<Tin, Tc, DK, DV><<<units * segments, 2 * DV, all, st>>>(a, segments, seg_tokens, work);
+  if (int e = prepare_lds(decay_outputs<Tin, Tc, DK, DV, REV>, all)) return e;
+  decay_outputs<Tin, Tc, DK, DV, REV><<<units * segments, 2 * DV, all, st>>>(a, segments, seg_tokens, work);
   return seq_launched("decay attention: launch");
 }
 
+template <class Tin, class Tc, bool REV> int by_dims(const Args& a, float* work, hipStream_t st) {
+  if (a.dim <= 64) return a.dim_v <= 64 ? run<Tin, Tc, 64, 64, REV>(a, work, st) : run<Tin, Tc, 64, 128, REV>(a, work, st);
+  return a.dim_v <= 64 ? run<Tin, Tc, 128, 64, REV>(a, work, st) : run<Tin, Tc, 128, 128, REV>(a, work, st);
+}
+
 template <class Tin, class Tc> int dispatch(const Args& a, float* work, hipStream_t st) {
-  if (a.dim <= 64) return a.dim_v <= 64 ? run<Tin, Tc, 64, 64>(a, work, st) : run<Tin, Tc, 64, 128>(a, work, st);
-  return a.dim_v <= 64 ? run<Tin, Tc, 128, 64>(a, work, st) : run<Tin, Tc, 128, 128>(a, work, st);
+  return a.reverse ? by_dims<Tin, Tc, true>(a, work, st) : by_dims<Tin, Tc, false>(a, work, st);
 }
 
 template <class T>

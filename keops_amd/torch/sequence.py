@@ -51,11 +51,15 @@ def _check_whole(what, name, t, shape, device):
     return t.to(torch.int32).contiguous()
 
 
+_MAX_ROW_STRIDE = 1 << 23  # kMaxRowStride of csrc/sequence/keops_seq.h
+
+
 def _rows(x):
-    """x with rows as the kernels read them: neighbouring components, every row at a multiple of 16 bytes (a copy if not)."""
+    """x with rows as the kernels read them: neighbouring components, every row at a multiple of 16 bytes and not too far from the
+    next (a copy if not)."""
     size = x.element_size()
     if x.numel() == 0 or (
-        x.stride(-1) == 1 and x.data_ptr() % 16 == 0
+        x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and (x.shape[-2] == 1 or x.stride(-2) <= _MAX_ROW_STRIDE)
         and all(s * size % 16 == 0 for s, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1)
     ):
         return x
@@ -81,7 +85,8 @@ def _ptr(t):
 
 
 def _stride(t):
-    return t.stride()[:3]
+    b, h, r = t.stride()[:3]
+    return b, h, r if t.shape[2] > 1 else 0
 
 
 def _needs_grad(*tensors):
@@ -246,7 +251,7 @@ def bucket_attention(q, k, v, bias, buckets, *, causal=False, key_lengths=None, 
             2**29.  For one new token against a cache that already holds its key: ``key_lengths - 1``.
         scale: default ``dim ** -0.5``.
 
-    A query that sees no key has output 0 and gives no gradient.  Keys that are only hidden by ``causal`` are read with their
+    A bias of -6e4 or less (``-inf``, the lowest value of a type) hides its pairs.  A query that sees no key has output 0 and gives no gradient.  Keys that are only hidden by ``causal`` are read with their
     tile: a value that is not finite there can reach earlier queries.
 
     Returns (batch, heads, queries, dim) in the type and order of dimensions of q.  Differentiable with respect to q, k, v and
