@@ -231,10 +231,17 @@ typedef struct keops_hip_decay_attention {
   const float* state_in;          /* (batch, heads) matrices of dim * dim_v contiguous values, or NULL: zeros */
   float* state_out;               /* the same, or NULL */
   int64_t state_in_stride[2], state_out_stride[2]; /* strides of a matrix along dim and along dim_v */
+  /* Workspace of keops_hip_decay_attention_bytes bytes: a call leaves in it the states before the segments that it cuts long
+     sequences into.  states_given = 1: it holds them already, from a call with the same batch, heads, tokens, lengths,
+     direction, and either the same dim, dim_v, k, v, scale and state_in or all of these exchanged (states_stride tells which:
+     (dim_v, 1), or (1, dim) for their transposes); no final state then. */
+  float* states;
+  int64_t states_bytes, states_stride[2];
+  int32_t states_given, reserved_states;
 } keops_hip_decay_attention;
 
 size_t keops_hip_decay_attention_bytes(const keops_hip_decay_attention* a);
-int keops_hip_decay_attention_run(const keops_hip_decay_attention* a, void* work, size_t work_bytes, int device, void* hip_stream);
+int keops_hip_decay_attention_run(const keops_hip_decay_attention* a, int device, void* hip_stream);
 
 /* One token: state (batch, heads, dim, dim_v) becomes g state + k v^T in place, out = scale q state.  q, k, v, out: strides of
    (batch, head); rows need not be aligned beyond their elements. */

@@ -36,7 +36,8 @@ class DecayAttention(ctypes.Structure):
         + [("tokens", _I64)] + [(n, _F32) for n in ("product_scale", "query_scale", "update_scale", "reserved")]
         + [(n, _P) for n in ("q", "k", "v", "out")] + [(n + "_stride", _I64 * 3) for n in ("q", "k", "v", "out")]
         + [(n, _P) for n in ("log_decay", "lengths", "state_in", "state_out")]
-        + [("state_in_stride", _I64 * 2), ("state_out_stride", _I64 * 2)]
+        + [("state_in_stride", _I64 * 2), ("state_out_stride", _I64 * 2), ("states", _P), ("states_bytes", _I64),
+           ("states_stride", _I64 * 2), ("states_given", _I32), ("reserved_states", _I32)]
     )
 
 
@@ -88,7 +89,9 @@ def lib():
             for p in passes:
                 size = getattr(L, f"keops_hip_{name}{p}_bytes")
                 size.restype, size.argtypes = _SIZE, [ctypes.POINTER(struct)]
-                getattr(L, f"keops_hip_{name}{p or '_run'}").argtypes = [ctypes.POINTER(struct), _P, _SIZE, ctypes.c_int, _P]
+                if p:
+                    getattr(L, f"keops_hip_{name}{p}").argtypes = [ctypes.POINTER(struct), _P, _SIZE, ctypes.c_int, _P]
+        L.keops_hip_decay_attention_run.argtypes = [ctypes.POINTER(DecayAttention), ctypes.c_int, _P]
         L.keops_hip_decay_attention_step.argtypes = [ctypes.c_int] * 6 + [_F32] + [_P] * 9 + [ctypes.c_int, _P]
         L.keops_hip_token_logprobs_bytes.restype = _SIZE
         L.keops_hip_token_logprobs_bytes.argtypes = [ctypes.c_int, _I64, _I64, ctypes.c_int]

@@ -401,23 +401,46 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_rows(const A
   }
 }
 
-// the shares of one row, joined in their order
-template <class Tin> __global__ void __launch_bounds__(128) attention_join(const Args A, int splits, int dp, const float* part) {
-  const int group = A.heads / A.kv_heads, M = (int)A.queries, rows = group * M;
+// the shares of one row, joined in an order that is always the same: four groups of threads take every fourth share
+template <class Tin> __global__ void __launch_bounds__(512) attention_join(const Args A, int splits, int dp, const float* part) {
+  __shared__ float weight[256], sums[4][128], red[8];
+  const int tid = threadIdx.x, lane = tid & 63, group = A.heads / A.kv_heads, M = (int)A.queries, rows = group * M;
   const int unit = blockIdx.x / rows, r = blockIdx.x % rows, b = unit / A.kv_heads, h = (unit % A.kv_heads) * group + r / M, qi = r % M;
-  const float* p = part + ((long long)unit * splits * rows + r) * (dp + 2);
   const long long step = (long long)rows * (dp + 2);
-  float mm = -kInf;
-  for (int s = 0; s < splits; s++) mm = fmaxf(mm, p[s * step]);
-  float ll = 0.f, o = 0.f;
-  const int d = threadIdx.x;
-  for (int s = 0; s < splits; s++) {
-    const float ms = p[s * step], a = ms == mm ? 1.f : __builtin_amdgcn_exp2f(ms - mm);
-    ll += a * p[s * step + 1];
-    if (d < A.dim) o += a * p[s * step + 2 + d];
+  const float* p = part + ((long long)unit * splits * rows + r) * (dp + 2);
+  float m = -kInf, l = 0.f;
+  if (tid < splits) {  // (at most 256)
+    m = p[tid * step];
+    l = p[tid * step + 1];
   }
-  if (d < A.dim) rows_of<Tin>(A.out, A.out_stride, b, h)[(long long)qi * A.out_stride[2] + d] = (Tin)(ll == 0.f ? 0.f : o / ll);
-  if (A.lse && d == 0) A.lse[((long long)b * A.heads + h) * M + qi] = ll == 0.f ? kInf : mm + __builtin_amdgcn_logf(ll);
+  float mm = m;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
+  if (lane == 0) red[tid >> 6] = mm;
+  __syncthreads();
+  mm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float a = m == mm ? 1.f : __builtin_amdgcn_exp2f(m - mm);
+  if (tid < 256) weight[tid] = a;
+  float ll = tid < splits ? a * l : 0.f;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) ll += __shfl_xor(ll, o);
+  __syncthreads();
+  if (lane == 0) red[tid >> 6] = ll;
+  __syncthreads();
+  ll = (red[0] + red[1]) + (red[2] + red[3]);
+  const int d = tid & 127, first = tid >> 7;
+  float o = 0.f;
+  if (d < A.dim) {
+#pragma unroll 8
+    for (int s = first; s < splits; s += 4) o = fmaf(weight[s], p[s * step + 2 + d], o);
+  }
+  sums[first][d] = o;
+  __syncthreads();
+  if (tid < A.dim) {
+    o = (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
+    rows_of<Tin>(A.out, A.out_stride, b, h)[(long long)qi * A.out_stride[2] + d] = (Tin)(ll == 0.f ? 0.f : o / ll);
+  }
+  if (A.lse && tid == 0) A.lse[((long long)b * A.heads + h) * M + qi] = ll == 0.f ? kInf : mm + __builtin_amdgcn_logf(ll);
 }
 
 // ---- gradient of the queries ------------------------------------------------------------------------------------------------
@@ -822,7 +845,7 @@ template <class Tin, class Tc, class Tg, int DP> struct Passes {
       const size_t v = 4 * 32 * (size_t)tile_stride<Tc, DP>() * sizeof(Tc), o = 4 * (size_t)rows * (DP + 2) * 4, lds = v > o ? v : o;
       if (int e = prepare_lds(attention_rows<Tin, Tc, DP>, lds)) return e;
       attention_rows<Tin, Tc, DP><<<a.batch * a.kv_heads * splits, 256, lds, st>>>(a, splits, work);
-      if (splits > 1) attention_join<Tin><<<a.batch * a.kv_heads * rows, 128, 0, st>>>(a, splits, DP, work);
+      if (splits > 1) attention_join<Tin><<<a.batch * a.kv_heads * rows, 512, 0, st>>>(a, splits, DP, work);
     } else {
       const size_t lds = tile_bytes<Tc, DP>(key_tile<DP>()) + 4 * (size_t)table_entries(&a);
       if (int e = prepare_lds(attention_forward<Tin, Tc, DP>, lds)) return e;

@@ -17,7 +17,7 @@ typedef keops_hip_decay_attention Args;
 
 constexpr int C = 64;  // tokens of a chunk
 
-// x as a sum of NT terms of the operand's type; bf16: two terms hold 16 bits, three all 24 of a float32
+// x as a sum of NT terms of the operand's type; bf16: one term holds 8 bits, two 16, three all 24 of a float32
 template <class T, int NT> struct Terms {
   typename Vec<T>::x8 t[NT];
   __device__ inline void set(const float (&x)[8]) {
@@ -33,8 +33,10 @@ template <class T, int NT> struct Terms {
     }
   }
 };
-template <class Tc> constexpr int state_terms() { return sizeof(Tc) == 2 ? 2 : 1; }   // the state as an operand for the output
-template <class Tc> constexpr int update_terms() { return sizeof(Tc) == 2 ? 3 : 1; }  // decayed values as an operand for the state
+// Decayed values as an operand for the state: all of a float32 where the state is a result (or becomes one over the segments
+// behind), 16 bits where it only serves outputs that are rounded to 8.  The state itself is float32; as an operand for those
+// outputs it is rounded once, as the products within the chunk are.
+template <class Tc, bool RESULT> constexpr int update_terms() { return sizeof(Tc) == 2 ? (RESULT ? 3 : 2) : 1; }
 
 // powers of the decay in LDS: entry kZero + n holds g^n for n = 0..C, zeros before and behind
 constexpr int kZero = 64, kPowers = kZero + C + 8;
@@ -53,9 +55,8 @@ __device__ inline int length_of(const Args& A, int b) {
 }
 
 // S = g^n S + sum_j weight_j k_j v_j^T of the chunk in LDS (n tokens); wavefront's 32 columns of v
-template <class Tc, int DK, int DV>
+template <class Tc, int DK, int DV, int NT>
 __device__ inline void update_state(f32x16 (&S)[DK / 32], const Tc* kt, const Tc* vt, const float* pw, int n, int shift, float scale, int wave, int lane) {
-  constexpr int NT = update_terms<Tc>();
   const int half = lane >> 5;
   const float all = pw[kZero + n];
 #pragma unroll
@@ -85,13 +86,14 @@ __device__ inline void update_state(f32x16 (&S)[DK / 32], const Tc* kt, const Tc
 // Few sequences and heads do not fill the chip, so a long sequence is cut into segments: their own states first (this kernel),
 // then decay_scan carries them on, then decay_outputs starts every segment from its state.
 template <class Tin, class Tc, int DK, int DV, bool REV>
-__global__ void __launch_bounds__(2 * DV, 1) decay_states(const Args A, int segments, int seg_tokens, float* states) {
+__global__ void __launch_bounds__(2 * DV, sizeof(Tc) == 2 ? 2 : 1) decay_states(const Args A, int segments, int seg_tokens, float* states) {
   constexpr int NT = 2 * DV, SK = tile_stride<Tc, DK>(), SV = tile_stride<Tc, DV>();
   extern __shared__ __align__(16) unsigned char smem[];
   Tc* const kt = (Tc*)smem;
   Tc* const vt = kt + C * SK;
   float* const pw = (float*)(vt + C * SV);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int lane = tid & 63;
   const int unit = blockIdx.x / segments, seg = blockIdx.x % segments, b = unit / A.heads, h = unit % A.heads;
   const int len = length_of(A, b), t0 = seg * seg_tokens, t1 = min(len, t0 + seg_tokens);
   fill_powers(pw, A.log_decay[h], tid, NT);
@@ -109,6 +111,7 @@ __global__ void __launch_bounds__(2 * DV, 1) decay_states(const Args A, int segm
     sv.load(v + at(t0) * vs, vs, t1 - t0, A.dim_v, tid);
   }
   for (int t = t0; t < t1; t += C) {
+    asm volatile("" : "+v"(lane));  // places in LDS are formed anew in every chunk
     __syncthreads();
     sk.store(kt, tid);
     sv.store(vt, tid);
@@ -117,8 +120,9 @@ __global__ void __launch_bounds__(2 * DV, 1) decay_states(const Args A, int segm
       sk.load(k + at(t + C) * ks, ks, t1 - t - C, A.dim, tid);
       sv.load(v + at(t + C) * vs, vs, t1 - t - C, A.dim_v, tid);
     }
-    update_state<Tc, DK, DV>(S, kt, vt, pw, min(C, t1 - t), REV ? 1 : 0, A.update_scale, wave, lane);
+    update_state<Tc, DK, DV, update_terms<Tc, true>()>(S, kt, vt, pw, min(C, t1 - t), REV ? 1 : 0, A.update_scale, wave, lane);
   }
+  const int half = lane >> 5, col = lane & 31;
   float* out = states + (long long)blockIdx.x * A.dim * A.dim_v;
   const int c = 32 * wave + col;
 #pragma unroll
@@ -139,26 +143,69 @@ __global__ void __launch_bounds__(256) decay_scan(const Args A, int segments, in
   const float lg = A.log_decay[h], whole = power(lg, seg_tokens);
   float x = A.state_in ? A.state_in[(long long)unit * size + d * A.state_in_stride[0] + c * A.state_in_stride[1]] : 0.f;
   float* s = states + (long long)unit * segments * size + e;
-  for (int g = 0; g < segments; g++) {
-    const int n = min(max(len - g * seg_tokens, 0), seg_tokens);
-    const float own = s[(long long)g * size];
-    s[(long long)g * size] = x;
-    x = (n == seg_tokens ? whole : power(lg, n)) * x + own;
+  constexpr int U = 16;  // loads in flight
+  for (int g0 = 0; g0 < segments; g0 += U) {
+    float own[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) own[u] = g0 + u < segments ? s[(long long)(g0 + u) * size] : 0.f;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int g = g0 + u;
+      if (g >= segments) break;
+      const int n = min(max(len - g * seg_tokens, 0), seg_tokens);
+      s[(long long)g * size] = x;
+      x = (n == seg_tokens ? whole : power(lg, n)) * x + own[u];
+    }
   }
   if (A.state_out) A.state_out[(long long)unit * size + d * A.state_out_stride[0] + c * A.state_out_stride[1]] = x;
 }
 
 // ---- outputs --------------------------------------------------------------------------------------------------------------------
-template <class Tin, class Tc, int DK, int DV, bool REV>
-__global__ void __launch_bounds__(2 * DV, 1) decay_outputs(const Args A, int segments, int seg_tokens, const float* states) {
+
+// Two C tiles (rows: 64 tokens, columns: the wavefront's 32 components) to memory, 16 bytes a lane, through 4096 bytes of LDS that
+// belong to the wavefront (`strip`)
+template <class T, bool REV>
+__device__ inline void store_rows(T* out, long long stride, const f32x16 (&o)[2], void* strip, int t, int t1, int len, int wave, int lane, int dim_v) {
+  constexpr int VE = 16 / (int)sizeof(T), PER_ROW = 32 / VE;
+  T* const tile = (T*)strip;
+  const int half = lane >> 5, col = lane & 31, row0 = lane / PER_ROW, c = 32 * wave + (lane % PER_ROW) * VE;
+#pragma unroll
+  for (int u = 0; u < 2; u++) {
+#pragma unroll
+    for (int r = 0; r < 16; r++) tile[c_row(r, half) * 32 + col] = (T)o[u][r];
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int i = 0; i < PER_ROW / 2; i++) {
+      const int row = row0 + i * (64 / PER_ROW), token = t + 32 * u + row;
+      const uint4 x = *reinterpret_cast<const uint4*>(tile + row * 32 + (lane % PER_ROW) * VE);
+      if (token < t1 && c < dim_v) *reinterpret_cast<uint4*>(out + (long long)(REV ? len - 1 - token : token) * stride + c) = x;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+}
+
+template <class Tc, int DK, int DV> constexpr size_t query_bytes() {
+  constexpr size_t q = (size_t)C * tile_stride<Tc, DK>() * sizeof(Tc), o = 4096 * (DV / 32);
+  return q > o ? q : o;
+}
+
+// CUT: sequences are cut into segments, whose states are known
+template <class Tin, class Tc, int DK, int DV, bool REV, bool CUT>
+__global__ void __launch_bounds__(2 * DV, sizeof(Tc) == 2 && DK <= DV ? 2 : 1) decay_outputs(const Args A, int segments, int seg_tokens, const float* states) {
   constexpr int NT = 2 * DV, NW = DV / 32, SK = tile_stride<Tc, DK>(), SV = tile_stride<Tc, DV>(), SP = tile_stride<Tc, C>();
   extern __shared__ __align__(16) unsigned char smem[];
-  Tc* const qt = (Tc*)smem;
-  Tc* const kt = qt + C * SK;
+  Tc* const qt = (Tc*)smem;  // and, once the chunk's queries have been used, the outputs on their way
+  Tc* const kt = (Tc*)(smem + query_bytes<Tc, DK, DV>());
   Tc* const vt = kt + C * SK;
   Tc* const pt = vt + C * SV;
   float* const pw = (float*)(pt + C * SP);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int lane = tid & 63, half = lane >> 5, col = lane & 31;
+  void* const strip = smem + 4096 * wave;
   const int unit = blockIdx.x / segments, seg = blockIdx.x % segments, b = unit / A.heads, h = unit % A.heads;
   const int len = length_of(A, b), t0 = seg * seg_tokens, t1 = min(len, t0 + seg_tokens);
   const int c = 32 * wave + col, shift = REV ? 0 : 1;
@@ -168,22 +215,28 @@ __global__ void __launch_bounds__(2 * DV, 1) decay_outputs(const Args A, int seg
   const Tin* const v = rows_of<Tin>(A.v, A.v_stride, b, h / (A.heads / A.v_heads));
   const long long qs = A.q_stride[2], ks = A.k_stride[2], vs = A.v_stride[2];
   const auto at = [&](int t) -> long long { return REV ? len - 1 - t : t; };  // row of the t-th token of the walk
-  const long long out0 = (long long)b * A.out_stride[0] + (long long)h * A.out_stride[1];
-  auto put = [&](int t, int d, float x) {  // component d of token t (in the order of the walk)
-    const long long place = out0 + (t < len ? at(t) : t) * A.out_stride[2] + d;
-    if (A.out_float32) ((float*)A.out)[place] = x; else ((Tin*)A.out)[place] = (Tin)x;
-  };
+  const long long os = A.out_stride[2], out0 = (long long)b * A.out_stride[0] + (long long)h * A.out_stride[1];
 
   f32x16 S[DK / 32];
   {
-    const float* from = segments > 1 ? states + (long long)blockIdx.x * A.dim * A.dim_v : (A.state_in ? A.state_in + (long long)unit * A.dim * A.dim_v : nullptr);
-    const long long s0 = segments > 1 ? A.dim_v : A.state_in_stride[0], s1 = segments > 1 ? 1 : A.state_in_stride[1];
+    const float* from = CUT ? states + (long long)blockIdx.x * A.dim * A.dim_v : (A.state_in ? A.state_in + (long long)unit * A.dim * A.dim_v : nullptr);
+    const int s0 = (int)(CUT ? A.states_stride[0] : A.state_in_stride[0]), s1 = (int)(CUT ? A.states_stride[1] : A.state_in_stride[1]);
 #pragma unroll
     for (int i = 0; i < DK / 32; i++)
 #pragma unroll
-      for (int r = 0; r < 16; r++) {
-        const int d = 32 * i + c_row(r, half);
-        S[i][r] = from && d < A.dim && c < A.dim_v ? from[d * s0 + c * s1] : 0.f;
+      for (int g = 0; g < 4; g++) {
+        const int d = 32 * i + 8 * g + 4 * half;  // (dim is a multiple of 4)
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        if (from && d < A.dim && c < A.dim_v) {
+          if (s0 == 1) {
+            x = *reinterpret_cast<const f32x4*>(from + c * s1 + d);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = from[(d + j) * s0 + c * s1];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) S[i][4 * g + j] = x[j];
       }
   }
   Staged<Tin, Tc, C, DK, NT, REV> sq, sk;
@@ -194,6 +247,10 @@ __global__ void __launch_bounds__(2 * DV, 1) decay_outputs(const Args A, int seg
     sv.load(v + at(t0) * vs, vs, t1 - t0, A.dim_v, tid);
   }
   for (int t = t0; t < t1; t += C) {
+    // places in LDS are the same in every chunk: formed anew, they do not stay in registers all along
+    asm volatile("" : "+v"(lane));
+    half = lane >> 5;
+    col = lane & 31;
     __syncthreads();
     sq.store(qt, tid);
     sk.store(kt, tid);
@@ -219,48 +276,37 @@ __global__ void __launch_bounds__(2 * DV, 1) decay_outputs(const Args A, int seg
         store4<Tc>(pt + tile_at<Tc, C>(i0 + col, j0 + 8 * g + 4 * half), x[0], x[1], x[2], x[3]);
       }
     }
-    __syncthreads();
     // outputs: the state's part first, decayed to each row in float32, then the chunk's own
     f32x16 o[2] = {zero16(), zero16()};
 #pragma unroll
     for (int i = 0; i < DK / 32; i++)
 #pragma unroll
       for (int s = 0; s < 2; s++) {
-        float x[8];
+        const typename Vec<Tc>::x8 st = pack<Tc>(S[i], s);
 #pragma unroll
-        for (int j = 0; j < 8; j++) x[j] = S[i][8 * s + j];
-        Terms<Tc, state_terms<Tc>()> st;
-        st.set(x);
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-          const typename Vec<Tc>::x8 qf = frag_rows_split<Tc, DK>(qt, 32 * u + col, 32 * i + 16 * s, half);
-#pragma unroll
-          for (int m = 0; m < state_terms<Tc>(); m++) o[u] = mma(qf, st.t[m], o[u]);
-        }
+        for (int u = 0; u < 2; u++) o[u] = mma(frag_rows_split<Tc, DK>(qt, 32 * u + col, 32 * i + 16 * s, half), st, o[u]);
       }
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
+    for (int u = 0; u < 2; u++)
 #pragma unroll
       for (int r = 0; r < 16; r++) o[u][r] *= pw[kZero + 32 * u + c_row(r, half) + shift] * A.query_scale;
+    __syncthreads();
 #pragma unroll
-      for (int s = 0; s < 2 * (u + 1); s++) o[u] = mma(frag_rows_split<Tc, C>(pt, 32 * u + col, 16 * s, half), frag_cols<Tc, DV>(vt, 16 * s, 32 * wave, lane), o[u]);
+    for (int s = 0; s < 4; s++) {
+      const typename Vec<Tc>::x8 vf = frag_cols<Tc, DV>(vt, 16 * s, 32 * wave, lane);
+#pragma unroll
+      for (int u = s / 2; u < 2; u++) o[u] = mma(frag_rows_split<Tc, C>(pt, 32 * u + col, 16 * s, half), vf, o[u]);
     }
-    if (c < A.dim_v) {
-#pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int r = 0; r < 16; r++) {
-          const int row = t + 32 * u + c_row(r, half);
-          if (row < t1) put(row, c, o[u][r]);
-        }
-    }
-    if (segments == 1 ? (A.state_out || t + C < t1) : t + C < t1)
-      update_state<Tc, DK, DV>(S, kt, vt, pw, min(C, t1 - t), REV ? 1 : 0, A.update_scale, wave, lane);
+    if (A.out_float32) store_rows<float, REV>((float*)A.out + out0, os, o, strip, t, t1, len, wave, lane, A.dim_v);
+    else store_rows<Tin, REV>((Tin*)A.out + out0, os, o, strip, t, t1, len, wave, lane, A.dim_v);
+    if ((!CUT && A.state_out) || t + C < t1) update_state<Tc, DK, DV, update_terms<Tc, !CUT>()>(S, kt, vt, pw, min(C, t1 - t), REV ? 1 : 0, A.update_scale, wave, lane);
   }
   // tokens behind the sequence
   for (int t = max(t0, len); t < min((int)A.tokens, t0 + seg_tokens); t++)
-    for (int d = tid; d < A.dim_v; d += NT) put(t, d, 0.f);
-  if (segments == 1 && A.state_out) {
+    for (int d = tid; d < A.dim_v; d += NT) {
+      if (A.out_float32) ((float*)A.out)[out0 + t * os + d] = 0.f; else ((Tin*)A.out)[out0 + t * os + d] = (Tin)0.f;
+    }
+  if (!CUT && A.state_out) {
     float* to = A.state_out + (long long)unit * A.dim * A.dim_v;
 #pragma unroll
     for (int i = 0; i < DK / 32; i++)
@@ -348,7 +394,7 @@ const char* check(const Args* a) {
   if (a->dim < ve || a->dim > 128 || a->dim % ve || a->dim_v < ve || a->dim_v > 128 || a->dim_v % ve)
     return "decay attention: dim and dim_v must be multiples of 16 bytes, at most 128";
   if (a->tokens < 0 || a->tokens > (1 << 29)) return "decay attention: tokens out of range";
-  for (const int64_t* x : {a->q_stride, a->k_stride, a->v_stride})
+  for (const int64_t* x : {a->q_stride, a->k_stride, a->v_stride, a->out_stride})
     if (x[2] < 0 || x[2] > kMaxRowStride) return "decay attention: rows too far apart";
   if (!a->log_decay || (a->tokens > 0 && (!a->q || !a->k || !a->v || !a->out))) return "decay attention: null data";
   if ((int64_t)a->batch * a->heads > 65535) return "decay attention: more than 65535 sequences times heads";
@@ -358,7 +404,8 @@ const char* check(const Args* a) {
 // Segments of a sequence: enough workgroups to fill the chip, whole chunks each.
 void segments_of(const Args* a, int& segments, int& seg_tokens) {
   const int64_t units = (int64_t)a->batch * a->heads, chunks = (a->tokens + C - 1) / C;
-  int64_t want = (512 + units - 1) / units;
+  const int64_t fill = a->dim_v > 64 ? 512 : 1024;  // workgroups of four or two wavefronts
+  int64_t want = (fill + units - 1) / units;
   if (want > chunks) want = chunks;
   if (want < 1) want = 1;
   const int64_t per = chunks < 1 ? 1 : (chunks + want - 1) / want;
@@ -372,29 +419,31 @@ template <class K> int prepare_lds(K kernel, size_t bytes) {
   return e == hipSuccess ? 0 : keops_seq_fail((int)e, "decay attention: shared memory");
 }
 
-template <class Tin, class Tc, int DK, int DV, bool REV> int run(const Args& a, float* work, hipStream_t st) {
+template <class Tin, class Tc, int DK, int DV, bool REV> int run(const Args& a, hipStream_t st) {
+  float* const work = a.states;
   int segments, seg_tokens;
   segments_of(&a, segments, seg_tokens);
   const int units = a.batch * a.heads;
   const size_t kv = (size_t)C * (tile_stride<Tc, DK>() + tile_stride<Tc, DV>()) * sizeof(Tc), pw = kPowers * sizeof(float);
-  const size_t all = kv + (size_t)C * (tile_stride<Tc, DK>() + tile_stride<Tc, C>()) * sizeof(Tc) + pw;
-  if (segments > 1) {
+  const size_t all = query_bytes<Tc, DK, DV>() + kv + (size_t)C * tile_stride<Tc, C>() * sizeof(Tc) + pw;
+  if (segments > 1 && !a.states_given) {
     if (int e = prepare_lds(decay_states<Tin, Tc, DK, DV, REV>, kv + pw)) return e;
     decay_states<Tin, Tc, DK, DV, REV><<<units * segments, 2 * DV, kv + pw, st>>>(a, segments, seg_tokens, work);
     decay_scan<<<dim3((a.dim * a.dim_v + 255) / 256, units), 256, 0, st>>>(a, segments, seg_tokens, work);
   }
-  if (int e = prepare_lds(decay_outputs<Tin, Tc, DK, DV, REV>, all)) return e;
-  decay_outputs<Tin, Tc, DK, DV, REV><<<units * segments, 2 * DV, all, st>>>(a, segments, seg_tokens, work);
+  const auto outputs = segments > 1 ? decay_outputs<Tin, Tc, DK, DV, REV, true> : decay_outputs<Tin, Tc, DK, DV, REV, false>;
+  if (int e = prepare_lds(outputs, all)) return e;
+  outputs<<<units * segments, 2 * DV, all, st>>>(a, segments, seg_tokens, work);
   return seq_launched("decay attention: launch");
 }
 
-template <class Tin, class Tc, bool REV> int by_dims(const Args& a, float* work, hipStream_t st) {
-  if (a.dim <= 64) return a.dim_v <= 64 ? run<Tin, Tc, 64, 64, REV>(a, work, st) : run<Tin, Tc, 64, 128, REV>(a, work, st);
-  return a.dim_v <= 64 ? run<Tin, Tc, 128, 64, REV>(a, work, st) : run<Tin, Tc, 128, 128, REV>(a, work, st);
+template <class Tin, class Tc, bool REV> int by_dims(const Args& a, hipStream_t st) {
+  if (a.dim <= 64) return a.dim_v <= 64 ? run<Tin, Tc, 64, 64, REV>(a, st) : run<Tin, Tc, 64, 128, REV>(a, st);
+  return a.dim_v <= 64 ? run<Tin, Tc, 128, 64, REV>(a, st) : run<Tin, Tc, 128, 128, REV>(a, st);
 }
 
-template <class Tin, class Tc> int dispatch(const Args& a, float* work, hipStream_t st) {
-  return a.reverse ? by_dims<Tin, Tc, true>(a, work, st) : by_dims<Tin, Tc, false>(a, work, st);
+template <class Tin, class Tc> int dispatch(const Args& a, hipStream_t st) {
+  return a.reverse ? by_dims<Tin, Tc, true>(a, st) : by_dims<Tin, Tc, false>(a, st);
 }
 
 template <class T>
@@ -419,15 +468,16 @@ size_t keops_hip_decay_attention_bytes(const keops_hip_decay_attention* a) {
   return segments > 1 ? (size_t)a->batch * a->heads * segments * a->dim * a->dim_v * sizeof(float) : 0;
 }
 
-int keops_hip_decay_attention_run(const keops_hip_decay_attention* a, void* work, size_t work_bytes, int device, void* hip_stream) {
+int keops_hip_decay_attention_run(const keops_hip_decay_attention* a, int device, void* hip_stream) {
   if (const char* why = check(a)) return keops_seq_fail(-1, why);
   const size_t need = keops_hip_decay_attention_bytes(a);
-  if (need > work_bytes || (need > 0 && !work)) return keops_seq_fail(-1, "decay attention: workspace too small");
+  if (need > (size_t)(a->states_bytes > 0 ? a->states_bytes : 0) || (need > 0 && !a->states)) return keops_seq_fail(-1, "decay attention: workspace too small");
+  if (a->states_given && need > 0 && a->state_out) return keops_seq_fail(-1, "decay attention: no final state where the states are given");
   SeqDevice on(device);
   hipStream_t st = (hipStream_t)hip_stream;
-  if (a->dtype == 0) return dispatch<bf16, bf16>(*a, (float*)work, st);
-  if (a->dtype == 1) return dispatch<f16, float>(*a, (float*)work, st);
-  return dispatch<float, float>(*a, (float*)work, st);
+  if (a->dtype == 0) return dispatch<bf16, bf16>(*a, st);
+  if (a->dtype == 1) return dispatch<f16, float>(*a, st);
+  return dispatch<float, float>(*a, st);
 }
 
 int keops_hip_decay_attention_step(int dtype, int batch, int heads, int kv_heads, int dim, int dim_v, float scale, const void* q, const int64_t* q_stride,

@@ -296,15 +296,16 @@ def bucket_attention(q, k, v, bias, buckets, *, causal=False, key_lengths=None, 
 
 # --------------------------------------------------------------------------------------------------- decay attention
 def _decay_run(q, k, v, log_decay, lengths, heads, *, reverse=False, product_scale=1.0, query_scale=1.0, update_scale=1.0, state=None,
-               transposed=False, out=None, float32=False, want_state=False):
-    """One walk over the tokens (keops_hip_decay_attention of include/keops_hip.h); ``transposed``: ``state`` holds the transpose
-    of the matrices that the walk starts from.  Returns the outputs and the final state (or None)."""
+               transposed=False, out=None, float32=False, want_state=False, states=None):
+    """One walk over the tokens (keops_hip_decay_attention of include/keops_hip.h).  ``transposed``: ``state`` and ``states`` hold
+    the transposes of the matrices that the walk starts from; ``states``: the workspace of the walk that left them.  Returns the
+    outputs, the final state (or None) and the workspace."""
     b, t, d, dv = q.shape[0], q.shape[2], q.shape[3], v.shape[3]
     if out is None:
         out = torch.empty(b, heads, t, dv, dtype=torch.float32 if float32 else q.dtype, device=q.device)
     last = torch.empty(b, heads, d, dv, dtype=torch.float32, device=q.device) if want_state else None
     if b == 0 or heads == 0:
-        return out, last
+        return out, last, None
     a = binder.DecayAttention()
     a.dtype, a.batch, a.heads, a.dim, a.dim_v, a.tokens = _DTYPES[q.dtype], b, heads, d, dv, t
     a.q_heads, a.k_heads, a.v_heads = q.shape[1], k.shape[1], v.shape[1]
@@ -315,8 +316,15 @@ def _decay_run(q, k, v, log_decay, lengths, heads, *, reverse=False, product_sca
     a.log_decay, a.lengths, a.state_in, a.state_out = _ptr(log_decay), _ptr(lengths), _ptr(state), _ptr(last)
     a.state_in_stride[:] = (1, d) if transposed else (dv, 1)
     a.state_out_stride[:] = (dv, 1)
-    _call("keops_hip_decay_attention_run", a, "keops_hip_decay_attention_bytes", q.device)
-    return out, last
+    lib = binder.lib()
+    a.states_given = int(states is not None)
+    a.states_stride[:] = (1, d) if transposed and states is not None else (dv, 1)
+    if states is None:
+        states = torch.empty(lib.keops_hip_decay_attention_bytes(ctypes.byref(a)) // 4, dtype=torch.float32, device=q.device)
+    a.states, a.states_bytes = _ptr(states), 4 * states.numel()
+    stream = torch.cuda.current_stream(q.device).cuda_stream
+    binder.check(lib.keops_hip_decay_attention_run(ctypes.byref(a), q.device.index, stream), "keops_hip_decay_attention_run")
+    return out, last, states
 
 
 def _decay_out(q, v):
@@ -330,44 +338,46 @@ def _decay_out(q, v):
 
 def _decay_forward(q, k, v, log_decay, state, lengths, scale):
     q, k, v = _rows(q), _rows(k), _rows(v)
-    out, last = _decay_run(q, k, v, log_decay, lengths, q.shape[1], product_scale=scale, query_scale=scale, state=state,
-                           out=_decay_out(q, v), want_state=True)
-    return q, k, v, out, last
+    out, last, states = _decay_run(q, k, v, log_decay, lengths, q.shape[1], product_scale=scale, query_scale=scale, state=state,
+                                   out=_decay_out(q, v), want_state=True)
+    return q, k, v, out, last, states
 
 
 class _DecayAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, state, log_decay, lengths, scale):
         ctx.set_materialize_grads(False)
-        q, k, v, out, last = _decay_forward(q, k, v, log_decay, state, lengths, scale)
+        q, k, v, out, last, states = _decay_forward(q, k, v, log_decay, state, lengths, scale)
         ctx.scale = scale
-        ctx.save_for_backward(q, k, v, state, log_decay, lengths)
+        ctx.save_for_backward(q, k, v, state, log_decay, lengths, states)
         return out, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, grad_last):
-        # gradients are walks of the same kind (csrc/sequence/keops_seq_decay.hip)
-        q, k, v, state, log_decay, lengths = ctx.saved_tensors
+        # gradients are walks of the same kind (csrc/sequence/keops_seq_decay.hip); that of q starts from the forward pass's states,
+        # that of k from those of v's
+        q, k, v, state, log_decay, lengths, states = ctx.saved_tensors
         (b, h, t, d), dv, scale, shared = q.shape, v.shape[3], ctx.scale, k.shape[1]
         grad = torch.zeros(b, h, t, dv, dtype=q.dtype, device=q.device) if grad is None else _rows(grad)
         grad_last = None if grad_last is None else grad_last.contiguous()
 
-        def walk(*data, want_state=False, like=None, **options):
+        def walk(*data, like, **options):
             # a shared head's gradient is the sum over the heads that share it, rounded once
-            out = None if like is not None and like.shape[1] != h else _like(like)
-            out, last = _decay_run(*data, log_decay, lengths, h, product_scale=scale, out=out, float32=True, want_state=want_state, **options)
-            if like is not None and like.shape[1] != h:
+            out = None if like.shape[1] != h else _like(like)
+            out, last, left = _decay_run(*data, log_decay, lengths, h, product_scale=scale, out=out, float32=True, **options)
+            if like.shape[1] != h:
                 out = out.view(b, shared, h // shared, t, -1).sum(2).to(like.dtype)
-            return out, last
+            return out, last, left
 
-        dq = dk = dv_ = ds = None
-        if ctx.needs_input_grad[0]:
-            dq, _ = walk(grad, v, k, like=q, query_scale=scale, state=state, transposed=True)
-        if ctx.needs_input_grad[1]:
-            dk, _ = walk(v, grad, q, like=k, reverse=True, update_scale=scale, state=grad_last, transposed=True)
-        if ctx.needs_input_grad[2] or ctx.needs_input_grad[3]:
-            dv_, ds = walk(k, q, grad, like=v, reverse=True, update_scale=scale, state=grad_last, want_state=ctx.needs_input_grad[3])
+        want_q, want_k, want_v, want_state = ctx.needs_input_grad[:4]
+        dq = dk = dv_ = ds = back = None
+        if want_q:
+            dq = walk(grad, v, k, like=q, query_scale=scale, state=state, transposed=True, states=states)[0]
+        if want_v or want_state:
+            dv_, ds, back = walk(k, q, grad, like=v, reverse=True, update_scale=scale, state=grad_last, want_state=want_state)
+        if want_k:
+            dk = walk(v, grad, q, like=k, reverse=True, update_scale=scale, state=grad_last, transposed=True, states=back)[0]
         return dq, dk, dv_, ds, None, None, None
 
 
@@ -431,7 +441,7 @@ def decay_attention(q, k, v, log_decay, *, initial_state=None, lengths=None, sca
     if _needs_grad(q, k, v, state):
         out, last = _DecayAttention.apply(q, k, v, state, log_decay, lengths, scale)
     else:
-        out, last = _decay_forward(q, k, v, log_decay, state, lengths, scale)[3:]
+        out, last = _decay_forward(q, k, v, log_decay, state, lengths, scale)[3:5]
     if out.shape[3] != dv:
         out = out[..., :dv].contiguous()
     if last.shape[2:] != (d, dv):

@@ -107,9 +107,25 @@ def test_decay_arguments_that_the_library_refuses(changes, message):
     for name, value in changes.items():
         setattr(a, name, value)
     lib = binder.lib()
-    assert lib.keops_hip_decay_attention_run(ctypes.byref(a), None, 0, 0, None) != 0
+    assert lib.keops_hip_decay_attention_run(ctypes.byref(a), 0, None) != 0
     assert message in binder.last_error() and "decay attention" in binder.last_error()
     assert lib.keops_hip_decay_attention_bytes(ctypes.byref(a)) == 0
+
+
+def test_decay_workspaces():
+    lib = binder.lib()
+    a = binder.DecayAttention()
+    a.dtype, a.batch, a.heads, a.q_heads, a.k_heads, a.v_heads, a.dim, a.dim_v, a.tokens = 0, 1, 2, 2, 2, 2, 64, 64, 64
+    for name in ("q", "k", "v", "out", "log_decay"):
+        setattr(a, name, 1 << 12)
+    assert lib.keops_hip_decay_attention_bytes(ctypes.byref(a)) == 0  # one chunk: nothing to carry
+    a.tokens = 6400
+    need = lib.keops_hip_decay_attention_bytes(ctypes.byref(a))
+    assert need > 0 and need % (2 * 64 * 64 * 4) == 0
+    a.states, a.states_bytes = 1 << 12, need - 1
+    assert lib.keops_hip_decay_attention_run(ctypes.byref(a), 0, None) != 0 and "workspace" in binder.last_error()
+    a.states_bytes, a.states_given, a.state_out = need, 1, 1 << 12
+    assert lib.keops_hip_decay_attention_run(ctypes.byref(a), 0, None) != 0 and "final state" in binder.last_error()
 
 
 def test_step_and_logprob_arguments_that_the_library_refuses():
