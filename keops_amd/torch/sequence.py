@@ -20,10 +20,13 @@ from torch.autograd.function import once_differentiable
 from .. import binder
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_MAX_ROW_STRIDE = 1 << 23  # kMaxRowStride of csrc/sequence/keops_seq.h
+_MAX_PLANS = 512
+_raw_stream = torch._C._cuda_getCurrentRawStream  # hipStream_t of a device's current stream
 
 
 def _check_data(what, **tensors):
-    """All on one HIP device, all of one supported type; returns them in order."""
+    """All on one HIP device, all of one supported type."""
     device = dtype = None
     for name, t in tensors.items():
         if not isinstance(t, torch.Tensor):
@@ -46,30 +49,33 @@ def _check_whole(what, name, t, shape, device):
         raise TypeError(f"[KeOps] {what}: {name} must be an int32 or int64 tensor.")
     if t.device != device:
         raise ValueError("[KeOps] Input arrays must be all located on the same device.")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"[KeOps] {what}: {name} must be of shape {shape}, got {tuple(t.shape)}.")
+    if t.shape != shape:
+        raise ValueError(f"[KeOps] {what}: {name} must be of shape {tuple(shape)}, got {tuple(t.shape)}.")
+    if t.dtype is torch.int32 and t.is_contiguous():
+        return t
     return t.to(torch.int32).contiguous()
 
 
-_MAX_ROW_STRIDE = 1 << 23  # kMaxRowStride of csrc/sequence/keops_seq.h
+def _strides_fit(x):
+    """Rows as the kernels read them: neighbouring components, every row a multiple of 16 bytes from the first and not too far
+    from the next."""
+    size = x.element_size()
+    shape, stride = x.shape, x.stride()
+    return x.numel() == 0 or (
+        (stride[-1] == 1 or shape[-1] == 1) and (shape[-2] == 1 or stride[-2] <= _MAX_ROW_STRIDE)
+        and all(s * size % 16 == 0 for s, n in zip(stride[:-1], shape[:-1]) if n > 1)
+    )
 
 
 def _rows(x):
-    """x with rows as the kernels read them: neighbouring components, every row at a multiple of 16 bytes and not too far from the
-    next (a copy if not)."""
-    size = x.element_size()
-    if x.numel() == 0 or (
-        x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and (x.shape[-2] == 1 or x.stride(-2) <= _MAX_ROW_STRIDE)
-        and all(s * size % 16 == 0 for s, n in zip(x.stride()[:-1], x.shape[:-1]) if n > 1)
-    ):
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
+    """x with rows as the kernels read them, a copy if they are not."""
+    return x if _strides_fit(x) and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
 
 
-def _like(x):
-    """Uninitialised tensor of x's shape, in x's order of dimensions where x is dense, with rows as the kernels write them."""
-    y = torch.empty_like(x)
-    return y if _rows(y) is y else torch.empty_like(x, memory_format=torch.contiguous_format)
+def _dense_strides(x):
+    """Strides of a new tensor of x's shape: x's own where x is dense and they fit, else those of the contiguous order."""
+    y = torch.empty_like(x, device="meta")
+    return y.stride() if _strides_fit(y) else torch.empty(x.shape, device="meta").stride()
 
 
 def _pad(x, *multiples):
@@ -84,22 +90,21 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _stride(t):
-    b, h, r = t.stride()[:3]
-    return b, h, r if t.shape[2] > 1 else 0
+def _stride(shape, stride):
+    """Strides of batch, head and row as the library takes them (a single row has none)."""
+    return stride[0], stride[1], stride[2] if shape[2] > 1 else 0
 
 
-def _needs_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+def _geometry(t):
+    """What a plan depends on of a tensor: everything but where it is."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
-def _call(name, args, size, device):
-    """Run an entry point of the library on the device's current stream, with the workspace that it asks for."""
-    lib = binder.lib()
-    nbytes = getattr(lib, size)(ctypes.byref(args))
-    work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-    stream = torch.cuda.current_stream(device).cuda_stream
-    binder.check(getattr(lib, name)(ctypes.byref(args), _ptr(work), nbytes, device.index, stream), name)
+def _keep(plans, key, plan):
+    if len(plans) >= _MAX_PLANS:
+        plans.clear()
+    plans[key] = plan
+    return plan
 
 
 # --------------------------------------------------------------------------------------------------- position buckets
@@ -158,6 +163,7 @@ class PositionBuckets:
         begin = [sum(b < k for b in bucket_of) for k in range(num_buckets + 1)]
         self._host = tuple(torch.tensor(x, dtype=torch.int32) for x in (bucket_of, order, begin))
         self._device = {}
+        self._plans = {}  # of bucket_attention with these buckets, by the geometry of the tensors
 
     def __call__(self, relative_position):
         """Bucket of each entry of an integer tensor of relative positions ``key - query``."""
@@ -173,65 +179,109 @@ class PositionBuckets:
 
 
 # --------------------------------------------------------------------------------------------------- bucket attention
-def _bucket_args(q, k, v, bias, buckets, causal, key_lengths, query_start, scale):
-    a = binder.BucketAttention()
-    a.dtype, a.batch, a.heads, a.kv_heads, a.dim = _DTYPES[q.dtype], q.shape[0], q.shape[1], k.shape[1], q.shape[3]
-    a.queries, a.keys, a.causal, a.scale = q.shape[2], k.shape[2], int(causal), scale
-    a.buckets, a.reach = buckets.num_buckets, buckets.reach
-    a.q, a.k, a.v, a.bias = _ptr(q), _ptr(k), _ptr(v), _ptr(bias)
-    a.q_stride[:], a.k_stride[:], a.v_stride[:] = _stride(q), _stride(k), _stride(v)
-    a.bucket_of, a.bucket_order, a.bucket_begin = (t.data_ptr() for t in buckets.on(q.device))
-    a.key_lengths = _ptr(key_lengths)
-    if isinstance(query_start, torch.Tensor):
-        a.query_start = _ptr(query_start)
-    else:
-        a.start = query_start
-    return a
+class _BucketPlan:
+    """Arguments of a call that depend on the geometry of its tensors alone, checked once."""
 
+    def __init__(self, q, k, v, bias, buckets, causal, start, scale):
+        self.tables = buckets.on(q.device)
+        self.out_strides, self.k_strides, self.v_strides = _dense_strides(q), _dense_strides(k), _dense_strides(v)
+        self.index = q.device.index
+        a = binder.BucketAttention()
+        a.dtype, a.batch, a.heads, a.kv_heads, a.dim = _DTYPES[q.dtype], q.shape[0], q.shape[1], k.shape[1], q.shape[3]
+        a.queries, a.keys, a.causal, a.scale = q.shape[2], k.shape[2], int(causal), scale
+        a.buckets, a.reach, a.start = buckets.num_buckets, buckets.reach, start
+        a.q_stride[:], a.k_stride[:], a.v_stride[:] = (_stride(x.shape, x.stride()) for x in (q, k, v))
+        a.out_stride[:] = a.grad_q_stride[:] = _stride(q.shape, self.out_strides)
+        a.grad_k_stride[:], a.grad_v_stride[:] = _stride(k.shape, self.k_strides), _stride(v.shape, self.v_strides)
+        a.bucket_of, a.bucket_order, a.bucket_begin = (t.data_ptr() for t in self.tables)
+        self.empty = q.numel() == 0
+        self.args = bytes(a)
+        if not self.empty:  # the library's own checks, on placeholders that it does not follow
+            lib = binder.lib()
+            a.q = a.k = a.v = a.out = a.bias = a.grad_bias = 16
+            self.forward_bytes = lib.keops_hip_bucket_attention_forward_bytes(ctypes.byref(a))
+            self.backward_bytes = lib.keops_hip_bucket_attention_backward_bytes(ctypes.byref(a))
 
-def _bucket_forward(q, k, v, bias, options, want_lse):
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    out = _like(q)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
-    if out.numel():
-        a = _bucket_args(q, k, v, bias, *options)
-        a.out, a.out_stride[:], a.lse = _ptr(out), _stride(out), _ptr(lse)
-        _call("keops_hip_bucket_attention_forward", a, "keops_hip_bucket_attention_forward_bytes", q.device)
-    return q, k, v, out, lse
+    def fill(self, q, k, v, bias, key_lengths, query_start):
+        a = binder.BucketAttention.from_buffer_copy(self.args)
+        a.q, a.k, a.v, a.bias = q.data_ptr(), k.data_ptr(), v.data_ptr(), bias.data_ptr()
+        if key_lengths is not None:
+            a.key_lengths = key_lengths.data_ptr()
+        if query_start is not None:
+            a.query_start = query_start.data_ptr()
+        return a
+
+    def run(self, name, a, nbytes, device):
+        work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        rc = getattr(binder.lib(), name)(ctypes.byref(a), _ptr(work), nbytes, self.index, _raw_stream(self.index))
+        if rc:
+            binder.check(rc, name)
+
+    def forward(self, q, k, v, bias, key_lengths, query_start, want_lse):
+        out = torch.empty_strided(q.shape, self.out_strides, dtype=q.dtype, device=q.device)
+        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
+        if not self.empty:
+            a = self.fill(q, k, v, bias, key_lengths, query_start)
+            a.out = out.data_ptr()
+            if want_lse:
+                a.lse = lse.data_ptr()
+            self.run("keops_hip_bucket_attention_forward", a, self.forward_bytes, q.device)
+        return out, lse
 
 
 class _BucketAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, bias, options):
-        q, k, v, out, lse = _bucket_forward(q, k, v, bias, options, True)
-        tensors = [t for t in options if isinstance(t, torch.Tensor)]
-        ctx.places = [i for i, t in enumerate(options) if isinstance(t, torch.Tensor)]
-        ctx.options = [None if isinstance(t, torch.Tensor) else t for t in options]
-        ctx.save_for_backward(q, k, v, bias, out, lse, *tensors)
+    def forward(ctx, q, k, v, bias, plan, key_lengths, query_start):
+        out, lse = plan.forward(q, k, v, bias, key_lengths, query_start, True)
+        ctx.plan = plan
+        ctx.save_for_backward(q, k, v, bias, out, lse, key_lengths, query_start)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, k, v, bias, out, lse, *tensors = ctx.saved_tensors
-        options = list(ctx.options)
-        for i, t in zip(ctx.places, tensors):
-            options[i] = t
-        if out.numel() == 0:
-            return (*(torch.zeros_like(t) for t in (q, k, v, bias)), None)
+        q, k, v, bias, out, lse, key_lengths, query_start = ctx.saved_tensors
+        plan = ctx.plan
+        if plan.empty:
+            return (*(torch.zeros_like(t) for t in (q, k, v, bias)), None, None, None)
         grad = _rows(grad)
-        dq, dk, dv = (_like(q) if ctx.needs_input_grad[0] else None), _like(k), _like(v)
+        new = lambda t, strides: torch.empty_strided(t.shape, strides, dtype=t.dtype, device=t.device)
+        dq = new(q, plan.out_strides) if ctx.needs_input_grad[0] else None
+        dk, dv = new(k, plan.k_strides), new(v, plan.v_strides)
         db = torch.empty_like(bias) if ctx.needs_input_grad[3] else None
         delta = torch.empty_like(lse)
-        a = _bucket_args(q, k, v, bias, *options)
-        a.out, a.out_stride[:], a.lse, a.delta = _ptr(out), _stride(out), _ptr(lse), _ptr(delta)
-        a.grad_out, a.grad_out_stride[:] = _ptr(grad), _stride(grad)
-        if dq is not None:
-            a.grad_q, a.grad_q_stride[:] = _ptr(dq), _stride(dq)
-        a.grad_k, a.grad_k_stride[:], a.grad_v, a.grad_v_stride[:] = _ptr(dk), _stride(dk), _ptr(dv), _stride(dv)
-        a.grad_bias = _ptr(db)
-        _call("keops_hip_bucket_attention_backward", a, "keops_hip_bucket_attention_backward_bytes", q.device)
-        return dq, dk, dv, db, None
+        a = plan.fill(q, k, v, bias, key_lengths, query_start)
+        a.out, a.lse, a.delta = out.data_ptr(), lse.data_ptr(), delta.data_ptr()
+        a.grad_out, a.grad_out_stride[:] = grad.data_ptr(), _stride(grad.shape, grad.stride())
+        a.grad_q, a.grad_k, a.grad_v, a.grad_bias = _ptr(dq), dk.data_ptr(), dv.data_ptr(), _ptr(db)
+        plan.run("keops_hip_bucket_attention_backward", a, 0 if db is None else plan.backward_bytes, q.device)
+        return dq, dk, dv, db, None, None, None
+
+
+def _check_bucket(q, k, v, bias, buckets, query_start):
+    what = "bucket_attention"
+    device, dtype = _check_data(what, q=q, k=k, v=v)
+    if not isinstance(buckets, PositionBuckets):
+        raise TypeError("[KeOps] bucket_attention: buckets must be a PositionBuckets.")
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError("[KeOps] bucket_attention: q must be (batch, heads, queries, dim), k and v (batch, kv_heads, keys, dim).")
+    b, h, m, d = q.shape
+    if k.shape[0] != b or k.shape[3] != d or k.shape[1] < 1 or h % k.shape[1]:
+        raise ValueError(f"[KeOps] bucket_attention: q {tuple(q.shape)} and k {tuple(k.shape)} do not fit: same batch and dim, heads a "
+                         "multiple of kv_heads.")
+    if not 1 <= d <= 128:
+        raise ValueError(f"[KeOps] bucket_attention: dim must be from 1 to 128, it is {d}.")
+    if max(m, k.shape[2]) > 1 << 29:
+        raise ValueError("[KeOps] bucket_attention: at most 2**29 queries and keys.")
+    _check_data(what, bias=bias)
+    if bias.device != device:
+        raise ValueError("[KeOps] Input arrays must be all located on the same device.")
+    if bias.dtype not in (torch.float32, dtype) or tuple(bias.shape) != (h, buckets.num_buckets):
+        raise ValueError(f"[KeOps] bucket_attention: bias must be ({h}, {buckets.num_buckets}), float32 or {dtype}; got "
+                         f"{tuple(bias.shape)}, {bias.dtype}.")
+    if not isinstance(query_start, torch.Tensor) and (
+            isinstance(query_start, bool) or not isinstance(query_start, int) or abs(query_start) > 1 << 29):
+        raise ValueError("[KeOps] bucket_attention: query_start must be a whole number of absolute value at most 2**29, or a tensor.")
 
 
 def bucket_attention(q, k, v, bias, buckets, *, causal=False, key_lengths=None, query_start=0, scale=None):
@@ -257,98 +307,143 @@ def bucket_attention(q, k, v, bias, buckets, *, causal=False, key_lengths=None, 
     Returns (batch, heads, queries, dim) in the type and order of dimensions of q.  Differentiable with respect to q, k, v and
     bias.  Up to 32 queries x shared heads use a form of their own that splits the keys over the chip (token generation).
     """
-    what = "bucket_attention"
-    device, dtype = _check_data(what, q=q, k=k, v=v)
-    if not isinstance(buckets, PositionBuckets):
-        raise TypeError("[KeOps] bucket_attention: buckets must be a PositionBuckets.")
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
-        raise ValueError("[KeOps] bucket_attention: q must be (batch, heads, queries, dim), k and v (batch, kv_heads, keys, dim).")
-    b, h, m, d = q.shape
-    if k.shape[0] != b or k.shape[3] != d or k.shape[1] < 1 or h % k.shape[1]:
-        raise ValueError(f"[KeOps] bucket_attention: q {tuple(q.shape)} and k {tuple(k.shape)} do not fit: same batch and dim, heads a "
-                         "multiple of kv_heads.")
-    if not 1 <= d <= 128:
-        raise ValueError(f"[KeOps] bucket_attention: dim must be from 1 to 128, it is {d}.")
-    if max(m, k.shape[2]) > 1 << 29:
-        raise ValueError("[KeOps] bucket_attention: at most 2**29 queries and keys.")
-    _check_data(what, bias=bias)
-    if bias.device != device:
-        raise ValueError("[KeOps] Input arrays must be all located on the same device.")
-    if bias.dtype not in (torch.float32, dtype) or tuple(bias.shape) != (h, buckets.num_buckets):
-        raise ValueError(f"[KeOps] bucket_attention: bias must be ({h}, {buckets.num_buckets}), float32 or {dtype}; got "
-                         f"{tuple(bias.shape)}, {bias.dtype}.")
+    start = query_start if type(query_start) is int else None
+    plan = key = None
+    try:
+        key = (_geometry(q), _geometry(k), _geometry(v), _geometry(bias), bool(causal), start, scale)
+        plan = buckets._plans.get(key)
+    except (AttributeError, TypeError):  # not tensors, no PositionBuckets: said below
+        pass
+    if plan is None:
+        _check_bucket(q, k, v, bias, buckets, query_start)
+        d = q.shape[3]
+        number = d ** -0.5 if scale is None else float(scale)
+        align = 16 // q.element_size()
+        if d % align or not all(map(_strides_fit, (q, k, v))) or bias.dtype != torch.float32 or not bias.is_contiguous():
+            out = bucket_attention(_rows(_pad(q, align)), _rows(_pad(k, align)), _rows(_pad(v, align)), bias.float().contiguous(), buckets,
+                                   causal=causal, key_lengths=key_lengths, query_start=query_start, scale=number)
+            return out if out.shape[3] == d else out[..., :d].contiguous()
+        plan = _keep(buckets._plans, key, _BucketPlan(q, k, v, bias, buckets, causal, start or 0, number))
+    if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15:
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        return bucket_attention(q, k, v, bias, buckets, causal=causal, key_lengths=key_lengths, query_start=query_start, scale=scale)
+    batch, device = q.shape[:1], q.device
     if key_lengths is not None:
-        key_lengths = _check_whole(what, "key_lengths", key_lengths, (b,), device)
-    if isinstance(query_start, torch.Tensor):
-        query_start = _check_whole(what, "query_start", query_start, (b,), device)
-    elif isinstance(query_start, bool) or not isinstance(query_start, int) or abs(query_start) > 1 << 29:
-        raise ValueError("[KeOps] bucket_attention: query_start must be a whole number of absolute value at most 2**29, or a tensor.")
-    scale = d ** -0.5 if scale is None else float(scale)
-    align = 16 // q.element_size()
-    q, k, v, bias = _pad(q, align), _pad(k, align), _pad(v, align), bias.float().contiguous()
-    options = (buckets, bool(causal), key_lengths, query_start, scale)
-    if _needs_grad(q, k, v, bias):
-        out = _BucketAttention.apply(q, k, v, bias, options)
-    else:
-        out = _bucket_forward(q, k, v, bias, options, False)[3]
-    return out if out.shape[3] == d else out[..., :d].contiguous()
+        key_lengths = _check_whole("bucket_attention", "key_lengths", key_lengths, batch, device)
+    start = _check_whole("bucket_attention", "query_start", query_start, batch, device) if start is None else None
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or bias.requires_grad):
+        return _BucketAttention.apply(q, k, v, bias, plan, key_lengths, start)
+    return plan.forward(q, k, v, bias, key_lengths, start, False)[0]
 
 
 # --------------------------------------------------------------------------------------------------- decay attention
-def _decay_run(q, k, v, log_decay, lengths, heads, *, reverse=False, product_scale=1.0, query_scale=1.0, update_scale=1.0, state=None,
-               transposed=False, out=None, float32=False, want_state=False, states=None):
-    """One walk over the tokens (keops_hip_decay_attention of include/keops_hip.h).  ``transposed``: ``state`` and ``states`` hold
-    the transposes of the matrices that the walk starts from; ``states``: the workspace of the walk that left them.  Returns the
-    outputs, the final state (or None) and the workspace."""
-    b, t, d, dv = q.shape[0], q.shape[2], q.shape[3], v.shape[3]
-    if out is None:
-        out = torch.empty(b, heads, t, dv, dtype=torch.float32 if float32 else q.dtype, device=q.device)
-    last = torch.empty(b, heads, d, dv, dtype=torch.float32, device=q.device) if want_state else None
-    if b == 0 or heads == 0:
-        return out, last, None
-    a = binder.DecayAttention()
-    a.dtype, a.batch, a.heads, a.dim, a.dim_v, a.tokens = _DTYPES[q.dtype], b, heads, d, dv, t
-    a.q_heads, a.k_heads, a.v_heads = q.shape[1], k.shape[1], v.shape[1]
-    a.reverse, a.out_float32 = int(reverse), int(out.dtype == torch.float32)
-    a.product_scale, a.query_scale, a.update_scale = product_scale, query_scale, update_scale
-    a.q, a.k, a.v, a.out = _ptr(q), _ptr(k), _ptr(v), _ptr(out)
-    a.q_stride[:], a.k_stride[:], a.v_stride[:], a.out_stride[:] = _stride(q), _stride(k), _stride(v), _stride(out)
-    a.log_decay, a.lengths, a.state_in, a.state_out = _ptr(log_decay), _ptr(lengths), _ptr(state), _ptr(last)
-    a.state_in_stride[:] = (1, d) if transposed else (dv, 1)
-    a.state_out_stride[:] = (dv, 1)
-    lib = binder.lib()
-    a.states_given = int(states is not None)
-    a.states_stride[:] = (1, d) if transposed and states is not None else (dv, 1)
-    if states is None:
-        states = torch.empty(lib.keops_hip_decay_attention_bytes(ctypes.byref(a)) // 4, dtype=torch.float32, device=q.device)
-    a.states, a.states_bytes = _ptr(states), 4 * states.numel()
-    stream = torch.cuda.current_stream(q.device).cuda_stream
-    binder.check(lib.keops_hip_decay_attention_run(ctypes.byref(a), q.device.index, stream), "keops_hip_decay_attention_run")
-    return out, last, states
+class _DecayWalk:
+    """One walk over the tokens (keops_hip_decay_attention of include/keops_hip.h): its arguments that depend on the geometry of
+    the tensors alone.  q, k, v, out: (shape, strides)."""
+
+    def __init__(self, dtype, device, heads, q, k, v, out, out_dtype, *, reverse=False, product_scale=1.0, query_scale=1.0,
+                 update_scale=1.0, transposed=False, given=False):
+        (b, _, t, d), dv = q[0], v[0][3]
+        self.device, self.index, self.out_dtype, self.given = device, device.index, out_dtype, given
+        self.out, self.state_shape = out, (b, heads, d, dv)
+        a = binder.DecayAttention()
+        a.dtype, a.batch, a.heads, a.dim, a.dim_v, a.tokens = _DTYPES[dtype], b, heads, d, dv, t
+        a.q_heads, a.k_heads, a.v_heads = q[0][1], k[0][1], v[0][1]
+        a.reverse, a.out_float32 = int(reverse), int(out_dtype == torch.float32)
+        a.product_scale, a.query_scale, a.update_scale = product_scale, query_scale, update_scale
+        a.q_stride[:], a.k_stride[:], a.v_stride[:], a.out_stride[:] = (_stride(*x) for x in (q, k, v, out))
+        a.state_in_stride[:] = (1, d) if transposed else (dv, 1)
+        a.state_out_stride[:] = (dv, 1)
+        a.states_stride[:] = (1, d) if transposed and given else (dv, 1)
+        a.states_given = int(given)
+        self.empty = b == 0 or heads == 0
+        if not self.empty:
+            a.q = a.k = a.v = a.out = a.log_decay = 16  # placeholders for the library's own checks
+            self.states = binder.lib().keops_hip_decay_attention_bytes(ctypes.byref(a)) // 4
+            a.states_bytes = 4 * self.states
+        self.args = bytes(a)
+
+    def __call__(self, q, k, v, log_decay, lengths, state, want_state=False, states=None):
+        """Outputs, the final state (or None) and the workspace; ``states``: the workspace of the walk that left the states."""
+        out = torch.empty_strided(*self.out, dtype=self.out_dtype, device=self.device)
+        last = torch.empty(self.state_shape, dtype=torch.float32, device=self.device) if want_state else None
+        if self.empty:
+            return out, last, None
+        if states is None:
+            states = torch.empty(self.states, dtype=torch.float32, device=self.device)
+        a = binder.DecayAttention.from_buffer_copy(self.args)
+        a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+        a.log_decay, a.states = log_decay.data_ptr(), states.data_ptr()
+        if lengths is not None:
+            a.lengths = lengths.data_ptr()
+        if state is not None:
+            a.state_in = state.data_ptr()
+        if want_state:
+            a.state_out = last.data_ptr()
+        rc = binder.lib().keops_hip_decay_attention_run(ctypes.byref(a), self.index, _raw_stream(self.index))
+        if rc:
+            binder.check(rc, "keops_hip_decay_attention_run")
+        return out, last, states
 
 
-def _decay_out(q, v):
-    """Outputs: q's order of dimensions, v's components."""
-    if q.shape[3] == v.shape[3]:
-        return _like(q)
-    if q.dim() == 4 and q.stride(1) < q.stride(2):  # (batch, tokens, heads, dim) in memory
-        return torch.empty(q.shape[0], q.shape[2], q.shape[1], v.shape[3], dtype=q.dtype, device=q.device).transpose(1, 2)
-    return torch.empty(*q.shape[:3], v.shape[3], dtype=q.dtype, device=q.device)
+class _DecayPlan:
+    """The walks of a call and of its gradients."""
 
+    def __init__(self, q, k, v, scale):
+        self.dtype, self.device, self.scale, self.heads, self.shared = q.dtype, q.device, scale, q.shape[1], k.shape[1]
+        self.q, self.k, self.v = ((x.shape, x.stride()) for x in (q, k, v))
+        shape = (*q.shape[:3], v.shape[3])
+        if q.shape[3] == v.shape[3]:
+            strides = _dense_strides(q)
+        elif q.stride(1) < q.stride(2):  # (batch, tokens, heads, dim) in memory
+            strides = torch.empty(shape[0], shape[2], shape[1], shape[3], device="meta").transpose(1, 2).stride()
+        else:
+            strides = torch.empty(shape, device="meta").stride()
+        self.out = (torch.Size(shape), strides)
+        self.like = {"q": (q.shape, _dense_strides(q)), "k": (k.shape, _dense_strides(k)), "v": (v.shape, _dense_strides(v))}
+        self.forward = self.walk(self.q, self.k, self.v, self.out, self.dtype, query_scale=scale)
+        self.gradients = {}
 
-def _decay_forward(q, k, v, log_decay, state, lengths, scale):
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    out, last, states = _decay_run(q, k, v, log_decay, lengths, q.shape[1], product_scale=scale, query_scale=scale, state=state,
-                                   out=_decay_out(q, v), want_state=True)
-    return q, k, v, out, last, states
+    def walk(self, q, k, v, out, out_dtype, **options):
+        return _DecayWalk(self.dtype, self.device, self.heads, q, k, v, out, out_dtype, product_scale=self.scale, **options)
+
+    def backward(self, grad_strides):
+        """The walks that give the gradients of q, v and k.  A shared head's gradient is the sum over the heads that share it, rounded
+        once: those walks leave float32 for each head."""
+        walks = self.gradients.get(grad_strides)
+        if walks is None:
+            g = (self.out[0], grad_strides)
+            per_head = self.heads == self.shared
+
+            def like(name):
+                shape, strides = self.like[name]
+                if per_head:
+                    return (shape, strides), self.dtype
+                shape = torch.Size((shape[0], self.heads, *shape[2:]))
+                return (shape, torch.empty(shape, device="meta").stride()), torch.float32
+
+            walks = _keep(self.gradients, grad_strides, (
+                self.walk(g, self.v, self.k, self.like["q"], self.dtype, query_scale=self.scale, transposed=True, given=True),
+                self.walk(self.k, self.q, g, *like("v"), reverse=True, update_scale=self.scale),
+                self.walk(self.v, g, self.q, *like("k"), reverse=True, update_scale=self.scale, transposed=True),
+                self.walk(self.v, g, self.q, *like("k"), reverse=True, update_scale=self.scale, transposed=True, given=True),
+            ))
+        return walks
+
+    def join(self, x):
+        """Per head -> per shared head."""
+        if self.heads == self.shared:
+            return x
+        b, h, t, d = x.shape
+        return x.view(b, self.shared, h // self.shared, t, d).sum(2).to(self.dtype)
 
 
 class _DecayAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, state, log_decay, lengths, scale):
+    def forward(ctx, q, k, v, state, log_decay, lengths, plan):
         ctx.set_materialize_grads(False)
-        q, k, v, out, last, states = _decay_forward(q, k, v, log_decay, state, lengths, scale)
-        ctx.scale = scale
+        out, last, states = plan.forward(q, k, v, log_decay, lengths, state, True)
+        ctx.plan = plan
         ctx.save_for_backward(q, k, v, state, log_decay, lengths, states)
         return out, last
 
@@ -358,27 +453,30 @@ class _DecayAttention(torch.autograd.Function):
         # gradients are walks of the same kind (csrc/sequence/keops_seq_decay.hip); that of q starts from the forward pass's states,
         # that of k from those of v's
         q, k, v, state, log_decay, lengths, states = ctx.saved_tensors
-        (b, h, t, d), dv, scale, shared = q.shape, v.shape[3], ctx.scale, k.shape[1]
-        grad = torch.zeros(b, h, t, dv, dtype=q.dtype, device=q.device) if grad is None else _rows(grad)
+        plan = ctx.plan
+        grad = torch.zeros(plan.out[0], dtype=q.dtype, device=q.device) if grad is None else _rows(grad)
         grad_last = None if grad_last is None else grad_last.contiguous()
-
-        def walk(*data, like, **options):
-            # a shared head's gradient is the sum over the heads that share it, rounded once
-            out = None if like.shape[1] != h else _like(like)
-            out, last, left = _decay_run(*data, log_decay, lengths, h, product_scale=scale, out=out, float32=True, **options)
-            if like.shape[1] != h:
-                out = out.view(b, shared, h // shared, t, -1).sum(2).to(like.dtype)
-            return out, last, left
-
+        to_q, to_v, to_k, to_k_given = plan.backward(grad.stride())
         want_q, want_k, want_v, want_state = ctx.needs_input_grad[:4]
-        dq = dk = dv_ = ds = back = None
+        dq = dk = dv = ds = None
         if want_q:
-            dq = walk(grad, v, k, like=q, query_scale=scale, state=state, transposed=True, states=states)[0]
+            dq = to_q(grad, v, k, log_decay, lengths, state, states=states)[0]
         if want_v or want_state:
-            dv_, ds, back = walk(k, q, grad, like=v, reverse=True, update_scale=scale, state=grad_last, want_state=want_state)
+            dv, ds, back = to_v(k, q, grad, log_decay, lengths, grad_last, want_state)
+            dv = plan.join(dv)
         if want_k:
-            dk = walk(v, grad, q, like=k, reverse=True, update_scale=scale, state=grad_last, transposed=True, states=back)[0]
-        return dq, dk, dv_, ds, None, None, None
+            if dv is None:
+                dk = to_k(v, grad, q, log_decay, lengths, grad_last)[0]
+            else:
+                dk = to_k_given(v, grad, q, log_decay, lengths, grad_last, states=back)[0]
+            dk = plan.join(dk)
+        return dq, dk, dv, ds, None, None, None
+
+
+_decay_plans, _step_plans = {}, {}
+
+
+_CONSTANT = "[KeOps] {}: log_decay is a constant of the layer, no gradient with respect to it is computed; detach it."
 
 
 def _check_decay(what, q, k, v, log_decay, state, dims):
@@ -403,7 +501,7 @@ def _check_decay(what, q, k, v, log_decay, state, dims):
     if log_decay is None:
         raise ValueError(f"[KeOps] {what}: log_decay must be a float32 tensor of shape ({h},).")
     if log_decay.requires_grad and torch.is_grad_enabled():
-        raise ValueError(f"[KeOps] {what}: log_decay is a constant of the layer, no gradient with respect to it is computed; detach it.")
+        raise ValueError(_CONSTANT.format(what))
     return device
 
 
@@ -426,27 +524,38 @@ def decay_attention(q, k, v, log_decay, *, initial_state=None, lengths=None, sca
     which :func:`decay_attention_step` or another call goes on.  Differentiable with respect to q, k, v and initial_state, through
     both results.  Tokens are worked on in chunks of 64; a value that is not finite can reach earlier tokens of its chunk.
     """
-    what = "decay_attention"
-    device = _check_decay(what, q, k, v, log_decay, initial_state, 4)
-    d, dv = q.shape[3], v.shape[3]
-    if q.shape[2] > 1 << 29:
-        raise ValueError("[KeOps] decay_attention: at most 2**29 tokens.")
+    plan = key = None
+    try:
+        key = (_geometry(q), _geometry(k), _geometry(v), _geometry(initial_state), _geometry(log_decay), scale)
+        plan = _decay_plans.get(key)
+    except (AttributeError, TypeError):  # not tensors: said below
+        pass
+    if plan is None:
+        device = _check_decay("decay_attention", q, k, v, log_decay, initial_state, 4)
+        if q.shape[2] > 1 << 29:
+            raise ValueError("[KeOps] decay_attention: at most 2**29 tokens.")
+        d, dv = q.shape[3], v.shape[3]
+        number = d ** -0.5 if scale is None else float(scale)
+        align = 16 // q.element_size()
+        if (d % align or dv % align or not all(map(_strides_fit, (q, k, v))) or not log_decay.is_contiguous()
+                or (initial_state is not None and not initial_state.is_contiguous())):
+            state = None if initial_state is None else _pad(initial_state, align, align).contiguous()
+            out, last = decay_attention(_rows(_pad(q, align)), _rows(_pad(k, align)), _rows(_pad(v, align)), log_decay.contiguous(),
+                                        initial_state=state, lengths=lengths, scale=number)
+            return (out if out.shape[3] == dv else out[..., :dv].contiguous(),
+                    last if last.shape[2:] == (d, dv) else last[:, :, :d, :dv].contiguous())
+        plan = _keep(_decay_plans, key, _DecayPlan(q, k, v, number))
+    if (q.data_ptr() | k.data_ptr() | v.data_ptr()) & 15 or (initial_state is not None and initial_state.data_ptr() & 15):
+        state = None if initial_state is None else initial_state.clone()
+        return decay_attention(_rows(q), _rows(k), _rows(v), log_decay, initial_state=state, lengths=lengths, scale=scale)
     if lengths is not None:
-        lengths = _check_whole(what, "lengths", lengths, (q.shape[0],), device)
-    scale = d ** -0.5 if scale is None else float(scale)
-    align = 16 // q.element_size()
-    q, k, v = _pad(q, align), _pad(k, align), _pad(v, align)
-    state = None if initial_state is None else _pad(initial_state, align, align).contiguous()
-    log_decay = log_decay.contiguous()
-    if _needs_grad(q, k, v, state):
-        out, last = _DecayAttention.apply(q, k, v, state, log_decay, lengths, scale)
-    else:
-        out, last = _decay_forward(q, k, v, log_decay, state, lengths, scale)[3:5]
-    if out.shape[3] != dv:
-        out = out[..., :dv].contiguous()
-    if last.shape[2:] != (d, dv):
-        last = last[:, :, :d, :dv].contiguous()
-    return out, last
+        lengths = _check_whole("decay_attention", "lengths", lengths, q.shape[:1], q.device)
+    if torch.is_grad_enabled():
+        if log_decay.requires_grad:
+            raise ValueError(_CONSTANT.format("decay_attention"))
+        if q.requires_grad or k.requires_grad or v.requires_grad or (initial_state is not None and initial_state.requires_grad):
+            return _DecayAttention.apply(q, k, v, initial_state, log_decay, lengths, plan)
+    return plan.forward(q, k, v, log_decay, lengths, initial_state, True)[:2]
 
 
 def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
@@ -461,28 +570,40 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
 
     Returns (batch, heads, dim_v) in the type of q.  No gradients.
     """
-    what = "decay_attention_step"
-    if state is None:
-        raise ValueError("[KeOps] decay_attention_step: state must be a float32 tensor of shape (batch, heads, dim, dim_v).")
-    device = _check_decay(what, q, k, v, log_decay, state, 3)
-    if _needs_grad(q, k, v, state):
+    key = plan = None
+    try:
+        key = (_geometry(q), _geometry(k), _geometry(v), _geometry(state), _geometry(log_decay), scale)
+        plan = _step_plans.get(key)
+    except (AttributeError, TypeError):  # not tensors: said below
+        pass
+    if plan is None:
+        what = "decay_attention_step"
+        if state is None:
+            raise ValueError("[KeOps] decay_attention_step: state must be a float32 tensor of shape (batch, heads, dim, dim_v).")
+        _check_decay(what, q, k, v, log_decay, state, 3)
+        if v.shape[2] % 4:
+            raise ValueError(f"[KeOps] decay_attention_step: dim_v must be a multiple of 4, it is {v.shape[2]}.")
+        if not state.is_contiguous():
+            raise ValueError("[KeOps] decay_attention_step: state must be contiguous, it is overwritten.")
+        if not all(x.stride(2) == 1 or x.shape[2] == 1 for x in (q, k, v)) or not log_decay.is_contiguous():
+            return decay_attention_step(q.contiguous(), k.contiguous(), v.contiguous(), log_decay.contiguous(), state, scale=scale)
+        b, h, d = q.shape
+        pair = ctypes.c_int64 * 2
+        plan = _keep(_step_plans, key, (
+            (_DTYPES[q.dtype], b, h, k.shape[1], d, v.shape[2], d ** -0.5 if scale is None else float(scale)),
+            pair(*q.stride()[:2]), pair(*k.stride()[:2]), pair(*v.stride()[:2]), (b, h, v.shape[2]), q.device.index))
+    if state.data_ptr() & 15:
+        raise ValueError("[KeOps] decay_attention_step: state must be aligned to 16 bytes, it is overwritten.")
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or state.requires_grad or log_decay.requires_grad):
         raise ValueError("[KeOps] decay_attention_step overwrites the state and has no gradient: use decay_attention, or torch.no_grad().")
-    if v.shape[2] % 4:
-        raise ValueError(f"[KeOps] decay_attention_step: dim_v must be a multiple of 4, it is {v.shape[2]}.")
-    if not state.is_contiguous() or state.data_ptr() % 16:
-        raise ValueError("[KeOps] decay_attention_step: state must be contiguous and aligned to 16 bytes, it is overwritten.")
-    b, h, d = q.shape
-    q, k, v = (x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous() for x in (q, k, v))
-    out = torch.empty(b, h, v.shape[2], dtype=q.dtype, device=device)
-    if out.numel() == 0:
-        return out
-    pair = ctypes.c_int64 * 2
-    log_decay = log_decay.contiguous()
-    rc = binder.lib().keops_hip_decay_attention_step(
-        _DTYPES[q.dtype], b, h, k.shape[1], d, v.shape[2], d ** -0.5 if scale is None else float(scale), _ptr(q), pair(*q.stride()[:2]),
-        _ptr(k), pair(*k.stride()[:2]), _ptr(v), pair(*v.stride()[:2]), _ptr(log_decay), _ptr(state), _ptr(out), device.index,
-        torch.cuda.current_stream(device).cuda_stream)
-    binder.check(rc, "keops_hip_decay_attention_step")
+    head, q_stride, k_stride, v_stride, shape, index = plan
+    out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    if shape[0] and shape[1]:
+        rc = binder.lib().keops_hip_decay_attention_step(
+            *head, q.data_ptr(), q_stride, k.data_ptr(), k_stride, v.data_ptr(), v_stride, log_decay.data_ptr(), state.data_ptr(),
+            out.data_ptr(), index, _raw_stream(index))
+        if rc:
+            binder.check(rc, "keops_hip_decay_attention_step")
     return out
 
 
@@ -497,21 +618,20 @@ class TokenLogprobs(NamedTuple):
 
 
 def _logprobs_forward(logits, tokens, top, ignore_index):
-    rows, vocab = logits.shape
-    f32 = dict(dtype=torch.float32, device=logits.device)
-    logprob, entropy, lse = torch.empty(rows, **f32), torch.empty(rows, **f32), torch.empty(rows, **f32)
-    top_logprob = torch.empty(rows, top, **f32)
-    top_index = torch.empty(rows, top, dtype=torch.int64, device=logits.device)
+    (rows, vocab), device = logits.shape, logits.device
+    logprob, entropy, lse = torch.empty((3, rows), dtype=torch.float32, device=device).unbind(0)
+    top_logprob = torch.empty((rows, top), dtype=torch.float32, device=device)
+    top_index = torch.empty((rows, top), dtype=torch.int64, device=device)
     if rows:
         lib = binder.lib()
         dt = _DTYPES[logits.dtype]
         nbytes = lib.keops_hip_token_logprobs_bytes(dt, rows, vocab, top)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
+        work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         rc = lib.keops_hip_token_logprobs(
             dt, rows, vocab, top, _ptr(logits), logits.stride(0), _ptr(tokens), ignore_index, _ptr(logprob), _ptr(entropy), _ptr(lse),
-            _ptr(top_logprob), _ptr(top_index), _ptr(work), nbytes, logits.device.index,
-            torch.cuda.current_stream(logits.device).cuda_stream)
-        binder.check(rc, "keops_hip_token_logprobs")
+            _ptr(top_logprob), _ptr(top_index), _ptr(work), nbytes, device.index, _raw_stream(device.index))
+        if rc:
+            binder.check(rc, "keops_hip_token_logprobs")
     return logprob, entropy, lse, top_logprob, top_index
 
 
@@ -536,8 +656,9 @@ class _TokenLogprobs(torch.autograd.Function):
             rc = binder.lib().keops_hip_token_logprobs_backward(
                 _DTYPES[logits.dtype], rows, vocab, ctx.top, _ptr(logits), logits.stride(0), _ptr(tokens), ctx.ignore_index,
                 _ptr(entropy), _ptr(lse), _ptr(top_index), _ptr(g_logprob), _ptr(g_entropy), _ptr(g_top), _ptr(grad), vocab,
-                logits.device.index, torch.cuda.current_stream(logits.device).cuda_stream)
-            binder.check(rc, "keops_hip_token_logprobs_backward")
+                logits.device.index, _raw_stream(logits.device.index))
+            if rc:
+                binder.check(rc, "keops_hip_token_logprobs_backward")
         return grad, None, None, None
 
 
@@ -576,7 +697,7 @@ def token_logprobs(logits, tokens, *, top=0, ignore_index=-100):
     if flat.stride(1) != 1 and vocab > 1:
         flat = flat.contiguous()
     tokens = tokens.reshape(-1).long().contiguous()
-    if _needs_grad(logits):
+    if torch.is_grad_enabled() and logits.requires_grad:
         logprob, entropy, top_logprob, top_index = _TokenLogprobs.apply(flat, tokens, top, int(ignore_index))
     else:
         logprob, entropy, _, top_logprob, top_index = _logprobs_forward(flat, tokens, top, int(ignore_index))
