@@ -4,10 +4,11 @@
 // are non-negative, so nothing cancels; x - m is formed before it is scaled, so large logits lose nothing.  m, s and t are kept
 // for each thread (a new maximum m' turns t into e^(m-m') (t + s (m-m'))) and joined at the end.
 //
-// The K largest: a value enters a list in LDS when it exceeds the K-th of what the list last held; the list is cut to its K
-// largest when half full.  The first threshold is the K-th largest of the threads' own maxima.  Keys are the value's bits in
-// increasing order, then the complement of the index, so equal values keep the lowest index and every key is different: the
-// result does not depend on the order in which values arrive.
+// The K largest: each wavefront keeps a list in LDS, which a value enters when it exceeds the K-th of what the list last held; the
+// list is cut to its K largest when it fills.  The first threshold is the K-th largest of the lanes' own maxima, so in the sweep
+// almost every vector of a row costs one comparison and no barrier.  Keys are the value's bits in increasing order, then the
+// complement of the index, so equal values keep the lowest index and every key is different: the result does not depend on the
+// order in which values arrive.
 #include "../../../include/keops_hip.h"
 #include "keops_seq.h"
 
@@ -15,25 +16,11 @@ using namespace kseq;
 
 namespace {
 
-constexpr int kThreads = 256, kList = 512, kMaxTop = KEOPS_HIP_MAX_TOP, kUnroll = 4;
+constexpr int kThreads = 256, kList = 512, kWaveList = 192, kMaxTop = KEOPS_HIP_MAX_TOP, kUnroll = 4;
 constexpr float kLn2 = 0.6931471805599453f;
 typedef unsigned long long u64;
 
 struct Stat { float m, s, t; };
-__device__ inline Stat join(const Stat& a, const Stat& b) {
-  if (a.m == -kInf) return b;
-  if (b.m == -kInf) return a;
-  const float m = fmaxf(a.m, b.m), da = a.m - m, db = b.m - m;
-  const float ea = __builtin_amdgcn_exp2f(da * kLog2e), eb = __builtin_amdgcn_exp2f(db * kLog2e);
-  Stat r;
-  r.m = m;
-  r.s = ea * a.s + eb * b.s;
-  // (a factor that has vanished takes its sums with it: s (m - m') may be infinite where logits are near the type's lowest value)
-  r.t = (ea == 0.f ? 0.f : ea * (a.t + a.s * da)) + (eb == 0.f ? 0.f : eb * (b.t + b.s * db));
-  // a value of +inf or NaN makes the row's sums NaN
-  if (!(m < kInf)) r.s = r.t = __builtin_nanf("");
-  return r;
-}
 
 __device__ inline unsigned ordered(float x) {
   const unsigned b = __float_as_uint(x + 0.f);
@@ -78,6 +65,25 @@ template <class T> __device__ inline void unpack(const uint4& u, float (&x)[16 /
   for (int k = 0; k < (int)(16 / sizeof(T)); k++) x[k] = (float)w.e[k];
 }
 
+// element k of a 16-byte vector
+template <class T> __device__ inline float element(const uint4& u, int k) {
+  if constexpr (sizeof(T) == 4) {
+    return __uint_as_float(k == 0 ? u.x : (k == 1 ? u.y : (k == 2 ? u.z : u.w)));
+  } else {
+    const unsigned w = k < 2 ? u.x : (k < 4 ? u.y : (k < 6 ? u.z : u.w));
+    union { unsigned short b; T e; } x;
+    x.b = (unsigned short)(k & 1 ? w >> 16 : w);
+    return (float)x.e;
+  }
+}
+
+// LDS accesses of a wavefront before this come before those behind it
+__device__ inline void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // list[0..n) -> its `top` largest in decreasing order, in list[0..); returns how many.  All threads of the workgroup.
 __device__ inline int cut(u64* list, u64* best, int n, int top, int tid) {
   __syncthreads();
@@ -88,6 +94,7 @@ __device__ inline int cut(u64* list, u64* best, int n, int top, int tid) {
     mine[i] = tid + i * kThreads < n ? list[tid + i * kThreads] : 0;
     rank[i] = 0;
   }
+#pragma unroll 8
   for (int j = 0; j < n; j++) {
     const u64 o = list[j];
 #pragma unroll
@@ -101,6 +108,30 @@ __device__ inline int cut(u64* list, u64* best, int n, int top, int tid) {
   if (tid < left) list[tid] = best[tid];
   __syncthreads();
   return left;
+}
+
+// the same for the list of one wavefront (n <= kWaveList different keys)
+__device__ inline int cut_wave(u64* list, int n, int top, int lane) {
+  constexpr int E = kWaveList / 64;
+  u64 mine[E];
+  int rank[E];
+#pragma unroll
+  for (int i = 0; i < E; i++) {
+    mine[i] = lane + 64 * i < n ? list[lane + 64 * i] : 0;
+    rank[i] = 0;
+  }
+#pragma unroll 8
+  for (int j = 0; j < n; j++) {
+    const u64 o = list[j];
+#pragma unroll
+    for (int i = 0; i < E; i++) rank[i] += o > mine[i] ? 1 : 0;
+  }
+  wave_fence();
+#pragma unroll
+  for (int i = 0; i < E; i++)
+    if (lane + 64 * i < n && rank[i] < top) list[rank[i]] = mine[i];
+  wave_fence();
+  return n < top ? n : top;
 }
 
 struct Out {
@@ -126,32 +157,43 @@ __device__ inline void finish_top(const Out& o, long long at, const Stat& st, u6
   o.top_index[at] = (int64_t)(0xffffffffu - (unsigned)key);
 }
 
-// joins the threads' sums; every thread gets the result
-__device__ inline Stat join_all(Stat st, Stat* red, int tid) {
+// joins the sums of a wavefront's lanes; every lane gets the result.  The largest m first, so that every lane scales its sums once.
+__device__ inline Stat join_lanes(Stat st) {
+  float m = st.m, bad = !(st.m < kInf) || st.s != st.s ? 1.f : 0.f;  // +inf or NaN: the row's sums are NaN
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  const float d = st.m - m, f = st.m == -kInf ? 0.f : __builtin_amdgcn_exp2f(d * kLog2e);
+  st.t = f == 0.f ? 0.f : f * (st.t + st.s * d);  // (a factor that has vanished takes its sums with it: s (m - m') may be infinite)
+  st.s = f == 0.f ? 0.f : f * st.s;
+  if (__any(bad != 0.f)) st.s = st.t = __builtin_nanf("");
+  st.m = m;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
-    Stat b;
-    b.m = __shfl_xor(st.m, o);
-    b.s = __shfl_xor(st.s, o);
-    b.t = __shfl_xor(st.t, o);
-    st = join(st, b);
+    st.s += __shfl_xor(st.s, o);
+    st.t += __shfl_xor(st.t, o);
   }
-  __syncthreads();
+  return st;
+}
+// joins the threads' sums (NT threads); the first wavefront gets the result
+template <int NT> __device__ inline Stat join_all(Stat st, Stat* red, int tid) {
+  st = join_lanes(st);
   if ((tid & 63) == 0) red[tid >> 6] = st;
   __syncthreads();
-  return join(join(red[0], red[1]), join(red[2], red[3]));
+  if (tid < 64) st = join_lanes(tid < NT / 64 ? red[tid] : Stat{-kInf, 0.f, 0.f});
+  return st;
 }
 
 // one row, or one share of a row's columns (which then leaves its sums and keys in `part`)
-template <class T, bool TOP>
-__global__ void __launch_bounds__(kThreads) logprobs_rows(long long vocab, int top, const T* logits, long long stride, const int64_t* tokens, int64_t ignore,
-                                                          Out out, int splits, float* part_stat, u64* part_key) {
-  constexpr int VE = 16 / (int)sizeof(T), U = kUnroll;
-  __shared__ Stat red[4];
-  __shared__ u64 list[TOP ? kList : 1], best[TOP ? kMaxTop : 1];
-  __shared__ unsigned maxima[TOP ? kThreads : 1], cutoff;
-  __shared__ int held;
-  const int tid = threadIdx.x;
+template <class T, bool TOP, int NT>
+__global__ void __launch_bounds__(NT) logprobs_rows(long long vocab, int top, const T* logits, long long stride, const int64_t* tokens, int64_t ignore,
+                                                    Out out, int splits, float* part_stat, u64* part_key) {
+  constexpr int VE = 16 / (int)sizeof(T), U = kUnroll, NW = NT / 64;
+  __shared__ Stat red[NW];
+  __shared__ u64 lists[TOP ? NW : 1][TOP ? kWaveList : 1], list[TOP ? NW * kMaxTop : 1], best[TOP ? kMaxTop : 1], floors[NW];
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  u64* const own = lists[TOP ? wave : 0];
+  int held = 0;  // keys in it
   const long long row = blockIdx.x / splits;
   const int split = blockIdx.x % splits;
   const T* x = logits + row * stride;
@@ -159,39 +201,49 @@ __global__ void __launch_bounds__(kThreads) logprobs_rows(long long vocab, int t
   const Row r = row_of(x, v0, v1 < v0 ? v0 : v1);
   Stat st = {-kInf, 0.f, 0.f};
   u64 least = 0;  // keys up to this one are not among the largest
-  float least_value = -kInf;
-  if (TOP && tid == 0) held = 0;
+  float least_value = -kInf, lane_max = -kInf;
+  bool lane_any = false;
+
+  // K-th largest of the lanes' maxima, to 16 bits and from below: at least K values reach it
+  const auto raise = [&]() __attribute__((always_inline)) {
+    const unsigned mine = lane_any ? ordered(lane_max) : 0u;
+    unsigned at = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; bit--) {
+      const unsigned with = at | 1u << bit;
+      if (__popcll(__ballot(mine >= with)) >= top) at = with;
+    }
+    if ((u64)at << 32 > least) {
+      least = (u64)at << 32;
+      least_value = value_of(least);
+    }
+  };
 
   uint4 next[U];
 #pragma unroll
   for (int u = 0; u < U; u++)
-    if (tid + u * kThreads < r.count) next[u] = load_vec(x, r, tid + u * kThreads);
-  for (int j0 = 0; j0 < r.count; j0 += U * kThreads) {
+    if (tid + u * NT < r.count) next[u] = load_vec(x, r, tid + u * NT);
+  for (int j0 = 0; j0 < r.count; j0 += U * NT) {
     uint4 now[U];
 #pragma unroll
     for (int u = 0; u < U; u++) now[u] = next[u];
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int j = j0 + (U + u) * kThreads + tid;
+      const int j = j0 + (U + u) * NT + tid;
       if (j < r.count) next[u] = load_vec(x, r, j);
     }
     float vmax[U];
 #pragma unroll
     for (int u = 0; u < U; u++) {
       vmax[u] = -kInf;
-      if (j0 + u * kThreads + tid >= r.count) continue;
+      if (j0 + u * NT + tid >= r.count) continue;
       float e[VE];
       unpack<T>(now[u], e);
       float mx = e[0];
-      bool nan = e[0] != e[0];
 #pragma unroll
-      for (int k = 1; k < VE; k++) {
-        mx = fmaxf(mx, e[k]);
-        nan |= e[k] != e[k];
-      }
-      if (nan) mx = __builtin_nanf("");
+      for (int k = 1; k < VE; k++) mx = fmaxf(mx, e[k]);  // (NaN only if all are: the sums below find the others)
       vmax[u] = mx;
-      if (!(mx <= st.m)) {  // a new maximum (or NaN, which stays)
+      if (!(mx <= st.m)) {  // a new maximum
         if (st.m != -kInf) {
           const float d = st.m - mx, f = __builtin_amdgcn_exp2f(d * kLog2e);
           st.t = f == 0.f ? 0.f : f * (st.t + st.s * d);
@@ -204,82 +256,97 @@ __global__ void __launch_bounds__(kThreads) logprobs_rows(long long vocab, int t
         for (int k = 0; k < VE; k++) {
           const float d = e[k] - st.m, f = __builtin_amdgcn_exp2f(d * kLog2e);
           st.s += f;
-          st.t += f == 0.f ? 0.f : f * d;  // -inf adds nothing
+          st.t = fmaf(f, fmaxf(d, -1e4f), st.t);  // (-inf adds nothing: 0 * -1e4)
         }
+      } else {
+#pragma unroll
+        for (int k = 0; k < VE; k++)
+          if (e[k] != e[k]) st.m = e[k];  // NaN beside -inf
+      }
+      if (TOP) {
+        lane_max = fmaxf(lane_max, mx);
+        lane_any = true;
       }
     }
     if constexpr (TOP) {
-      const auto in_row = [&](int u) { return j0 + u * kThreads + tid < r.count; };
-      if (j0 == 0) {
-        // K-th largest of the threads' maxima: at least K values reach it
-        unsigned mine = 0;
+      if (j0 == 0) raise();
 #pragma unroll
-        for (int u = 0; u < U; u++)
-          if (in_row(u)) mine = max(mine, vmax[u] != vmax[u] ? 0xffffffffu : ordered(vmax[u]));
-        maxima[tid] = mine;
-        if (tid == 0) cutoff = 0;
-        __syncthreads();
-        int rank = 0;
-        for (int i = 0; i < kThreads; i += 4) {
-          const uint4 o = *reinterpret_cast<const uint4*>(maxima + i);
-          rank += (o.x > mine || (o.x == mine && i < tid)) + (o.y > mine || (o.y == mine && i + 1 < tid)) + (o.z > mine || (o.z == mine && i + 2 < tid)) +
-                  (o.w > mine || (o.w == mine && i + 3 < tid));
+      for (int u = 0; u < U; u++) {
+        if (!__any(j0 + u * NT + tid < r.count && !(vmax[u] < least_value))) continue;
+        const uint4 cur = now[u];
+        const long long i0 = r.first + (long long)(j0 + u * NT + tid) * VE;
+        unsigned bits = 0;  // the lane's elements to look at
+        if (j0 + u * NT + tid < r.count) {
+          float e[VE];
+          unpack<T>(cur, e);
+#pragma unroll
+          for (int k = 0; k < VE; k++)
+            if (!(e[k] < least_value)) bits |= 1u << k;
+          if (i0 < r.v0) bits &= ~0u << (int)(r.v0 - i0);
+          if (i0 + VE > r.v1) bits &= (1u << (int)(r.v1 - i0)) - 1u;
         }
-        if (rank == top - 1) cutoff = mine;
-        __syncthreads();
-        least = (u64)cutoff << 32;
-        if (cutoff == 0xffffffffu) least = 0;
-        least_value = least == 0 ? -kInf : value_of(least);
-      }
-      unsigned wait = 0;  // elements of this thread that may have to go into the list
+        while (__any(bits != 0)) {
+          const int k = bits ? __builtin_ctz(bits) : 0;
+          const u64 key = key_of(element<T>(cur, k), i0 + k);
+          const bool enters = bits != 0 && key > least;
+          bits &= bits - 1;
+          const unsigned long long who = __ballot(enters);
+          if (enters) own[held + __popcll(who & ((1ull << lane) - 1))] = key;
+          held += __popcll(who);
+          if (held > kWaveList - 64) {
+            // a higher threshold and what it leaves; where that is not enough, the K largest themselves
+            raise();
+            wave_fence();
+            u64 had[kWaveList / 64];
 #pragma unroll
-      for (int u = 0; u < U; u++)
-        if (in_row(u) && !(vmax[u] < least_value)) wait |= ((1u << VE) - 1u) << (u * VE);
-      for (;;) {
-        if (wait) {
+            for (int q = 0; q < kWaveList / 64; q++) had[q] = 64 * q + lane < held ? own[64 * q + lane] : 0;
+            wave_fence();
+            held = 0;
 #pragma unroll
-          for (int u = 0; u < U; u++) {
-            if (!(wait >> (u * VE) & ((1u << VE) - 1u))) continue;
-            float e[VE];
-            unpack<T>(now[u], e);
-#pragma unroll
-            for (int k = 0; k < VE; k++) {
-              if (!(wait >> (u * VE + k) & 1u)) continue;
-              const long long i = r.first + (long long)(j0 + u * kThreads + tid) * VE + k;
-              const u64 key = key_of(e[k], i);
-              bool done = i < r.v0 || i >= r.v1 || key <= least;
-              if (!done) {
-                const int at = atomicAdd(&held, 1);
-                if (at < kList) {
-                  list[at] = key;
-                  done = true;
-                }
+            for (int q = 0; q < kWaveList / 64; q++) {
+              const unsigned long long stay = __ballot(had[q] > least);
+              if (had[q] > least) own[held + __popcll(stay & ((1ull << lane) - 1))] = had[q];
+              held += __popcll(stay);
+            }
+            if (held > kWaveList / 2) {
+              wave_fence();
+              held = cut_wave(own, held, top, lane);
+              if (held == top) {
+                least = own[top - 1];
+                least_value = value_of(least);
               }
-              if (done) wait &= ~(1u << (u * VE + k));
             }
           }
         }
-        __syncthreads();
-        const int n = held;
-        const bool full = n > kList, last = j0 + U * kThreads >= r.count;
-        __syncthreads();
-        if (n > kList / 2 || (last && n > 0)) {
-          const int left = cut(list, best, full ? kList : n, top, tid);
-          if (tid == 0) held = left;
-          if (left == top) {
-            least = list[top - 1];
-            least_value = value_of(least);
-          }
-          __syncthreads();
-        }
-        if (!full) break;
       }
     }
   }
-  st = join_all(st, red, tid);
+  if constexpr (TOP) {
+    wave_fence();
+    held = cut_wave(own, held, top, lane);
+    if (lane == 0) floors[wave] = held == top ? own[top - 1] : 0;
+    if (tid == 0) count = 0;
+    __syncthreads();
+    // of the wavefronts' lists, what reaches the largest of their last keys, in order
+    u64 floor = floors[0];
+#pragma unroll
+    for (int w = 1; w < NW; w++) floor = floors[w] > floor ? floors[w] : floor;
+    if (lane < held && own[lane] >= floor) list[atomicAdd(&count, 1)] = own[lane];
+    if (tid < top) best[tid] = 0;
+    __syncthreads();
+    const int n = count;
+    if (tid < n) {
+      const u64 mine = list[tid];
+      int rank = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; j++) rank += list[j] > mine ? 1 : 0;
+      if (rank < top) best[rank] = mine;
+    }
+  }
+  st = join_all<NT>(st, red, tid);
   if (splits == 1) {
     if (tid == 0) finish(out, row, st, x, vocab, tokens[row], ignore);
-    if (TOP && tid < top) finish_top(out, row * top + tid, st, list[tid]);
+    if (TOP && tid < top) finish_top(out, row * top + tid, st, best[tid]);
   } else {
     if (tid == 0) {
       float* p = part_stat + (long long)blockIdx.x * 4;
@@ -287,7 +354,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_rows(long long vocab, int t
       p[1] = st.s;
       p[2] = st.t;
     }
-    if (TOP && tid < top) part_key[(long long)blockIdx.x * top + tid] = tid < held ? list[tid] : 0;
+    if (TOP && tid < top) part_key[(long long)blockIdx.x * top + tid] = best[tid];
   }
 }
 
@@ -297,6 +364,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_join(long long vocab, int t
                                                           Out out, int splits, const float* part_stat, const u64* part_key) {
   __shared__ Stat red[4];
   __shared__ u64 list[kList], best[kMaxTop];
+  __shared__ int held;
   const int tid = threadIdx.x;
   const long long row = blockIdx.x;
   Stat st = {-kInf, 0.f, 0.f};
@@ -306,18 +374,35 @@ __global__ void __launch_bounds__(kThreads) logprobs_join(long long vocab, int t
     st.s = p[1];
     st.t = p[2];
   }
-  st = join_all(st, red, tid);
+  st = join_all<kThreads>(st, red, tid);
   if (tid == 0) finish(out, row, st, logits + row * stride, vocab, tokens[row], ignore);
   if (top == 0) return;
   const u64* keys = part_key + row * splits * top;
   const int all = splits * top;
-  int n = 0;
-  for (int at = 0; at < all;) {  // the list holds the largest so far and as many more as there is room for
-    const int take = min(kList - n, all - at);
+  // the last of any share's keys is reached by K of them: what lies below the largest such key is out
+  u64 floor = tid < splits ? keys[tid * top + top - 1] : 0;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const u64 x = __shfl_xor(floor, o);
+    floor = x > floor ? x : floor;
+  }
+  if ((tid & 63) == 0) best[tid >> 6] = floor;
+  if (tid == 0) held = 0;
+  __syncthreads();
+  floor = best[0];
+#pragma unroll
+  for (int w = 1; w < kThreads / 64; w++) floor = best[w] > floor ? best[w] : floor;
+  for (int at = 0; at < all; at += kThreads) {
+    const u64 key = at + tid < all ? keys[at + tid] : 0;
+    if (key != 0 && key >= floor) list[atomicAdd(&held, 1)] = key;
     __syncthreads();
-    for (int i = tid; i < take; i += kThreads) list[n + i] = keys[at + i];
-    at += take;
-    n = cut(list, best, n + take, top, tid);
+    const int n = held;
+    __syncthreads();
+    if (n > kList - kThreads || at + kThreads >= all) {
+      const int left = cut(list, best, n, top, tid);
+      if (tid == 0) held = left;
+      __syncthreads();
+    }
   }
   if (tid < top) finish_top(out, row * top + tid, st, list[tid]);
 }
@@ -410,10 +495,12 @@ const char* check(int dtype, int64_t rows, int64_t vocab, int top) {
   return nullptr;
 }
 
-// Shares of a row: enough workgroups for four on every CU, at least 4096 columns to a share.
+// Few rows: workgroups of 1024 threads.  One has all of a row up to 32768 columns and more (32003 bf16 columns: 11.9 us; shares of
+// 4096 and their join: 11.7 + 4.9 us and the gap between them), beyond two and more shares are joined.
+bool wide(int64_t rows, int64_t vocab) { return rows < 1024 && vocab >= 8192; }
 int splits_of(int64_t rows, int64_t vocab) {
-  if (rows < 1) return 1;
-  int64_t s = 1024 / rows, most = vocab / 4096;
+  if (!wide(rows, vocab)) return 1;
+  int64_t s = 512 / rows, most = vocab / 32768;
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : (s > 64 ? 64 : s));
 }
@@ -424,10 +511,9 @@ int forward(int64_t rows, int64_t vocab, int top, const void* logits, int64_t st
   u64* keys = (u64*)work;
   float* stats = (float*)(keys + (size_t)rows * splits * top);
   const unsigned grid = (unsigned)(rows * splits);
-  if (top)
-    logprobs_rows<T, true><<<grid, kThreads, 0, st>>>(vocab, top, (const T*)logits, stride, tokens, ignore, out, splits, stats, keys);
-  else
-    logprobs_rows<T, false><<<grid, kThreads, 0, st>>>(vocab, top, (const T*)logits, stride, tokens, ignore, out, splits, stats, keys);
+  const bool w = wide(rows, vocab);
+  const auto kernel = top ? (w ? logprobs_rows<T, true, 1024> : logprobs_rows<T, true, 256>) : (w ? logprobs_rows<T, false, 1024> : logprobs_rows<T, false, 256>);
+  kernel<<<grid, w ? 1024 : 256, 0, st>>>(vocab, top, (const T*)logits, stride, tokens, ignore, out, splits, stats, keys);
   if (splits > 1) logprobs_join<T><<<(unsigned)rows, kThreads, 0, st>>>(vocab, top, (const T*)logits, stride, tokens, ignore, out, splits, stats, keys);
   return seq_launched("token log probabilities: launch");
 }

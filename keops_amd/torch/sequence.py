@@ -617,19 +617,24 @@ class TokenLogprobs(NamedTuple):
     top_index: torch.Tensor    # (..., top) int64
 
 
+_logprob_bytes = {}  # workspace by type, rows, vocabulary and alternatives
+
+
 def _logprobs_forward(logits, tokens, top, ignore_index):
     (rows, vocab), device = logits.shape, logits.device
     logprob, entropy, lse = torch.empty((3, rows), dtype=torch.float32, device=device).unbind(0)
     top_logprob = torch.empty((rows, top), dtype=torch.float32, device=device)
     top_index = torch.empty((rows, top), dtype=torch.int64, device=device)
     if rows:
-        lib = binder.lib()
-        dt = _DTYPES[logits.dtype]
-        nbytes = lib.keops_hip_token_logprobs_bytes(dt, rows, vocab, top)
+        lib, index = binder.lib(), device.index
+        key = (_DTYPES[logits.dtype], rows, vocab, top)
+        nbytes = _logprob_bytes.get(key)
+        if nbytes is None:
+            nbytes = _keep(_logprob_bytes, key, lib.keops_hip_token_logprobs_bytes(*key))
         work = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         rc = lib.keops_hip_token_logprobs(
-            dt, rows, vocab, top, _ptr(logits), logits.stride(0), _ptr(tokens), ignore_index, _ptr(logprob), _ptr(entropy), _ptr(lse),
-            _ptr(top_logprob), _ptr(top_index), _ptr(work), nbytes, device.index, _raw_stream(device.index))
+            *key, logits.data_ptr(), logits.stride(0), tokens.data_ptr(), ignore_index, logprob.data_ptr(), entropy.data_ptr(),
+            lse.data_ptr(), top_logprob.data_ptr(), top_index.data_ptr(), _ptr(work), nbytes, index, _raw_stream(index))
         if rc:
             binder.check(rc, "keops_hip_token_logprobs")
     return logprob, entropy, lse, top_logprob, top_index
@@ -679,8 +684,7 @@ def token_logprobs(logits, tokens, *, top=0, ignore_index=-100):
     Returns a :class:`TokenLogprobs`, float32.  Differentiable with respect to the logits through ``logprob``, ``entropy`` and
     ``top_logprob``.
     """
-    what = "token_logprobs"
-    device, _ = _check_data(what, logits=logits)
+    device, _ = _check_data("token_logprobs", logits=logits)
     if not isinstance(tokens, torch.Tensor) or tokens.dtype not in (torch.int64, torch.int32):
         raise TypeError("[KeOps] token_logprobs: tokens must be an int64 or int32 tensor.")
     if tokens.device != device:
@@ -693,12 +697,15 @@ def token_logprobs(logits, tokens, *, top=0, ignore_index=-100):
     if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= min(64, vocab):
         raise ValueError(f"[KeOps] token_logprobs: top must be a whole number from 0 to {min(64, vocab)}, got {top}.")
     shape = tokens.shape
-    flat = logits.reshape(-1, vocab)
+    flat = logits if logits.dim() == 2 else logits.reshape(-1, vocab)
     if flat.stride(1) != 1 and vocab > 1:
         flat = flat.contiguous()
-    tokens = tokens.reshape(-1).long().contiguous()
+    if tokens.dtype != torch.int64 or tokens.dim() != 1 or not tokens.is_contiguous():
+        tokens = tokens.reshape(-1).long().contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
         logprob, entropy, top_logprob, top_index = _TokenLogprobs.apply(flat, tokens, top, int(ignore_index))
     else:
         logprob, entropy, _, top_logprob, top_index = _logprobs_forward(flat, tokens, top, int(ignore_index))
+    if len(shape) == 1:
+        return TokenLogprobs(logprob, entropy, top_logprob, top_index)
     return TokenLogprobs(logprob.view(shape), entropy.view(shape), top_logprob.view(*shape, top), top_index.view(*shape, top))

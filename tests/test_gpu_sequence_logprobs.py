@@ -37,14 +37,15 @@ def _check(x, tokens, top, ignore_index=-100, seed=0):
 
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("rows,vocab,top", [(1, 1, 1), (1, 1, 0), (3, 5, 5), (7, 1000, 3), (2, 2048, 64), (5, 4099, 20), (1, 50021, 5), (600, 777, 2),
-                                            (4, 32003, 64), (1100, 8193, 1), (2, 200000, 20)])
+                                            (4, 32003, 64), (1100, 8193, 1), (2, 200000, 20), (1, 400003, 20),
+                                            (2, 300000, 64), (3, 262145, 0), (700, 8192, 64)])
 def test_values_and_gradients(rows, vocab, top, dtype):
     gen = torch.Generator(device="cuda").manual_seed(rows * vocab)
     x = (torch.randn(rows, vocab, device="cuda", generator=gen) * 3).to(dtype)  # 16 bits: many equal values
     _check(x, torch.randint(0, vocab, (rows,), device="cuda", generator=gen), top)
 
 
-@pytest.mark.parametrize("vocab", [40, 3000, 70001])
+@pytest.mark.parametrize("vocab", [40, 3000, 70001, 280001])
 def test_equal_ordered_and_masked_values(vocab):
     """All equal; increasing (every value is a new maximum); decreasing; few that are not -inf; the type's lowest value; none at all;
     zeros of both signs; the given token -inf."""

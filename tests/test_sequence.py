@@ -142,7 +142,7 @@ def test_step_and_logprob_arguments_that_the_library_refuses():
         return lib.keops_hip_token_logprobs(dtype, rows, vocab, top, logits, vocab, 1 << 12, -100, *[1 << 12] * 5, None, 0, 0, None)
 
     for args, message in (((3, 2, 10, 0), "dtype"), ((0, -1, 10, 0), "rows"), ((0, 2, 0, 0), "vocabulary"), ((0, 2, 1 << 31, 0), "vocabulary"),
-                          ((0, 2, 100, 65), "top"), ((0, 2, 10, 11), "top"), ((0, 2, 100000, 3), "workspace"), ((0, 2, 10, 1, None), "null")):
+                          ((0, 2, 100, 65), "top"), ((0, 2, 10, 11), "top"), ((0, 2, 300000, 3), "workspace"), ((0, 2, 10, 1, None), "null")):
         assert call(*args) != 0, args
         assert message in binder.last_error(), (args, binder.last_error())
     assert call(0, 0, 10, 0) == 0  # no rows: nothing to do
