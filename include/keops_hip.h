@@ -182,7 +182,7 @@ int keops_hip_path_status(void* module, unsigned* taken);
  * neighbours and every row starts at a multiple of 16 bytes.  Launches go to hip_stream, nothing is allocated, nothing waits;
  * workspaces are the caller's, of the size that the *_bytes function names.  dtype: 0 bfloat16, 1 float16, 2 float32.
  */
-#define KEOPS_HIP_MAX_REACH 2048
+#define KEOPS_HIP_MAX_REACH 1024
 
 typedef struct keops_hip_bucket_attention {
   int32_t dtype, batch, heads, kv_heads, dim, causal, buckets, reach;

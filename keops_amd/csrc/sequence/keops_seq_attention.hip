@@ -58,11 +58,11 @@ template <class T> __device__ inline const T* rows_of(const void* p, const int64
 template <class T> __device__ inline T* rows_of(void* p, const int64_t* s, int b, int h) { return (T*)p + (long long)b * s[0] + (long long)h * s[1]; }
 
 // keys of a staged tile: 32 where 64 would not leave the rows in flight, the logits and the sums in 256 registers
-template <int DP> constexpr int key_tile() { return DP <= 64 ? 64 : 32; }
-template <class Tc> constexpr int query_tile() { return sizeof(Tc) == 2 ? 64 : 32; }  // queries of one, where keys are in registers
+template <class Tc, int DP> constexpr int key_tile() { return Vec<Tc>::terms == 1 && DP <= 64 ? 64 : 32; }
+template <class Tc> constexpr int query_tile() { return Vec<Tc>::terms == 1 ? 64 : 32; }  // queries of one, where keys are in registers
 
-// wavefronts a SIMD: wide float32 rows need more than 256 registers
-template <class Tc, int DP> constexpr int waves() { return sizeof(Tc) == 4 && DP > 64 ? 1 : 2; }
+// wavefronts a SIMD: wide split rows need more than 256 registers
+template <class Tc, int DP> constexpr int waves(int widest = 64) { return Vec<Tc>::terms > 1 && DP > widest ? 1 : 2; }
 
 // logits (base 2, less `less`) of a 32 x 32 tile in place: rows are keys kb + 8g + 4 half + t, the lane's column is the query at
 // position pos.  kind: 0 within the reach of the buckets, otherwise the bias is `far`; keys from `lim` on do not count (mask).
@@ -84,6 +84,41 @@ __device__ inline void logits_by_key(f32x16& s, float scale2, const float* table
   }
 }
 
+template <class T> constexpr bool is_f16 = false;
+template <> constexpr bool is_f16<f16> = true;
+
+// Score gradients as float16 operands: products of probabilities and gradients may lie far below or above float16's range, so each
+// lane's column is held times a power of two that puts its largest value so far between 2^13 and 2^15; what has been summed
+// follows when that changes.  (Types with float32's range are left alone.)
+template <class Tc> struct Scaled {
+  template <int ND> __device__ inline void fit(f32x16&, f32x16 (&)[ND]) {}
+  __device__ inline float inverse() const { return 1.f; }
+};
+template <> struct Scaled<f16> {
+  float factor = 1.f, most = 0.f;  // most: the largest value that the factor is good for (0: none seen)
+  template <int ND> __device__ inline void fit(f32x16& s, f32x16 (&acc)[ND]) {
+    float mx = fabsf(s[0]);
+#pragma unroll
+    for (int r = 1; r < 16; r++) mx = fmaxf(mx, fabsf(s[r]));
+    if (__any(mx > most)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      if (mx > most && mx < kInf) {
+        const int e = __builtin_amdgcn_frexp_expf(mx);                  // 2^(e-1) <= mx < 2^e
+        const float to = __builtin_amdgcn_ldexpf(1.f, min(14 - e, 120)), by = most == 0.f ? 0.f : to / factor;
+#pragma unroll
+        for (int k = 0; k < ND; k++)
+#pragma unroll
+          for (int r = 0; r < 16; r++) acc[k][r] *= by;
+        factor = to;
+        most = 32768.f / to;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; r++) s[r] *= factor;
+  }
+  __device__ inline float inverse() const { return 1.f / factor; }
+};
+
 // ---- forward --------------------------------------------------------------------------------------------------------------
 //
 // One pass over the keys with a running reference point and sum.  A workgroup of four wavefronts has 128 queries of one head, a
@@ -96,13 +131,14 @@ __device__ inline void logits_by_key(f32x16& s, float scale2, const float* table
 // relative step there).
 template <class Tin, class Tc, int DP>
 __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_forward(const Args A) {
-  constexpr int KT = key_tile<DP>(), SUB = KT / 32, ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32;
+  constexpr int KT = key_tile<Tc, DP>(), SUB = KT / 32, ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32;
   typedef typename Vec<Tc>::x8 frag;
   extern __shared__ __align__(16) unsigned char smem[];
-  Tc* const ktiles = (Tc*)smem;  // [2][KT][ST]
-  Tc* const vtiles = ktiles + 2 * KT * ST;
+  lds_t<Tc>* const ktiles = (lds_t<Tc>*)smem;  // [2][KT][ST]
+  lds_t<Tc>* const vtiles = ktiles + 2 * KT * ST;
   float* const table = (float*)(vtiles + 2 * KT * ST);
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int group = A.heads / A.kv_heads, M = (int)A.queries, nqb = (M + 127) / 128;
   int unit, block;
   block_of(blockIdx.x, group * nqb, A.batch * A.kv_heads, unit, block);
@@ -145,8 +181,9 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_forward(cons
   __syncthreads();
   const float left = table[0], right = table[2 * A.reach + 2 * kPad];
   for (int t = 0; t < ntiles; t++) {
-    const Tc* kt = ktiles + (t & 1) * KT * ST;
-    const Tc* vt = vtiles + (t & 1) * KT * ST;
+    if constexpr (Vec<Tc>::terms > 1) forget(lane, half, col);
+    const lds_t<Tc>* kt = ktiles + (t & 1) * KT * ST;
+    const lds_t<Tc>* vt = vtiles + (t & 1) * KT * ST;
     if (t + 1 < ntiles) {
       sk.store(ktiles + ((t + 1) & 1) * KT * ST, tid);
       sv.store(vtiles + ((t + 1) & 1) * KT * ST, tid);
@@ -246,11 +283,11 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_forward(cons
 // piece of LDS for the transposing read.  Shares of a long sequence go to different workgroups, which leave their sums for
 // attention_join.
 template <class Tin, class Tc, int DP>
-__global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_rows(const Args A, int splits, float* part) {
+__global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_rows(const Args A, int splits, float* part) {
   constexpr int ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32, VE = 16 / (int)sizeof(Tin), PER_ROW = DP / VE, NV = 32 * PER_ROW / 64;
   extern __shared__ __align__(16) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
-  Tc* const vt = (Tc*)smem + wave * 32 * ST;
+  lds_t<Tc>* const vt = (lds_t<Tc>*)smem + wave * 32 * ST;
   const int group = A.heads / A.kv_heads, M = (int)A.queries, rows = group * M;
   const int unit = blockIdx.x / splits, split = blockIdx.x % splits, b = unit / A.kv_heads, kvh = unit % A.kv_heads;
   const Span sp = span_of(A, b);
@@ -301,15 +338,7 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_rows(const A
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       const int c = lane + 64 * i;
-      Tc* dst = vt + tile_at<Tc, DP>(c / PER_ROW, (c % PER_ROW) * VE);
-      if constexpr (sizeof(Tin) == sizeof(Tc)) {
-        *reinterpret_cast<uint4*>(dst) = vr[i];
-      } else {
-        union { uint4 u; Tin e[VE]; } x;
-        x.u = vr[i];
-#pragma unroll
-        for (int j = 0; j < VE; j++) dst[j] = (Tc)x.e[j];
-      }
+      put_piece<Tin, Tc, DP>(vt, c / PER_ROW, (c % PER_ROW) * VE, vr[i]);
     }
     if (kb + 128 < k1) fetch(kb + 128);
     if (kb - pos_hi >= A.reach || kb + 31 - pos_lo <= -A.reach) {
@@ -451,14 +480,15 @@ template <class Tin> __global__ void __launch_bounds__(512) attention_join(const
 // <dO_i, o_i>, and the row sums of that dS, which are what delta is off by, are added to the delta that the gradient of keys,
 // values and biases uses.
 template <class Tin, class Tc, int DP>
-__global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_grad_q(const Args A) {
-  constexpr int KT = key_tile<DP>(), SUB = KT / 32, ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32;
+__global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_grad_q(const Args A) {
+  constexpr int KT = key_tile<Tc, DP>(), SUB = KT / 32, ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32;
   typedef typename Vec<Tc>::x8 frag;
   extern __shared__ __align__(16) unsigned char smem[];
-  Tc* const ktiles = (Tc*)smem;
-  Tc* const vtiles = ktiles + 2 * KT * ST;
+  lds_t<Tc>* const ktiles = (lds_t<Tc>*)smem;
+  lds_t<Tc>* const vtiles = ktiles + 2 * KT * ST;
   float* const table = (float*)(vtiles + 2 * KT * ST);
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int group = A.heads / A.kv_heads, M = (int)A.queries, nqb = (M + 127) / 128;
   int unit, block;
   block_of(blockIdx.x, group * nqb, A.batch * A.kv_heads, unit, block);
@@ -480,9 +510,11 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_grad_q(const
     for (int i = 0; i < NS; i++) {
       qf[i] = frag_global<Tin, Tc>(q, row < M, 16 * i, half, A.dim);
       gf[i] = frag_global<Tin, Tc>(g, row < M, 16 * i, half, A.dim);
-      const frag of = frag_global<Tin, Tc>(o, row < M, 16 * i, half, A.dim);
+      float gx[8], ox[8];
+      to_float(gf[i], gx);
+      to_float(frag_global<Tin, Tc>(o, row < M, 16 * i, half, A.dim), ox);
 #pragma unroll
-      for (int j = 0; j < 8; j++) delta = fmaf((float)gf[i][j], (float)of[j], delta);
+      for (int j = 0; j < 8; j++) delta = fmaf(gx[j], ox[j], delta);
     }
     delta += __shfl_xor(delta, 32);
   }
@@ -498,6 +530,7 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_grad_q(const
 #pragma unroll
   for (int i = 0; i < ND; i++) acc[i] = zero16();
   float over = 0.f;
+  Scaled<Tc> ds_scale;
 
   Staged<Tin, Tc, KT, DP> sk, sv;
   if (ntiles > 0) {
@@ -513,8 +546,9 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_grad_q(const
   __syncthreads();
   const float left = table[0], right = table[2 * A.reach + 2 * kPad];
   for (int t = 0; t < ntiles; t++) {
-    const Tc* kt = ktiles + (t & 1) * KT * ST;
-    const Tc* vt = vtiles + (t & 1) * KT * ST;
+    if constexpr (Vec<Tc>::terms > 1) forget(lane, half, col);
+    const lds_t<Tc>* kt = ktiles + (t & 1) * KT * ST;
+    const lds_t<Tc>* vt = vtiles + (t & 1) * KT * ST;
     if (t + 1 < ntiles) {
       sk.store(ktiles + ((t + 1) & 1) * KT * ST, tid);
       sv.store(vtiles + ((t + 1) & 1) * KT * ST, tid);
@@ -542,6 +576,7 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_grad_q(const
         s[r] = __builtin_amdgcn_exp2f(s[r]) * p[r];
         over += s[r];
       }
+      ds_scale.fit(s, acc);
 #pragma unroll
       for (int k = 0; k < 2; k++) {
         const frag ds = pack<Tc>(s, k);
@@ -555,6 +590,7 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_grad_q(const
   if (row < M) {
     if (half == 0) A.delta[stat] = delta + over;
     if (A.grad_q) {
+      const float back = A.scale * ds_scale.inverse();
       Tin* o = rows_of<Tin>(A.grad_q, A.grad_q_stride, b, h) + (long long)row * A.grad_q_stride[2];
 #pragma unroll
       for (int i = 0; i < ND; i++)
@@ -562,7 +598,7 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_grad_q(const
         for (int g = 0; g < 4; g++) {
           const int d = 32 * i + 8 * g + 4 * half;
           if (d < A.dim)
-            store4<Tin>(o + d, acc[i][4 * g] * A.scale, acc[i][4 * g + 1] * A.scale, acc[i][4 * g + 2] * A.scale, acc[i][4 * g + 3] * A.scale);
+            store4<Tin>(o + d, acc[i][4 * g] * back, acc[i][4 * g + 1] * back, acc[i][4 * g + 2] * back, acc[i][4 * g + 3] * back);
         }
     }
   }
@@ -576,15 +612,16 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_grad_q(const
 // register's row, so that equal distances meet in a lane) into a table by distance that belongs to the wavefront, and the tables
 // become sums by bucket when the head is done.
 template <class Tin, class Tc, int DP>
-__global__ void __launch_bounds__(256, sizeof(Tc) == 2 && DP <= 64 ? 2 : 1) attention_grad_kv(const Args A, float* part) {
+__global__ void __launch_bounds__(256, (Vec<Tc>::terms == 1 && DP <= 64 ? 2 : 1)) attention_grad_kv(const Args A, float* part) {
   constexpr int QT = query_tile<Tc>(), ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32, SUB = QT / 32;
   extern __shared__ __align__(16) unsigned char smem[];
-  Tc* const tiles = (Tc*)smem;                          // [2][queries, output gradients][QT][ST]
+  lds_t<Tc>* const tiles = (lds_t<Tc>*)smem;            // [2][queries, output gradients][QT][ST]
   float* const stats = (float*)(tiles + 4 * QT * ST);   // [2][lse, delta][QT]
   const int tlen = 2 * A.reach + 1 + 2 * kPad;
   float* const table = stats + 4 * QT;
   float* const sums = table + tlen;                     // [4][tlen]
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5, col = lane & 31;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int group = A.heads / A.kv_heads, M = (int)A.queries, N = (int)A.keys, nkb = (N + 127) / 128;
   int unit, kblock;
   block_of(blockIdx.x, nkb, A.batch * A.kv_heads, unit, kblock);
@@ -608,6 +645,9 @@ __global__ void __launch_bounds__(256, sizeof(Tc) == 2 && DP <= 64 ? 2 : 1) atte
     dk[i] = zero16();
     dv[i] = zero16();
   }
+  // float16 probabilities are held times 2^15 (1 is 32768; 2^-29 is still a normal number), and the score gradients with them
+  constexpr float up = is_f16<Tc> ? 15.f : 0.f, down = is_f16<Tc> ? 1.f / 32768.f : 1.f;
+  Scaled<Tc> ds_scale;
   const float scale2 = A.scale * kLog2e;
   // first query tile that can see a key of this workgroup
   int q_first = 0;
@@ -628,7 +668,7 @@ __global__ void __launch_bounds__(256, sizeof(Tc) == 2 && DP <= 64 ? 2 : 1) atte
       sq.load(Q + (long long)q0 * A.q_stride[2], A.q_stride[2], M - q0, A.dim, tid);
       sg.load(G + (long long)q0 * A.grad_out_stride[2], A.grad_out_stride[2], M - q0, A.dim, tid);
       if (tid < QT) {  // the negatives, as they are added
-        s_lse = q0 + tid < M ? -lse[q0 + tid] : -kInf;
+        s_lse = q0 + tid < M ? up - lse[q0 + tid] : -kInf;
         s_del = q0 + tid < M ? -del[q0 + tid] : 0.f;
       }
     };
@@ -651,8 +691,9 @@ __global__ void __launch_bounds__(256, sizeof(Tc) == 2 && DP <= 64 ? 2 : 1) atte
     __syncthreads();
     const float left = table[0], right = table[tlen - 1];
     for (int t = 0; t < ntiles; t++) {
-      const Tc* qt = tiles + (t & 1) * 2 * QT * ST;
-      const Tc* gt = qt + QT * ST;
+      if constexpr (Vec<Tc>::terms > 1) forget(lane, half, col);
+      const lds_t<Tc>* qt = tiles + (t & 1) * 2 * QT * ST;
+      const lds_t<Tc>* gt = qt + QT * ST;
       const float* st = stats + (t & 1) * 2 * QT;
       if (t + 1 < ntiles) {
         put((t + 1) & 1);
@@ -700,15 +741,6 @@ __global__ void __launch_bounds__(256, sizeof(Tc) == 2 && DP <= 64 ? 2 : 1) atte
           e[r] = __builtin_amdgcn_exp2f(e[r]);
           s[r] = e[r] * p[r];
         }
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-          const typename Vec<Tc>::x8 pf = pack<Tc>(e, k), df = pack<Tc>(s, k);
-#pragma unroll
-          for (int i = 0; i < ND; i++) {
-            dv[i] = mma(frag_cols<Tc, DP>(gt, 32 * u + 16 * k, 32 * i, lane), pf, dv[i]);
-            dk[i] = mma(frag_cols<Tc, DP>(qt, 32 * u + 16 * k, 32 * i, lane), df, dk[i]);
-          }
-        }
         if (want_bias) {
           if (kind != 0) {
             float x = 0.f;
@@ -730,6 +762,16 @@ __global__ void __launch_bounds__(256, sizeof(Tc) == 2 && DP <= 64 ? 2 : 1) atte
             *d += mine;
           }
         }
+        ds_scale.fit(s, dk);
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const typename Vec<Tc>::x8 pf = pack<Tc>(e, k), df = pack<Tc>(s, k);
+#pragma unroll
+          for (int i = 0; i < ND; i++) {
+            dv[i] = mma(frag_cols<Tc, DP>(gt, 32 * u + 16 * k, 32 * i, lane), pf, dv[i]);
+            dk[i] = mma(frag_cols<Tc, DP>(qt, 32 * u + 16 * k, 32 * i, lane), df, dk[i]);
+          }
+        }
       }
       __syncthreads();
     }
@@ -745,7 +787,7 @@ __global__ void __launch_bounds__(256, sizeof(Tc) == 2 && DP <= 64 ? 2 : 1) atte
         sums[wave * tlen + tlen - 1] += far_right;
       }
       __syncthreads();
-      for (int i = tid; i < tlen; i += 256) table[i] = (sums[i] + sums[tlen + i]) + (sums[2 * tlen + i] + sums[3 * tlen + i]);
+      for (int i = tid; i < tlen; i += 256) table[i] = ((sums[i] + sums[tlen + i]) + (sums[2 * tlen + i] + sums[3 * tlen + i])) * down;
       __syncthreads();
       float* out = part + ((long long)(b * nkb + kblock) * A.heads + h) * A.buckets;
       for (int bu = wave; bu < A.buckets; bu += 4) {
@@ -766,6 +808,7 @@ __global__ void __launch_bounds__(256, sizeof(Tc) == 2 && DP <= 64 ? 2 : 1) atte
     __syncthreads();
   }
   if (key < N) {
+    const float back = A.scale * down * ds_scale.inverse();
     Tin* ok = rows_of<Tin>(A.grad_k, A.grad_k_stride, b, kvh) + (long long)key * A.grad_k_stride[2];
     Tin* ov = rows_of<Tin>(A.grad_v, A.grad_v_stride, b, kvh) + (long long)key * A.grad_v_stride[2];
 #pragma unroll
@@ -774,8 +817,8 @@ __global__ void __launch_bounds__(256, sizeof(Tc) == 2 && DP <= 64 ? 2 : 1) atte
       for (int g = 0; g < 4; g++) {
         const int d = 32 * i + 8 * g + 4 * half;
         if (d < A.dim) {
-          store4<Tin>(ok + d, dk[i][4 * g] * A.scale, dk[i][4 * g + 1] * A.scale, dk[i][4 * g + 2] * A.scale, dk[i][4 * g + 3] * A.scale);
-          store4<Tin>(ov + d, dv[i][4 * g], dv[i][4 * g + 1], dv[i][4 * g + 2], dv[i][4 * g + 3]);
+          store4<Tin>(ok + d, dk[i][4 * g] * back, dk[i][4 * g + 1] * back, dk[i][4 * g + 2] * back, dk[i][4 * g + 3] * back);
+          store4<Tin>(ov + d, dv[i][4 * g] * down, dv[i][4 * g + 1] * down, dv[i][4 * g + 2] * down, dv[i][4 * g + 3] * down);
         }
       }
   }
@@ -826,7 +869,7 @@ int splits_of(const Args* a) {
   return (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
 }
 
-template <class Tc, int DP> constexpr size_t tile_bytes(int rows) { return 4 * (size_t)rows * tile_stride<Tc, DP>() * sizeof(Tc); }  // two tensors, two buffers
+template <class Tc, int DP> constexpr size_t tile_bytes(int rows) { return 4 * (size_t)rows * tile_stride<Tc, DP>() * 2; }  // two tensors, two buffers
 int table_entries(const Args* a) { return 2 * a->reach + 1 + 2 * kPad; }
 
 template <class K> int prepare_lds(K kernel, size_t bytes) {
@@ -835,19 +878,17 @@ template <class K> int prepare_lds(K kernel, size_t bytes) {
   return e == hipSuccess ? 0 : keops_seq_fail((int)e, "bucket attention: shared memory");
 }
 
-// fp16 in the gradients: dS is a product of small numbers that would fall below fp16's normal range, so these two passes compute
-// in float32
-template <class Tin, class Tc, class Tg, int DP> struct Passes {
+template <class Tin, class Tc, int DP> struct Passes {
   static int forward(const Args& a, float* work, hipStream_t st) {
     const int group = a.heads / a.kv_heads;
     if (few_rows(&a)) {
       const int rows = group * (int)a.queries, splits = splits_of(&a);
-      const size_t v = 4 * 32 * (size_t)tile_stride<Tc, DP>() * sizeof(Tc), o = 4 * (size_t)rows * (DP + 2) * 4, lds = v > o ? v : o;
+      const size_t v = 4 * 32 * (size_t)tile_stride<Tc, DP>() * 2, o = 4 * (size_t)rows * (DP + 2) * 4, lds = v > o ? v : o;
       if (int e = prepare_lds(attention_rows<Tin, Tc, DP>, lds)) return e;
       attention_rows<Tin, Tc, DP><<<a.batch * a.kv_heads * splits, 256, lds, st>>>(a, splits, work);
       if (splits > 1) attention_join<Tin><<<a.batch * a.kv_heads * rows, 512, 0, st>>>(a, splits, DP, work);
     } else {
-      const size_t lds = tile_bytes<Tc, DP>(key_tile<DP>()) + 4 * (size_t)table_entries(&a);
+      const size_t lds = tile_bytes<Tc, DP>(key_tile<Tc, DP>()) + 4 * (size_t)table_entries(&a);
       if (int e = prepare_lds(attention_forward<Tin, Tc, DP>, lds)) return e;
       const int nqb = (int)((a.queries + 127) / 128);
       attention_forward<Tin, Tc, DP><<<a.batch * a.heads * nqb, 256, lds, st>>>(a);
@@ -856,26 +897,26 @@ template <class Tin, class Tc, class Tg, int DP> struct Passes {
   }
   static int backward(const Args& a, float* work, hipStream_t st) {
     const int nqb = (int)((a.queries + 127) / 128), nkb = (int)((a.keys + 127) / 128);
-    const size_t tb = tile_bytes<Tg, DP>(key_tile<DP>()), te = 4 * (size_t)table_entries(&a);
-    if (int e = prepare_lds(attention_grad_q<Tin, Tg, DP>, tb + te)) return e;
-    attention_grad_q<Tin, Tg, DP><<<a.batch * a.heads * nqb, 256, tb + te, st>>>(a);
+    const size_t tb = tile_bytes<Tc, DP>(key_tile<Tc, DP>()), te = 4 * (size_t)table_entries(&a);
+    if (int e = prepare_lds(attention_grad_q<Tin, Tc, DP>, tb + te)) return e;
+    attention_grad_q<Tin, Tc, DP><<<a.batch * a.heads * nqb, 256, tb + te, st>>>(a);
     if (nkb > 0) {
       float* part = a.grad_bias ? work : nullptr;
-      const size_t lds = tile_bytes<Tg, DP>(query_tile<Tg>()) + 4 * query_tile<Tg>() * sizeof(float) + 5 * te;
-      if (int e = prepare_lds(attention_grad_kv<Tin, Tg, DP>, lds)) return e;
-      attention_grad_kv<Tin, Tg, DP><<<a.batch * a.kv_heads * nkb, 256, lds, st>>>(a, part);
+      const size_t lds = tile_bytes<Tc, DP>(query_tile<Tc>()) + 4 * query_tile<Tc>() * sizeof(float) + 5 * te;
+      if (int e = prepare_lds(attention_grad_kv<Tin, Tc, DP>, lds)) return e;
+      attention_grad_kv<Tin, Tc, DP><<<a.batch * a.kv_heads * nkb, 256, lds, st>>>(a, part);
     }
     if (a.grad_bias) attention_grad_bias<<<a.heads * a.buckets, 256, 0, st>>>(work, a.grad_bias, a.batch * nkb, a.heads * a.buckets);
     return seq_launched("bucket attention: launch of the backward pass");
   }
 };
 
-template <class Tin, class Tc, class Tg> int dispatch(const Args& a, bool backward, float* work, hipStream_t st) {
+template <class Tin, class Tc> int dispatch(const Args& a, bool backward, float* work, hipStream_t st) {
   switch (padded_dim(a.dim)) {
-    case 32: return backward ? Passes<Tin, Tc, Tg, 32>::backward(a, work, st) : Passes<Tin, Tc, Tg, 32>::forward(a, work, st);
-    case 64: return backward ? Passes<Tin, Tc, Tg, 64>::backward(a, work, st) : Passes<Tin, Tc, Tg, 64>::forward(a, work, st);
-    case 96: return backward ? Passes<Tin, Tc, Tg, 96>::backward(a, work, st) : Passes<Tin, Tc, Tg, 96>::forward(a, work, st);
-    default: return backward ? Passes<Tin, Tc, Tg, 128>::backward(a, work, st) : Passes<Tin, Tc, Tg, 128>::forward(a, work, st);
+    case 32: return backward ? Passes<Tin, Tc, 32>::backward(a, work, st) : Passes<Tin, Tc, 32>::forward(a, work, st);
+    case 64: return backward ? Passes<Tin, Tc, 64>::backward(a, work, st) : Passes<Tin, Tc, 64>::forward(a, work, st);
+    case 96: return backward ? Passes<Tin, Tc, 96>::backward(a, work, st) : Passes<Tin, Tc, 96>::forward(a, work, st);
+    default: return backward ? Passes<Tin, Tc, 128>::backward(a, work, st) : Passes<Tin, Tc, 128>::forward(a, work, st);
   }
 }
 
@@ -887,9 +928,9 @@ int enter(const Args* a, bool backward, void* work, size_t work_bytes, int devic
   if (need > work_bytes || (need > 0 && !work)) return keops_seq_fail(-1, "bucket attention: workspace too small");
   SeqDevice on(device);
   hipStream_t st = (hipStream_t)stream;
-  if (a->dtype == 0) return dispatch<bf16, bf16, bf16>(*a, backward, (float*)work, st);
-  if (a->dtype == 1) return dispatch<f16, f16, float>(*a, backward, (float*)work, st);
-  return dispatch<float, float, float>(*a, backward, (float*)work, st);
+  if (a->dtype == 0) return dispatch<bf16, bf16>(*a, backward, (float*)work, st);
+  if (a->dtype == 1) return dispatch<f16, f16>(*a, backward, (float*)work, st);
+  return dispatch<float, Split<3>>(*a, backward, (float*)work, st);
 }
 
 }  // namespace

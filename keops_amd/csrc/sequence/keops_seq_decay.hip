@@ -15,34 +15,19 @@ namespace {
 
 typedef keops_hip_decay_attention Args;
 
-constexpr int C = 64;  // tokens of a chunk
+constexpr int kChunk = 64;  // tokens of a chunk
+template <class Tc> constexpr int chunk() { return Vec<Tc>::terms > 2 ? 32 : kChunk; }  // (tiles of three terms: what LDS holds)
 
-// x as a sum of NT terms of the operand's type; bf16: one term holds 8 bits, two 16, three all 24 of a float32
-template <class T, int NT> struct Terms {
-  typename Vec<T>::x8 t[NT];
-  __device__ inline void set(const float (&x)[8]) {
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      float rest = x[j];
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        const T e = (T)rest;
-        t[n][j] = e;
-        rest -= (float)e;
-      }
-    }
-  }
-};
 // Decayed values as an operand for the state: all of a float32 where the state is a result (or becomes one over the segments
 // behind), 16 bits where it only serves outputs that are rounded to 8.  The state itself is float32; as an operand for those
 // outputs it is rounded once, as the products within the chunk are.
-template <class Tc, bool RESULT> constexpr int update_terms() { return sizeof(Tc) == 2 ? (RESULT ? 3 : 2) : 1; }
+template <class Tc, bool RESULT> constexpr int update_terms() { return RESULT || Vec<Tc>::terms == 3 ? 3 : 2; }
 
-// powers of the decay in LDS: entry kZero + n holds g^n for n = 0..C, zeros before and behind
-constexpr int kZero = 64, kPowers = kZero + C + 8;
+// powers of the decay in LDS: entry kZero + n holds g^n for n = 0..kChunk, zeros before and behind
+constexpr int kZero = 64, kPowers = kZero + kChunk + 8;
 __device__ inline float power(float log_decay, long long n) { return n == 0 ? 1.f : (float)exp((double)log_decay * (double)n); }
 __device__ inline void fill_powers(float* pw, float log_decay, int tid, int nt) {
-  for (int i = tid; i < kPowers; i += nt) pw[i] = i < kZero || i > kZero + C ? 0.f : power(log_decay, i - kZero);
+  for (int i = tid; i < kPowers; i += nt) pw[i] = i < kZero || i > kZero + kChunk ? 0.f : power(log_decay, i - kZero);
 }
 
 template <class T> __device__ inline const T* rows_of(const void* p, const int64_t* s, int b, int h) { return (const T*)p + (long long)b * s[0] + (long long)h * s[1]; }
@@ -56,7 +41,8 @@ __device__ inline int length_of(const Args& A, int b) {
 
 // S = g^n S + sum_j weight_j k_j v_j^T of the chunk in LDS (n tokens); wavefront's 32 columns of v
 template <class Tc, int DK, int DV, int NT>
-__device__ inline void update_state(f32x16 (&S)[DK / 32], const Tc* kt, const Tc* vt, const float* pw, int n, int shift, float scale, int wave, int lane) {
+__device__ inline void update_state(f32x16 (&S)[DK / 32], const lds_t<Tc>* kt, const lds_t<Tc>* vt, const float* pw, int n, int shift, float scale, int wave,
+                                    int lane) {
   const int half = lane >> 5;
   const float all = pw[kZero + n];
 #pragma unroll
@@ -65,19 +51,14 @@ __device__ inline void update_state(f32x16 (&S)[DK / 32], const Tc* kt, const Tc
     for (int r = 0; r < 16; r++) S[i][r] *= all;
   const float* w = pw + kZero + n - 1 + shift - 4 * half;  // weight of token j is w[-j], zero behind the chunk's end
 #pragma unroll
-  for (int s = 0; s < C / 16; s++) {
-    const typename Vec<Tc>::x8 v = frag_cols<Tc, DV>(vt, 16 * s, 32 * wave, lane);
+  for (int s = 0; s < chunk<Tc>() / 16; s++) {
     float x[8];
+    to_float(frag_cols<Tc, DV>(vt, 16 * s, 32 * wave, lane), x);
 #pragma unroll
-    for (int j = 0; j < 8; j++) x[j] = (float)v[j] * (w[-(16 * s + (j & 3) + 2 * (j & 4))] * scale);
-    Terms<Tc, NT> t;
-    t.set(x);
+    for (int j = 0; j < 8; j++) x[j] *= w[-(16 * s + (j & 3) + 2 * (j & 4))] * scale;
+    const SplitX8<NT> v = to_split<NT>(x);
 #pragma unroll
-    for (int i = 0; i < DK / 32; i++) {
-      const typename Vec<Tc>::x8 k = frag_cols<Tc, DK>(kt, 16 * s, 32 * i, lane);
-#pragma unroll
-      for (int m = 0; m < NT; m++) S[i] = mma(k, t.t[m], S[i]);
-    }
+    for (int i = 0; i < DK / 32; i++) S[i] = mma(frag_cols<Tc, DK>(kt, 16 * s, 32 * i, lane), v, S[i]);
   }
 }
 
@@ -86,11 +67,11 @@ __device__ inline void update_state(f32x16 (&S)[DK / 32], const Tc* kt, const Tc
 // Few sequences and heads do not fill the chip, so a long sequence is cut into segments: their own states first (this kernel),
 // then decay_scan carries them on, then decay_outputs starts every segment from its state.
 template <class Tin, class Tc, int DK, int DV, bool REV>
-__global__ void __launch_bounds__(2 * DV, sizeof(Tc) == 2 ? 2 : 1) decay_states(const Args A, int segments, int seg_tokens, float* states) {
-  constexpr int NT = 2 * DV, SK = tile_stride<Tc, DK>(), SV = tile_stride<Tc, DV>();
+__global__ void __launch_bounds__(2 * DV, (Vec<Tc>::terms < 3 ? 2 : 1)) decay_states(const Args A, int segments, int seg_tokens, float* states) {
+  constexpr int C = chunk<Tc>(), NT = 2 * DV, SK = tile_stride<Tc, DK>(), SV = tile_stride<Tc, DV>();
   extern __shared__ __align__(16) unsigned char smem[];
-  Tc* const kt = (Tc*)smem;
-  Tc* const vt = kt + C * SK;
+  lds_t<Tc>* const kt = (lds_t<Tc>*)smem;
+  lds_t<Tc>* const vt = kt + C * SK;
   float* const pw = (float*)(vt + C * SV);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int lane = tid & 63;
@@ -162,15 +143,15 @@ __global__ void __launch_bounds__(256) decay_scan(const Args A, int segments, in
 
 // ---- outputs --------------------------------------------------------------------------------------------------------------------
 
-// Two C tiles (rows: 64 tokens, columns: the wavefront's 32 components) to memory, 16 bytes a lane, through 4096 bytes of LDS that
+// C tiles (rows: 32 tokens each, columns: the wavefront's 32 components) to memory, 16 bytes a lane, through 4096 bytes of LDS that
 // belong to the wavefront (`strip`)
-template <class T, bool REV>
-__device__ inline void store_rows(T* out, long long stride, const f32x16 (&o)[2], void* strip, int t, int t1, int len, int wave, int lane, int dim_v) {
+template <class T, bool REV, int U>
+__device__ inline void store_rows(T* out, long long stride, const f32x16 (&o)[U], void* strip, int t, int t1, int len, int wave, int lane, int dim_v) {
   constexpr int VE = 16 / (int)sizeof(T), PER_ROW = 32 / VE;
   T* const tile = (T*)strip;
   const int half = lane >> 5, col = lane & 31, row0 = lane / PER_ROW, c = 32 * wave + (lane % PER_ROW) * VE;
 #pragma unroll
-  for (int u = 0; u < 2; u++) {
+  for (int u = 0; u < U; u++) {
 #pragma unroll
     for (int r = 0; r < 16; r++) tile[c_row(r, half) * 32 + col] = (T)o[u][r];
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -189,19 +170,19 @@ __device__ inline void store_rows(T* out, long long stride, const f32x16 (&o)[2]
 }
 
 template <class Tc, int DK, int DV> constexpr size_t query_bytes() {
-  constexpr size_t q = (size_t)C * tile_stride<Tc, DK>() * sizeof(Tc), o = 4096 * (DV / 32);
+  constexpr size_t q = (size_t)chunk<Tc>() * tile_stride<Tc, DK>() * 2, o = 4096 * (DV / 32);
   return q > o ? q : o;
 }
 
 // CUT: sequences are cut into segments, whose states are known
 template <class Tin, class Tc, int DK, int DV, bool REV, bool CUT>
-__global__ void __launch_bounds__(2 * DV, sizeof(Tc) == 2 && DK <= DV ? 2 : 1) decay_outputs(const Args A, int segments, int seg_tokens, const float* states) {
-  constexpr int NT = 2 * DV, NW = DV / 32, SK = tile_stride<Tc, DK>(), SV = tile_stride<Tc, DV>(), SP = tile_stride<Tc, C>();
+__global__ void __launch_bounds__(2 * DV, (Vec<Tc>::terms == 1 && DK <= DV ? 2 : 1)) decay_outputs(const Args A, int segments, int seg_tokens, const float* states) {
+  constexpr int C = chunk<Tc>(), U = C / 32, NT = 2 * DV, NW = DV / 32, SK = tile_stride<Tc, DK>(), SV = tile_stride<Tc, DV>(), SP = tile_stride<Tc, C>();
   extern __shared__ __align__(16) unsigned char smem[];
-  Tc* const qt = (Tc*)smem;  // and, once the chunk's queries have been used, the outputs on their way
-  Tc* const kt = (Tc*)(smem + query_bytes<Tc, DK, DV>());
-  Tc* const vt = kt + C * SK;
-  Tc* const pt = vt + C * SV;
+  lds_t<Tc>* const qt = (lds_t<Tc>*)smem;  // and, once the chunk's queries have been used, the outputs on their way
+  lds_t<Tc>* const kt = (lds_t<Tc>*)(smem + query_bytes<Tc, DK, DV>());
+  lds_t<Tc>* const vt = kt + C * SK;
+  lds_t<Tc>* const pt = vt + C * SV;
   float* const pw = (float*)(pt + C * SP);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int lane = tid & 63, half = lane >> 5, col = lane & 31;
@@ -247,10 +228,7 @@ __global__ void __launch_bounds__(2 * DV, sizeof(Tc) == 2 && DK <= DV ? 2 : 1) d
     sv.load(v + at(t0) * vs, vs, t1 - t0, A.dim_v, tid);
   }
   for (int t = t0; t < t1; t += C) {
-    // places in LDS are the same in every chunk: formed anew, they do not stay in registers all along
-    asm volatile("" : "+v"(lane));
-    half = lane >> 5;
-    col = lane & 31;
+    forget(lane, half, col);
     __syncthreads();
     sq.store(qt, tid);
     sk.store(kt, tid);
@@ -261,8 +239,8 @@ __global__ void __launch_bounds__(2 * DV, sizeof(Tc) == 2 && DK <= DV ? 2 : 1) d
       sk.load(k + at(t + C) * ks, ks, t1 - t - C, A.dim, tid);
       sv.load(v + at(t + C) * vs, vs, t1 - t - C, A.dim_v, tid);
     }
-    // decayed products within the chunk: three 32 x 32 tiles (rows tokens j, columns tokens i >= j), shared through LDS
-    for (int tile = wave; tile < 3; tile += NW) {
+    // decayed products within the chunk: 32 x 32 tiles (rows tokens j, columns tokens i >= j), shared through LDS
+    for (int tile = wave; tile < U * (U + 1) / 2; tile += NW) {
       const int i0 = tile == 0 ? 0 : 32, j0 = tile == 2 ? 32 : 0;
       f32x16 a = zero16();
 #pragma unroll
@@ -273,29 +251,31 @@ __global__ void __launch_bounds__(2 * DV, sizeof(Tc) == 2 && DK <= DV ? 2 : 1) d
         float x[4];
 #pragma unroll
         for (int u = 0; u < 4; u++) x[u] = i0 + col >= j0 + 8 * g + 4 * half + u ? a[4 * g + u] * (w[-(8 * g + u)] * A.product_scale) : 0.f;
-        store4<Tc>(pt + tile_at<Tc, C>(i0 + col, j0 + 8 * g + 4 * half), x[0], x[1], x[2], x[3]);
+        put4<Tc, C>(pt, i0 + col, j0 + 8 * g + 4 * half, x[0], x[1], x[2], x[3]);
       }
     }
     // outputs: the state's part first, decayed to each row in float32, then the chunk's own
-    f32x16 o[2] = {zero16(), zero16()};
+    f32x16 o[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) o[u] = zero16();
 #pragma unroll
     for (int i = 0; i < DK / 32; i++)
 #pragma unroll
       for (int s = 0; s < 2; s++) {
         const typename Vec<Tc>::x8 st = pack<Tc>(S[i], s);
 #pragma unroll
-        for (int u = 0; u < 2; u++) o[u] = mma(frag_rows_split<Tc, DK>(qt, 32 * u + col, 32 * i + 16 * s, half), st, o[u]);
+        for (int u = 0; u < U; u++) o[u] = mma(frag_rows_split<Tc, DK>(qt, 32 * u + col, 32 * i + 16 * s, half), st, o[u]);
       }
 #pragma unroll
-    for (int u = 0; u < 2; u++)
+    for (int u = 0; u < U; u++)
 #pragma unroll
       for (int r = 0; r < 16; r++) o[u][r] *= pw[kZero + 32 * u + c_row(r, half) + shift] * A.query_scale;
     __syncthreads();
 #pragma unroll
-    for (int s = 0; s < 4; s++) {
+    for (int s = 0; s < C / 16; s++) {
       const typename Vec<Tc>::x8 vf = frag_cols<Tc, DV>(vt, 16 * s, 32 * wave, lane);
 #pragma unroll
-      for (int u = s / 2; u < 2; u++) o[u] = mma(frag_rows_split<Tc, C>(pt, 32 * u + col, 16 * s, half), vf, o[u]);
+      for (int u = s / 2; u < U; u++) o[u] = mma(frag_rows_split<Tc, C>(pt, 32 * u + col, 16 * s, half), vf, o[u]);
     }
     if (A.out_float32) store_rows<float, REV>((float*)A.out + out0, os, o, strip, t, t1, len, wave, lane, A.dim_v);
     else store_rows<Tin, REV>((Tin*)A.out + out0, os, o, strip, t, t1, len, wave, lane, A.dim_v);
@@ -403,14 +383,14 @@ const char* check(const Args* a) {
 
 // Segments of a sequence: enough workgroups to fill the chip, whole chunks each.
 void segments_of(const Args* a, int& segments, int& seg_tokens) {
-  const int64_t units = (int64_t)a->batch * a->heads, chunks = (a->tokens + C - 1) / C;
+  const int64_t units = (int64_t)a->batch * a->heads, chunks = (a->tokens + kChunk - 1) / kChunk;
   const int64_t fill = a->dim_v > 64 ? 512 : 1024;  // workgroups of four or two wavefronts
   int64_t want = (fill + units - 1) / units;
   if (want > chunks) want = chunks;
   if (want < 1) want = 1;
   const int64_t per = chunks < 1 ? 1 : (chunks + want - 1) / want;
   segments = (int)(chunks < 1 ? 1 : (chunks + per - 1) / per);
-  seg_tokens = (int)(per * C);
+  seg_tokens = (int)(per * kChunk);
 }
 
 template <class K> int prepare_lds(K kernel, size_t bytes) {
@@ -424,8 +404,9 @@ template <class Tin, class Tc, int DK, int DV, bool REV> int run(const Args& a, 
   int segments, seg_tokens;
   segments_of(&a, segments, seg_tokens);
   const int units = a.batch * a.heads;
-  const size_t kv = (size_t)C * (tile_stride<Tc, DK>() + tile_stride<Tc, DV>()) * sizeof(Tc), pw = kPowers * sizeof(float);
-  const size_t all = query_bytes<Tc, DK, DV>() + kv + (size_t)C * tile_stride<Tc, C>() * sizeof(Tc) + pw;
+  constexpr int C = chunk<Tc>();
+  const size_t kv = (size_t)C * (tile_stride<Tc, DK>() + tile_stride<Tc, DV>()) * 2, pw = kPowers * sizeof(float);
+  const size_t all = query_bytes<Tc, DK, DV>() + kv + (size_t)C * tile_stride<Tc, C>() * 2 + pw;
   if (segments > 1 && !a.states_given) {
     if (int e = prepare_lds(decay_states<Tin, Tc, DK, DV, REV>, kv + pw)) return e;
     decay_states<Tin, Tc, DK, DV, REV><<<units * segments, 2 * DV, kv + pw, st>>>(a, segments, seg_tokens, work);
@@ -476,8 +457,8 @@ int keops_hip_decay_attention_run(const keops_hip_decay_attention* a, int device
   SeqDevice on(device);
   hipStream_t st = (hipStream_t)hip_stream;
   if (a->dtype == 0) return dispatch<bf16, bf16>(*a, st);
-  if (a->dtype == 1) return dispatch<f16, float>(*a, st);
-  return dispatch<float, float>(*a, st);
+  if (a->dtype == 1) return dispatch<f16, Split<2>>(*a, st);
+  return dispatch<float, Split<3>>(*a, st);
 }
 
 int keops_hip_decay_attention_step(int dtype, int batch, int heads, int kv_heads, int dim, int dim_v, float scale, const void* q, const int64_t* q_stride,

@@ -120,7 +120,7 @@ class PositionBuckets:
     device.
     """
 
-    MAX_REACH = 2048  # KEOPS_HIP_MAX_REACH
+    MAX_REACH = 1024  # KEOPS_HIP_MAX_REACH
 
     def __init__(self, num_buckets=32, max_distance=128, bidirectional=True):
         count = num_buckets // 2 if bidirectional else num_buckets

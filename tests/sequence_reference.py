@@ -42,7 +42,7 @@ def bucket(rel, num_buckets, max_distance, bidirectional):
 
 def attention(q, k, v, bias, bucket_of, causal, lengths, start, scale, grad=None):
     """Everything about one call, in 64 bits: a dict with out, the gradients, and the bounds ``tol_*`` of what a kernel that rounds
-    probabilities (and, in 16 bits other than fp16, the score gradients) to the inputs' type may be off by."""
+    probabilities and score gradients to the inputs' type may be off by."""
     dtype = q.dtype
     reach = bucket_of.numel() // 2
     b, h, m, d = q.shape
@@ -57,7 +57,7 @@ def attention(q, k, v, bias, bucket_of, causal, lengths, start, scale, grad=None
         for name, x in (("q", q), ("k", k), ("v", v), ("bias", bias)):
             res["grad_" + name], res["tol_grad_" + name] = torch.zeros_like(x), torch.zeros_like(x)
     up = u(dtype)                                          # probabilities as operands
-    us = 0.0 if dtype == torch.float16 else u(dtype)       # score gradients as operands (fp16: computed in float32)
+    us = u(dtype)                                          # score gradients as operands (fp16: scaled, so never subnormal)
     for i in range(b):
         end = lens[i]
         if end == 0 or m == 0:
@@ -138,8 +138,9 @@ def decay(q, k, v, log_decay, state, lengths, scale, grad=None, grad_last=None):
     S0 = zero if state is None else state.double()
     out, last, states = walk(q, k, v, S0, scale)
     oabs, labs, sabs = walk(q.abs(), k.abs(), v.abs(), S0.abs(), abs(scale))
-    # products of a chunk are rounded to a bf16 operand, the state is two bf16 terms (2^-16); fp16 computes in float32
-    op = u(dtype) + 2.0 ** -16 if dtype == torch.bfloat16 else 0.0
+    # products of a chunk and the state are rounded to a bf16 operand, decayed values are two bf16 terms (2^-17, and 2^-16 with what
+    # they add up to); fp16: products and state are two terms, the product of two terms leaves out 2^-18
+    op = {torch.bfloat16: u(dtype) + 2.0 ** -16, torch.float16: 2.0 ** -15, torch.float32: 0.0, torch.float64: 0.0}[dtype]
     # sums over a row of the state (d), over tokens (t) and the decay's powers (a chunk's power is off by 2^-24, t / 64 times)
     e32 = U32 * (2 * t + d + dv + 64)
     res = {"out": out, "state": last, "tol_out": (op + e32) * oabs * 1.01 + rounding(out, dtype) + VANISHED,

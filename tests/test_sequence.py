@@ -12,7 +12,7 @@ from keops_amd.torch import PositionBuckets, bucket_attention, decay_attention, 
 
 
 @pytest.mark.parametrize("num_buckets,max_distance,both", [(32, 128, True), (32, 128, False), (4, 2, True), (2, 2, False), (16, 64, True),
-                                                           (64, 64, False), (64, 2048, True), (17, 100, False)])
+                                                           (64, 64, False), (64, 1024, True), (17, 100, False)])
 def test_buckets_follow_their_definition(num_buckets, max_distance, both):
     b = PositionBuckets(num_buckets, max_distance, both)
     x = torch.arange(-2 * max_distance, 2 * max_distance + 1)
@@ -33,7 +33,7 @@ def test_bucket_tables_of_the_device_code():
     lambda: PositionBuckets(31, 128, True), lambda: PositionBuckets(2, 128, True), lambda: PositionBuckets(1, 128, False),
     lambda: PositionBuckets(32, 8, True), lambda: PositionBuckets(62, 30, True), lambda: PositionBuckets(32, 4096, True), lambda: PositionBuckets.from_map([0, 1]),
     lambda: PositionBuckets.from_map([0]), lambda: PositionBuckets.from_map([0, -1, 0]), lambda: PositionBuckets.from_map([0, 1, 2], 2),
-    lambda: PositionBuckets.from_map([0, 0, 0], 4), lambda: PositionBuckets.from_map([0] * 4099)])
+    lambda: PositionBuckets.from_map([0, 0, 0], 4), lambda: PositionBuckets.from_map([0] * 2051)])
 def test_buckets_that_are_refused(make):
     with pytest.raises(ValueError, match="PositionBuckets"):
         make()
@@ -69,7 +69,7 @@ def _attention_args(**changes):
 @pytest.mark.parametrize("changes,message", [
     (dict(dtype=3), "dtype"), (dict(heads=3), "multiple of kv_heads"), (dict(kv_heads=0), "kv_heads"), (dict(dim=12), "dim"),
     (dict(dim=136), "dim"), (dict(queries=0), "queries"), (dict(keys=-1), "keys"), (dict(keys=1 << 30), "keys"), (dict(reach=0), "reach"),
-    (dict(reach=2049), "reach"), (dict(buckets=184), "buckets"), (dict(start=1 << 30), "query_start"), (dict(q=None), "null"),
+    (dict(reach=1025), "reach"), (dict(buckets=184), "buckets"), (dict(start=1 << 30), "query_start"), (dict(q=None), "null"),
     (dict(v=None), "null"), (dict(batch=1 << 20, heads=1 << 14, kv_heads=1), "workgroups")])
 def test_attention_arguments_that_the_library_refuses(changes, message):
     a = _attention_args(**changes)
