@@ -119,6 +119,13 @@ template <> struct Scaled<f16> {
   __device__ inline float inverse() const { return 1.f / factor; }
 };
 
+// Where few blocks would leave the chip empty, the tiles that a block walks over are shared by several workgroups, whose float32
+// sums are joined: place of one row in the workspace, in records.
+__device__ inline long long share_of(const Args& A, int unit, int splits, int split, int h, int row) {
+  const int group = A.heads / A.kv_heads;
+  return ((long long)(unit * splits + split) * group + h % group) * A.queries + row;
+}
+
 // ---- forward --------------------------------------------------------------------------------------------------------------
 //
 // One pass over the keys with a running reference point and sum.  A workgroup of four wavefronts has 128 queries of one head, a
@@ -130,7 +137,7 @@ template <> struct Scaled<f16> {
 // exceeds it by more than 8 (probabilities up to 2^8 lose nothing: the sum is kept in float32 and 16-bit operands have the same
 // relative step there).
 template <class Tin, class Tc, int DP>
-__global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_forward(const Args A) {
+__global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_forward(const Args A, int splits, float* part) {
   constexpr int KT = key_tile<Tc, DP>(), SUB = KT / 32, ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32;
   typedef typename Vec<Tc>::x8 frag;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -141,7 +148,9 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_forward(cons
   int lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int group = A.heads / A.kv_heads, M = (int)A.queries, nqb = (M + 127) / 128;
   int unit, block;
-  block_of(blockIdx.x, group * nqb, A.batch * A.kv_heads, unit, block);
+  block_of(blockIdx.x, group * nqb * splits, A.batch * A.kv_heads, unit, block);
+  const int split = block % splits;
+  block /= splits;
   const int b = unit / A.kv_heads, kvh = unit % A.kv_heads, h = kvh * group + block % group, qb = nqb - 1 - block / group;
   const Span sp = span_of(A, b);
   fill_table(table, A, h, tid, 256);
@@ -158,7 +167,7 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_forward(cons
   }
   const int kend = A.causal ? min(sp.klen, sp.start + min(qb * 128 + 128, M)) : sp.klen;  // keys that the workgroup sees
   const int wend = A.causal ? min(kend, pos_hi + 1) : kend;                                // and this wavefront
-  const int ntiles = kend > 0 ? (kend + KT - 1) / KT : 0;
+  const int alltiles = kend > 0 ? (kend + KT - 1) / KT : 0, first = alltiles * split / splits, ntiles = alltiles * (split + 1) / splits;
   const int lim = A.causal ? min(sp.klen, pos + 1) : sp.klen;
   const float scale2 = A.scale * kLog2e;
 
@@ -168,29 +177,28 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_forward(cons
   float m = 0.f, l = 0.f, above = -kInf;  // reference point, sum, by what a logit may exceed the reference (-inf: none yet)
 
   Staged<Tin, Tc, KT, DP> sk, sv;
-  if (ntiles > 0) {
-    sk.load(K, ks, sp.klen, A.dim, tid);
-    sv.load(V, vs, sp.klen, A.dim, tid);
-    sk.store(ktiles, tid);
-    sv.store(vtiles, tid);
-    if (ntiles > 1) {
-      sk.load(K + KT * ks, ks, sp.klen - KT, A.dim, tid);
-      sv.load(V + KT * vs, vs, sp.klen - KT, A.dim, tid);
-    }
+  const auto fetch = [&](int t) __attribute__((always_inline)) {
+    sk.load(K + (long long)t * KT * ks, ks, sp.klen - t * KT, A.dim, tid);
+    sv.load(V + (long long)t * KT * vs, vs, sp.klen - t * KT, A.dim, tid);
+  };
+  const auto put = [&](int t) __attribute__((always_inline)) {
+    sk.store(ktiles + (t & 1) * KT * ST, tid);
+    sv.store(vtiles + (t & 1) * KT * ST, tid);
+  };
+  if (first < ntiles) {
+    fetch(first);
+    put(first);
+    if (first + 1 < ntiles) fetch(first + 1);
   }
   __syncthreads();
   const float left = table[0], right = table[2 * A.reach + 2 * kPad];
-  for (int t = 0; t < ntiles; t++) {
+  for (int t = first; t < ntiles; t++) {
     if constexpr (Vec<Tc>::terms > 1) forget(lane, half, col);
     const lds_t<Tc>* kt = ktiles + (t & 1) * KT * ST;
     const lds_t<Tc>* vt = vtiles + (t & 1) * KT * ST;
     if (t + 1 < ntiles) {
-      sk.store(ktiles + ((t + 1) & 1) * KT * ST, tid);
-      sv.store(vtiles + ((t + 1) & 1) * KT * ST, tid);
-      if (t + 2 < ntiles) {
-        sk.load(K + (long long)(t + 2) * KT * ks, ks, sp.klen - (t + 2) * KT, A.dim, tid);
-        sv.load(V + (long long)(t + 2) * KT * vs, vs, sp.klen - (t + 2) * KT, A.dim, tid);
-      }
+      put(t + 1);
+      if (t + 2 < ntiles) fetch(t + 2);
     }
     const int kb = t * KT;
     if (kb < wend) {
@@ -261,6 +269,20 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_forward(cons
     __syncthreads();
   }
   l += __shfl_xor(l, 32);
+  if (splits > 1) {
+    if (row < M) {
+      float* p = part + share_of(A, unit, splits, split, h, row) * (DP + 4);
+      if (half == 0) {
+        p[0] = l == 0.f ? -kInf : m;
+        p[1] = l;
+      }
+#pragma unroll
+      for (int i = 0; i < ND; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) store4<float>(p + 4 + 32 * i + 8 * g + 4 * half, acc[i][4 * g], acc[i][4 * g + 1], acc[i][4 * g + 2], acc[i][4 * g + 3]);
+    }
+    return;
+  }
   if (row < M) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
     Tin* o = rows_of<Tin>(A.out, A.out_stride, b, h) + (long long)row * A.out_stride[2];
@@ -472,6 +494,62 @@ template <class Tin> __global__ void __launch_bounds__(512) attention_join(const
   if (A.lse && tid == 0) A.lse[((long long)b * A.heads + h) * M + qi] = ll == 0.f ? kInf : mm + __builtin_amdgcn_logf(ll);
 }
 
+// The shares of rows, four components of one to a thread.  GRAD: gradients of queries (sums) and what delta is off by, otherwise
+// outputs (sums with reference points).
+template <class Tin, bool GRAD> __global__ void __launch_bounds__(256) attention_join_rows(const Args A, int splits, int dp, const float* part) {
+  const int quads = A.dim / 4, group = A.heads / A.kv_heads;
+  const long long e = (long long)blockIdx.x * 256 + threadIdx.x, r = e / quads;  // row: (unit, head of the group, query)
+  if (r >= (long long)A.batch * A.heads * A.queries) return;
+  const int c = 4 * (int)(e % quads), q = (int)(r % A.queries), g = (int)(r / A.queries % group), unit = (int)(r / A.queries / group);
+  const int b = unit / A.kv_heads, h = unit % A.kv_heads * group + g;
+  const float* p = part + share_of(A, unit, splits, 0, g, q) * (dp + 4);
+  const long long step = (long long)group * A.queries * (dp + 4);
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (GRAD) {
+    float over = 0.f;
+    for (int s = 0; s < splits; s++) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p + s * step + 4 + c);
+      over += p[s * step];
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[j] += x[j];
+    }
+    if (c == 0) A.delta[((long long)b * A.heads + h) * A.queries + q] = p[1] + over;
+    if (A.grad_q) store4<Tin>(rows_of<Tin>(A.grad_q, A.grad_q_stride, b, h) + (long long)q * A.grad_q_stride[2] + c, o[0], o[1], o[2], o[3]);
+  } else {
+    float mm = -kInf, l = 0.f;
+    for (int s = 0; s < splits; s++) mm = fmaxf(mm, p[s * step]);
+    for (int s = 0; s < splits; s++) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(p + s * step + 4 + c);
+      const float m = p[s * step], a = m == mm ? 1.f : __builtin_amdgcn_exp2f(m - mm);
+      l = fmaf(a, p[s * step + 1], l);
+#pragma unroll
+      for (int j = 0; j < 4; j++) o[j] = fmaf(a, x[j], o[j]);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    store4<Tin>(rows_of<Tin>(A.out, A.out_stride, b, h) + (long long)q * A.out_stride[2] + c, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    if (A.lse && c == 0) A.lse[((long long)b * A.heads + h) * A.queries + q] = l == 0.f ? kInf : mm + __builtin_amdgcn_logf(l);
+  }
+}
+
+// the same for gradients of keys and values
+template <class Tin> __global__ void __launch_bounds__(256) attention_join_keys(const Args A, int splits, int dp, const float* part) {
+  const int quads = A.dim / 4;
+  const long long e = (long long)blockIdx.x * 256 + threadIdx.x, r = e / (2 * quads);  // key: (unit, key)
+  if (r >= (long long)A.batch * A.kv_heads * A.keys) return;
+  const int x = (int)(e % (2 * quads)), c = 4 * (x % quads), key = (int)(r % A.keys), unit = (int)(r / A.keys), b = unit / A.kv_heads, h = unit % A.kv_heads;
+  const bool values = x >= quads;
+  const float* p = part + ((long long)unit * splits * A.keys + key) * (2 * dp) + (values ? dp : 0) + c;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < splits; s++) {
+    const f32x4 y = *reinterpret_cast<const f32x4*>(p + (long long)s * A.keys * (2 * dp));
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] += y[j];
+  }
+  Tin* to = values ? rows_of<Tin>(A.grad_v, A.grad_v_stride, b, h) + (long long)key * A.grad_v_stride[2]
+                   : rows_of<Tin>(A.grad_k, A.grad_k_stride, b, h) + (long long)key * A.grad_k_stride[2];
+  store4<Tin>(to + c, o[0], o[1], o[2], o[3]);
+}
+
 // ---- gradient of the queries ------------------------------------------------------------------------------------------------
 //
 // P = exp2(z - lse), dP = dO V^T, dS = P (dP - delta), dq = scale dS K, laid out as in the forward pass.  delta_i = sum_j P_ij dP_ij
@@ -480,7 +558,7 @@ template <class Tin> __global__ void __launch_bounds__(512) attention_join(const
 // <dO_i, o_i>, and the row sums of that dS, which are what delta is off by, are added to the delta that the gradient of keys,
 // values and biases uses.
 template <class Tin, class Tc, int DP>
-__global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_grad_q(const Args A) {
+__global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_grad_q(const Args A, int splits, float* part) {
   constexpr int KT = key_tile<Tc, DP>(), SUB = KT / 32, ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32;
   typedef typename Vec<Tc>::x8 frag;
   extern __shared__ __align__(16) unsigned char smem[];
@@ -491,7 +569,9 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_grad_q(con
   int lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int group = A.heads / A.kv_heads, M = (int)A.queries, nqb = (M + 127) / 128;
   int unit, block;
-  block_of(blockIdx.x, group * nqb, A.batch * A.kv_heads, unit, block);
+  block_of(blockIdx.x, group * nqb * splits, A.batch * A.kv_heads, unit, block);
+  const int split = block % splits;
+  block /= splits;
   const int b = unit / A.kv_heads, kvh = unit % A.kv_heads, h = kvh * group + block % group, qb = nqb - 1 - block / group;
   const Span sp = span_of(A, b);
   fill_table(table, A, h, tid, 256);
@@ -522,7 +602,8 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_grad_q(con
   const float lse = row < M ? A.lse[stat] : kInf;
   const int kend = A.causal ? min(sp.klen, sp.start + min(qb * 128 + 128, M)) : sp.klen;
   const int wend = A.causal ? min(kend, pos_hi + 1) : kend;
-  const int ntiles = kend > 0 ? (kend + KT - 1) / KT : 0, nsub = wend > 0 ? (wend + 31) / 32 : 0;
+  const int alltiles = kend > 0 ? (kend + KT - 1) / KT : 0, first = alltiles * split / splits, ntiles = alltiles * (split + 1) / splits;
+  const int nsub = wend > 0 ? (wend + 31) / 32 : 0;
   const int lim = A.causal ? min(sp.klen, pos + 1) : sp.klen;
   const float scale2 = A.scale * kLog2e;
 
@@ -533,29 +614,28 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_grad_q(con
   Scaled<Tc> ds_scale;
 
   Staged<Tin, Tc, KT, DP> sk, sv;
-  if (ntiles > 0) {
-    sk.load(K, ks, sp.klen, A.dim, tid);
-    sv.load(V, vs, sp.klen, A.dim, tid);
-    sk.store(ktiles, tid);
-    sv.store(vtiles, tid);
-    if (ntiles > 1) {
-      sk.load(K + KT * ks, ks, sp.klen - KT, A.dim, tid);
-      sv.load(V + KT * vs, vs, sp.klen - KT, A.dim, tid);
-    }
+  const auto fetch = [&](int t) __attribute__((always_inline)) {
+    sk.load(K + (long long)t * KT * ks, ks, sp.klen - t * KT, A.dim, tid);
+    sv.load(V + (long long)t * KT * vs, vs, sp.klen - t * KT, A.dim, tid);
+  };
+  const auto put = [&](int t) __attribute__((always_inline)) {
+    sk.store(ktiles + (t & 1) * KT * ST, tid);
+    sv.store(vtiles + (t & 1) * KT * ST, tid);
+  };
+  if (first < ntiles) {
+    fetch(first);
+    put(first);
+    if (first + 1 < ntiles) fetch(first + 1);
   }
   __syncthreads();
   const float left = table[0], right = table[2 * A.reach + 2 * kPad];
-  for (int t = 0; t < ntiles; t++) {
+  for (int t = first; t < ntiles; t++) {
     if constexpr (Vec<Tc>::terms > 1) forget(lane, half, col);
     const lds_t<Tc>* kt = ktiles + (t & 1) * KT * ST;
     const lds_t<Tc>* vt = vtiles + (t & 1) * KT * ST;
     if (t + 1 < ntiles) {
-      sk.store(ktiles + ((t + 1) & 1) * KT * ST, tid);
-      sv.store(vtiles + ((t + 1) & 1) * KT * ST, tid);
-      if (t + 2 < ntiles) {
-        sk.load(K + (long long)(t + 2) * KT * ks, ks, sp.klen - (t + 2) * KT, A.dim, tid);
-        sv.load(V + (long long)(t + 2) * KT * vs, vs, sp.klen - (t + 2) * KT, A.dim, tid);
-      }
+      put(t + 1);
+      if (t + 2 < ntiles) fetch(t + 2);
     }
 #pragma unroll
     for (int u = 0; u < SUB; u++) {
@@ -587,6 +667,22 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_grad_q(con
     __syncthreads();
   }
   over += __shfl_xor(over, 32);
+  if (splits > 1) {
+    if (row < M) {
+      const float back = A.scale * ds_scale.inverse();
+      float* p = part + share_of(A, unit, splits, split, h, row) * (DP + 4);
+      if (half == 0) {
+        p[0] = over;
+        p[1] = delta;
+      }
+#pragma unroll
+      for (int i = 0; i < ND; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+          store4<float>(p + 4 + 32 * i + 8 * g + 4 * half, acc[i][4 * g] * back, acc[i][4 * g + 1] * back, acc[i][4 * g + 2] * back, acc[i][4 * g + 3] * back);
+    }
+    return;
+  }
   if (row < M) {
     if (half == 0) A.delta[stat] = delta + over;
     if (A.grad_q) {
@@ -607,12 +703,12 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_grad_q(con
 // ---- gradients of keys, values and biases -----------------------------------------------------------------------------------
 //
 // A workgroup has 128 keys of one key/value head, a wavefront 32 of them as columns, and walks over the queries of all heads that
-// share them, so nothing is added by two workgroups and no order of additions is left to chance.  Biases: pairs beyond the reach
+// share them (or over a share of them, joined in order), so no order of additions is left to chance.  Biases: pairs beyond the reach
 // add to one sum a side; a 32 x 32 tile within it is summed along its 63 diagonals (each distance is one: lanes are rotated by the
 // register's row, so that equal distances meet in a lane) into a table by distance that belongs to the wavefront, and the tables
 // become sums by bucket when the head is done.
 template <class Tin, class Tc, int DP>
-__global__ void __launch_bounds__(256, (Vec<Tc>::terms == 1 && DP <= 64 ? 2 : 1)) attention_grad_kv(const Args A, float* part) {
+__global__ void __launch_bounds__(256, (Vec<Tc>::terms == 1 && DP <= 64 ? 2 : 1)) attention_grad_kv(const Args A, float* part, int splits, float* share) {
   constexpr int QT = query_tile<Tc>(), ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32, SUB = QT / 32;
   extern __shared__ __align__(16) unsigned char smem[];
   lds_t<Tc>* const tiles = (lds_t<Tc>*)smem;            // [2][queries, output gradients][QT][ST]
@@ -624,7 +720,9 @@ __global__ void __launch_bounds__(256, (Vec<Tc>::terms == 1 && DP <= 64 ? 2 : 1)
   int lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int group = A.heads / A.kv_heads, M = (int)A.queries, N = (int)A.keys, nkb = (N + 127) / 128;
   int unit, kblock;
-  block_of(blockIdx.x, nkb, A.batch * A.kv_heads, unit, kblock);
+  block_of(blockIdx.x, nkb * splits, A.batch * A.kv_heads, unit, kblock);
+  const int split = kblock % splits;
+  kblock /= splits;
   const int b = unit / A.kv_heads, kvh = unit % A.kv_heads;
   const Span sp = span_of(A, b);
   const int kb = kblock * 128 + wave * 32, key = kb + col;
@@ -653,7 +751,9 @@ __global__ void __launch_bounds__(256, (Vec<Tc>::terms == 1 && DP <= 64 ? 2 : 1)
   int q_first = 0;
   if (A.causal) q_first = max(0, kblock * 128 - sp.start) / QT * QT;
   const int q_end = kblock * 128 < sp.klen ? M : 0;
-  const int ntiles = q_end > q_first ? (q_end - q_first + QT - 1) / QT : 0;
+  const int alltiles = q_end > q_first ? (q_end - q_first + QT - 1) / QT : 0;
+  q_first += alltiles * split / splits * QT;  // this workgroup's share of them
+  const int ntiles = alltiles * (split + 1) / splits - alltiles * split / splits;
 
   for (int g = 0; g < group; g++) {
     const int h = kvh * group + g;
@@ -789,23 +889,44 @@ __global__ void __launch_bounds__(256, (Vec<Tc>::terms == 1 && DP <= 64 ? 2 : 1)
       __syncthreads();
       for (int i = tid; i < tlen; i += 256) table[i] = ((sums[i] + sums[tlen + i]) + (sums[2 * tlen + i] + sums[3 * tlen + i])) * down;
       __syncthreads();
-      float* out = part + ((long long)(b * nkb + kblock) * A.heads + h) * A.buckets;
+      if (wave < 2) {  // what lies in the padding belongs to the ends of the reach
+        const int at = wave == 0 ? 0 : tlen - kPad;
+        float x = table[at + lane] + (lane < kPad - 64 ? table[at + 64 + lane] : 0.f);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+        if (lane == 0) sums[wave] = x;
+      }
+      __syncthreads();
+      if (tid == 0) {
+        table[kPad] += sums[0];
+        table[tlen - 1 - kPad] += sums[1];
+      }
+      __syncthreads();
+      float* out = part + ((long long)((b * nkb + kblock) * splits + split) * A.heads + h) * A.buckets;
       for (int bu = wave; bu < A.buckets; bu += 4) {
         float x = 0.f;
-        for (int e = A.bucket_begin[bu] + lane; e < A.bucket_begin[bu + 1]; e += 64) {
-          const int d = A.bucket_order[e];  // 0 .. 2 reach
-          x += table[d + kPad];
-          if (d == 0)
-            for (int i = 0; i < kPad; i++) x += table[i];
-          if (d == 2 * A.reach)
-            for (int i = 0; i < kPad; i++) x += table[d + kPad + 1 + i];
-        }
+        for (int e = A.bucket_begin[bu] + lane; e < A.bucket_begin[bu + 1]; e += 64) x += table[A.bucket_order[e] + kPad];
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
         if (lane == 0) out[bu] = x;
       }
     }
     __syncthreads();
+  }
+  if (splits > 1) {
+    if (key < N) {
+      const float back = A.scale * down * ds_scale.inverse();
+      float* p = share + ((long long)(unit * splits + split) * N + key) * (2 * DP);
+#pragma unroll
+      for (int i = 0; i < ND; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          const int d = 32 * i + 8 * g + 4 * half;
+          store4<float>(p + d, dk[i][4 * g] * back, dk[i][4 * g + 1] * back, dk[i][4 * g + 2] * back, dk[i][4 * g + 3] * back);
+          store4<float>(p + DP + d, dv[i][4 * g] * down, dv[i][4 * g + 1] * down, dv[i][4 * g + 2] * down, dv[i][4 * g + 3] * down);
+        }
+    }
+    return;
   }
   if (key < N) {
     const float back = A.scale * down * ds_scale.inverse();
@@ -878,6 +999,29 @@ template <class K> int prepare_lds(K kernel, size_t bytes) {
   return e == hipSuccess ? 0 : keops_seq_fail((int)e, "bucket attention: shared memory");
 }
 
+// Workgroups of one block, for `blocks` blocks that walk over `rows` rows: two workgroups on every CU, but shares of at least 256
+// rows (128 of float32, whose steps take three times as long), or the join costs more than it gives.
+int shares_of(int64_t blocks, int64_t rows, int dtype) {
+  int64_t s = blocks < 1 ? 1 : 512 / blocks, most = rows / (dtype == 2 ? 128 : 256);
+  s = s < most ? s : most;
+  return (int)(s < 1 ? 1 : (s > 16 ? 16 : s));
+}
+struct Shares {  // of a call's three walks, and where the backward pass's sums lie in its workspace (bytes)
+  int forward, q, k;
+  size_t forward_bytes, q_at, k_at, backward_bytes;
+  explicit Shares(const Args* a) {
+    const int64_t qblocks = (int64_t)a->batch * a->heads * ((a->queries + 127) / 128), nkb = (a->keys + 127) / 128, kblocks = (int64_t)a->batch * a->kv_heads * nkb;
+    const size_t dp = padded_dim(a->dim), rows = (size_t)a->batch * a->heads * a->queries, keys = (size_t)a->batch * a->kv_heads * a->keys;
+    forward = q = shares_of(qblocks, a->keys, a->dtype);
+    k = shares_of(kblocks, a->queries, a->dtype);
+    forward_bytes = forward > 1 ? (size_t)forward * rows * (dp + 4) * sizeof(float) : 0;
+    const size_t bias = a->grad_bias ? (size_t)a->batch * nkb * k * a->heads * a->buckets * sizeof(float) : 0;
+    q_at = (bias + 15) / 16 * 16;
+    k_at = q_at + (q > 1 ? (size_t)q * rows * (dp + 4) * sizeof(float) : 0);
+    backward_bytes = k_at + (k > 1 ? (size_t)k * keys * 2 * dp * sizeof(float) : 0);
+  }
+};
+
 template <class Tin, class Tc, int DP> struct Passes {
   static int forward(const Args& a, float* work, hipStream_t st) {
     const int group = a.heads / a.kv_heads;
@@ -888,25 +1032,32 @@ template <class Tin, class Tc, int DP> struct Passes {
       attention_rows<Tin, Tc, DP><<<a.batch * a.kv_heads * splits, 256, lds, st>>>(a, splits, work);
       if (splits > 1) attention_join<Tin><<<a.batch * a.kv_heads * rows, 512, 0, st>>>(a, splits, DP, work);
     } else {
+      const Shares shares(&a);
       const size_t lds = tile_bytes<Tc, DP>(key_tile<Tc, DP>()) + 4 * (size_t)table_entries(&a);
       if (int e = prepare_lds(attention_forward<Tin, Tc, DP>, lds)) return e;
       const int nqb = (int)((a.queries + 127) / 128);
-      attention_forward<Tin, Tc, DP><<<a.batch * a.heads * nqb, 256, lds, st>>>(a);
+      attention_forward<Tin, Tc, DP><<<a.batch * a.heads * nqb * shares.forward, 256, lds, st>>>(a, shares.forward, work);
+      if (shares.forward > 1) attention_join_rows<Tin, false><<<join_blocks((int64_t)a.batch * a.heads * a.queries * (a.dim / 4)), 256, 0, st>>>(a, shares.forward, DP, work);
     }
     return seq_launched("bucket attention: launch");
   }
+  static unsigned join_blocks(int64_t threads) { return (unsigned)((threads + 255) / 256); }
   static int backward(const Args& a, float* work, hipStream_t st) {
+    const Shares shares(&a);
+    float* const qpart = (float*)((char*)work + shares.q_at), * const kpart = (float*)((char*)work + shares.k_at);
     const int nqb = (int)((a.queries + 127) / 128), nkb = (int)((a.keys + 127) / 128);
     const size_t tb = tile_bytes<Tc, DP>(key_tile<Tc, DP>()), te = 4 * (size_t)table_entries(&a);
     if (int e = prepare_lds(attention_grad_q<Tin, Tc, DP>, tb + te)) return e;
-    attention_grad_q<Tin, Tc, DP><<<a.batch * a.heads * nqb, 256, tb + te, st>>>(a);
+    attention_grad_q<Tin, Tc, DP><<<a.batch * a.heads * nqb * shares.q, 256, tb + te, st>>>(a, shares.q, qpart);
+    if (shares.q > 1) attention_join_rows<Tin, true><<<join_blocks((int64_t)a.batch * a.heads * a.queries * (a.dim / 4)), 256, 0, st>>>(a, shares.q, DP, qpart);
     if (nkb > 0) {
       float* part = a.grad_bias ? work : nullptr;
       const size_t lds = tile_bytes<Tc, DP>(query_tile<Tc>()) + 4 * query_tile<Tc>() * sizeof(float) + 5 * te;
       if (int e = prepare_lds(attention_grad_kv<Tin, Tc, DP>, lds)) return e;
-      attention_grad_kv<Tin, Tc, DP><<<a.batch * a.kv_heads * nkb, 256, lds, st>>>(a, part);
+      attention_grad_kv<Tin, Tc, DP><<<a.batch * a.kv_heads * nkb * shares.k, 256, lds, st>>>(a, part, shares.k, kpart);
+      if (shares.k > 1) attention_join_keys<Tin><<<join_blocks((int64_t)a.batch * a.kv_heads * a.keys * (a.dim / 2)), 256, 0, st>>>(a, shares.k, DP, kpart);
     }
-    if (a.grad_bias) attention_grad_bias<<<a.heads * a.buckets, 256, 0, st>>>(work, a.grad_bias, a.batch * nkb, a.heads * a.buckets);
+    if (a.grad_bias) attention_grad_bias<<<a.heads * a.buckets, 256, 0, st>>>(work, a.grad_bias, a.batch * nkb * shares.k, a.heads * a.buckets);
     return seq_launched("bucket attention: launch of the backward pass");
   }
 };
@@ -938,14 +1089,15 @@ int enter(const Args* a, bool backward, void* work, size_t work_bytes, int devic
 extern "C" {
 
 size_t keops_hip_bucket_attention_forward_bytes(const keops_hip_bucket_attention* a) {
-  if (check(a) || !few_rows(a) || splits_of(a) == 1) return 0;
+  if (check(a)) return 0;
+  if (!few_rows(a)) return Shares(a).forward_bytes;
+  if (splits_of(a) == 1) return 0;
   const size_t rows = (size_t)(a->heads / a->kv_heads) * a->queries;
   return (size_t)a->batch * a->kv_heads * splits_of(a) * rows * (padded_dim(a->dim) + 2) * sizeof(float);
 }
 
 size_t keops_hip_bucket_attention_backward_bytes(const keops_hip_bucket_attention* a) {
-  if (check(a) || !a->grad_bias) return 0;
-  return (size_t)a->batch * ((a->keys + 127) / 128) * a->heads * a->buckets * sizeof(float);
+  return check(a) ? 0 : Shares(a).backward_bytes;
 }
 
 int keops_hip_bucket_attention_forward(const keops_hip_bucket_attention* a, void* work, size_t work_bytes, int device, void* hip_stream) {

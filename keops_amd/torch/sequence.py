@@ -200,7 +200,7 @@ class _BucketPlan:
             lib = binder.lib()
             a.q = a.k = a.v = a.out = a.bias = a.grad_bias = 16
             self.forward_bytes = lib.keops_hip_bucket_attention_forward_bytes(ctypes.byref(a))
-            self.backward_bytes = lib.keops_hip_bucket_attention_backward_bytes(ctypes.byref(a))
+            self.backward_bytes = lib.keops_hip_bucket_attention_backward_bytes(ctypes.byref(a))  # at most this much without grad_bias
 
     def fill(self, q, k, v, bias, key_lengths, query_start):
         a = binder.BucketAttention.from_buffer_copy(self.args)
@@ -254,7 +254,7 @@ class _BucketAttention(torch.autograd.Function):
         a.out, a.lse, a.delta = out.data_ptr(), lse.data_ptr(), delta.data_ptr()
         a.grad_out, a.grad_out_stride[:] = grad.data_ptr(), _stride(grad.shape, grad.stride())
         a.grad_q, a.grad_k, a.grad_v, a.grad_bias = _ptr(dq), dk.data_ptr(), dv.data_ptr(), _ptr(db)
-        plan.run("keops_hip_bucket_attention_backward", a, 0 if db is None else plan.backward_bytes, q.device)
+        plan.run("keops_hip_bucket_attention_backward", a, plan.backward_bytes, q.device)
         return dq, dk, dv, db, None, None, None
 
 

@@ -270,3 +270,15 @@ def test_refusals_on_the_device():
         gx.float().sum().backward()
     empty = bucket_attention(q[:, :, :0].detach().requires_grad_(True), k, v, bias, b)
     assert empty.shape == (2, 4, 0, 16)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("m,n,causal,lengths", [(40, 1500, False, [1500, 700]), (1100, 1100, True, None), (1300, 90, False, [90, 0])])
+def test_walks_shared_by_workgroups(m, n, causal, lengths, dtype):
+    """Few blocks and long walks: shares of the keys (forward, gradient of q) and of the queries (gradients of k and v), joined."""
+    from keops_amd.torch import PositionBuckets
+
+    for d, h, kv in ((64, 2, 1), (96, 1, 1)):
+        q, k, v, bias, go = _make(dtype, 2, h, kv, m, n, d, seed=m + d)
+        lens = None if lengths is None else torch.tensor(lengths, device="cuda")
+        _check(q, k, v, bias, go, PositionBuckets(32, 128, True), causal, lens, 0, True)

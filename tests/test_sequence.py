@@ -85,6 +85,9 @@ def test_attention_workspaces():
     a = _attention_args()
     need = lib.keops_hip_bucket_attention_backward_bytes(ctypes.byref(a))
     assert need == 2 * 1 * 4 * 32 * 4
+    long = _attention_args(queries=3000, keys=3000)  # few blocks: shares of their walks are joined
+    assert lib.keops_hip_bucket_attention_forward_bytes(ctypes.byref(long)) >= 2 * 4 * 3000 * 64 * 4
+    assert lib.keops_hip_bucket_attention_backward_bytes(ctypes.byref(long)) > lib.keops_hip_bucket_attention_forward_bytes(ctypes.byref(long))
     assert lib.keops_hip_bucket_attention_backward(ctypes.byref(a), 1 << 12, need - 1, 0, None) != 0 and "workspace" in binder.last_error()
     assert lib.keops_hip_bucket_attention_forward_bytes(ctypes.byref(a)) == 0
     few = _attention_args(queries=1, keys=100000)
