@@ -630,7 +630,7 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_grad_q(con
   __syncthreads();
   const float left = table[0], right = table[2 * A.reach + 2 * kPad];
   for (int t = first; t < ntiles; t++) {
-    if constexpr (Vec<Tc>::terms > 1) forget(lane, half, col);
+    if constexpr (Vec<Tc>::terms > 1 || DP == 128) forget(lane, half, col);
     const lds_t<Tc>* kt = ktiles + (t & 1) * KT * ST;
     const lds_t<Tc>* vt = vtiles + (t & 1) * KT * ST;
     if (t + 1 < ntiles) {
