@@ -173,8 +173,8 @@ template <class T> __device__ inline frag_t<T> pack(const f32x16& c, int s) {
   return to_frag<T>(x);
 }
 
-// 16 bytes of a row in memory (column `col`) into a tile
-template <class Tin, class T, int DP> __device__ inline void put_piece(lds_t<T>* tile, int row, int col, const uint4& r) {
+// 16 bytes of a row in memory (column `col`) into a tile, times `weight` where the type is split
+template <class Tin, class T, int DP> __device__ inline void put_piece(lds_t<T>* tile, int row, int col, const uint4& r, float weight = 1.f) {
   constexpr int VE = 16 / (int)sizeof(Tin);
   if constexpr (Vec<T>::terms == 1) {
     *reinterpret_cast<uint4*>(tile + tile_at<T, DP>(row, col)) = r;
@@ -183,7 +183,7 @@ template <class Tin, class T, int DP> __device__ inline void put_piece(lds_t<T>*
     x.u = r;
     float rest[VE];
 #pragma unroll
-    for (int j = 0; j < VE; j++) rest[j] = (float)x.e[j];
+    for (int j = 0; j < VE; j++) rest[j] = (float)x.e[j] * weight;
 #pragma unroll
     for (int n = 0; n < Vec<T>::terms; n++) {
       bf16 t[VE] __attribute__((aligned(16)));
@@ -250,6 +250,15 @@ template <class Tin, class Tc, int ROWS, int DP, int NT = 256, bool REVERSE = fa
       const int c = tid + NT * i;
       if (TOTAL % NT != 0 && c >= TOTAL) break;
       put_piece<Tin, Tc, DP>(tile, c / PER_ROW, (c % PER_ROW) * VE, r[i]);
+    }
+  }
+  // row j times weights[-j] * scale
+  __device__ inline void store(lds_t<Tc>* tile, int tid, const float* weights, float scale) const {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int c = tid + NT * i, row = c / PER_ROW;
+      if (TOTAL % NT != 0 && c >= TOTAL) break;
+      put_piece<Tin, Tc, DP>(tile, row, (c % PER_ROW) * VE, r[i], weights[-row] * scale);
     }
   }
 };

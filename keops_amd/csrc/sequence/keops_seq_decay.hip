@@ -66,15 +66,17 @@ __device__ inline void update_state(f32x16 (&S)[DK / 32], const lds_t<Tc>* kt, c
 //
 // Few sequences and heads do not fill the chip, so a long sequence is cut into segments: their own states first (this kernel),
 // then decay_scan carries them on, then decay_outputs starts every segment from its state.
+// A wavefront has 32 columns and half of the rows of a state.  The decayed values, which every row needs, are formed once, on their
+// way to LDS, as three bf16 terms each (all 24 bits: these states are results).
 template <class Tin, class Tc, int DK, int DV, bool REV>
-__global__ void __launch_bounds__(2 * DV, (Vec<Tc>::terms < 3 ? 2 : 1)) decay_states(const Args A, int segments, int seg_tokens, float* states) {
-  constexpr int C = chunk<Tc>(), NT = 2 * DV, SK = tile_stride<Tc, DK>(), SV = tile_stride<Tc, DV>();
+__global__ void __launch_bounds__(4 * DV, 2) decay_states(const Args A, int segments, int seg_tokens, float* states) {
+  constexpr int C = chunk<Tc>(), NT = 4 * DV, SK = tile_stride<Tc, DK>(), SV = tile_stride<Split<3>, DV>(), I = DK / 64;
   extern __shared__ __align__(16) unsigned char smem[];
   lds_t<Tc>* const kt = (lds_t<Tc>*)smem;
-  lds_t<Tc>* const vt = kt + C * SK;
+  bf16* const vt = (bf16*)(kt + C * SK);
   float* const pw = (float*)(vt + C * SV);
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int lane = tid & 63;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), column = 32 * (wave % (DV / 32)), row = DK / 2 * (wave / (DV / 32));
+  int lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int unit = blockIdx.x / segments, seg = blockIdx.x % segments, b = unit / A.heads, h = unit % A.heads;
   const int len = length_of(A, b), t0 = seg * seg_tokens, t1 = min(len, t0 + seg_tokens);
   fill_powers(pw, A.log_decay[h], tid, NT);
@@ -82,35 +84,45 @@ __global__ void __launch_bounds__(2 * DV, (Vec<Tc>::terms < 3 ? 2 : 1)) decay_st
   const Tin* const v = rows_of<Tin>(A.v, A.v_stride, b, h / (A.heads / A.v_heads));
   const long long ks = A.k_stride[2], vs = A.v_stride[2];
   const auto at = [&](int t) -> long long { return REV ? len - 1 - t : t; };  // row of the t-th token of the walk
-  f32x16 S[DK / 32];
+  f32x16 S[I];
 #pragma unroll
-  for (int i = 0; i < DK / 32; i++) S[i] = zero16();
+  for (int i = 0; i < I; i++) S[i] = zero16();
   Staged<Tin, Tc, C, DK, NT, REV> sk;
-  Staged<Tin, Tc, C, DV, NT, REV> sv;
+  Staged<Tin, Split<3>, C, DV, NT, REV> sv;
   if (t0 < t1) {
     sk.load(k + at(t0) * ks, ks, t1 - t0, A.dim, tid);
     sv.load(v + at(t0) * vs, vs, t1 - t0, A.dim_v, tid);
   }
   for (int t = t0; t < t1; t += C) {
-    asm volatile("" : "+v"(lane));  // places in LDS are formed anew in every chunk
+    forget(lane, half, col);
+    const int n = min(C, t1 - t);
     __syncthreads();
     sk.store(kt, tid);
-    sv.store(vt, tid);
+    sv.store(vt, tid, pw + kZero + n - 1 + (REV ? 1 : 0), A.update_scale);  // weight of token j: n - 1 - j powers (one more in reverse)
     __syncthreads();
     if (t + C < t1) {
       sk.load(k + at(t + C) * ks, ks, t1 - t - C, A.dim, tid);
       sv.load(v + at(t + C) * vs, vs, t1 - t - C, A.dim_v, tid);
     }
-    update_state<Tc, DK, DV, update_terms<Tc, true>()>(S, kt, vt, pw, min(C, t1 - t), REV ? 1 : 0, A.update_scale, wave, lane);
-  }
-  const int half = lane >> 5, col = lane & 31;
-  float* out = states + (long long)blockIdx.x * A.dim * A.dim_v;
-  const int c = 32 * wave + col;
+    const float all = pw[kZero + n];
 #pragma unroll
-  for (int i = 0; i < DK / 32; i++)
+    for (int i = 0; i < I; i++)
+#pragma unroll
+      for (int r = 0; r < 16; r++) S[i][r] *= all;
+#pragma unroll
+    for (int s = 0; s < C / 16; s++) {
+      const SplitX8<3> x = frag_cols<Split<3>, DV>(vt, 16 * s, column, lane);
+#pragma unroll
+      for (int i = 0; i < I; i++) S[i] = mma(frag_cols<Tc, DK>(kt, 16 * s, row + 32 * i, lane), x, S[i]);
+    }
+  }
+  float* out = states + (long long)blockIdx.x * A.dim * A.dim_v;
+  const int c = column + col;
+#pragma unroll
+  for (int i = 0; i < I; i++)
 #pragma unroll
     for (int r = 0; r < 16; r++) {
-      const int d = 32 * i + c_row(r, half);
+      const int d = row + 32 * i + c_row(r, half);
       if (d < A.dim && c < A.dim_v) out[(long long)d * A.dim_v + c] = S[i][r];
     }
 }
@@ -408,8 +420,9 @@ template <class Tin, class Tc, int DK, int DV, bool REV> int run(const Args& a, 
   const size_t kv = (size_t)C * (tile_stride<Tc, DK>() + tile_stride<Tc, DV>()) * 2, pw = kPowers * sizeof(float);
   const size_t all = query_bytes<Tc, DK, DV>() + kv + (size_t)C * tile_stride<Tc, C>() * 2 + pw;
   if (segments > 1 && !a.states_given) {
-    if (int e = prepare_lds(decay_states<Tin, Tc, DK, DV, REV>, kv + pw)) return e;
-    decay_states<Tin, Tc, DK, DV, REV><<<units * segments, 2 * DV, kv + pw, st>>>(a, segments, seg_tokens, work);
+    const size_t lds = (size_t)C * (tile_stride<Tc, DK>() + tile_stride<Split<3>, DV>()) * 2 + pw;
+    if (int e = prepare_lds(decay_states<Tin, Tc, DK, DV, REV>, lds)) return e;
+    decay_states<Tin, Tc, DK, DV, REV><<<units * segments, 4 * DV, lds, st>>>(a, segments, seg_tokens, work);
     decay_scan<<<dim3((a.dim * a.dim_v + 255) / 256, units), 256, 0, st>>>(a, segments, seg_tokens, work);
   }
   const auto outputs = segments > 1 ? decay_outputs<Tin, Tc, DK, DV, REV, true> : decay_outputs<Tin, Tc, DK, DV, REV, false>;
