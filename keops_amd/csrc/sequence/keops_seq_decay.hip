@@ -396,7 +396,7 @@ const char* check(const Args* a) {
 // Segments of a sequence: enough workgroups to fill the chip, whole chunks each.
 void segments_of(const Args* a, int& segments, int& seg_tokens) {
   const int64_t units = (int64_t)a->batch * a->heads, chunks = (a->tokens + kChunk - 1) / kChunk;
-  const int64_t fill = a->dim_v > 64 ? 512 : 1024;  // workgroups of four or two wavefronts
+  const int64_t fill = a->dim > 64 || a->dim_v > 64 ? 512 : 1024;  // (the same for exchanged dims: the states are shared)
   int64_t want = (fill + units - 1) / units;
   if (want > chunks) want = chunks;
   if (want < 1) want = 1;
@@ -466,6 +466,7 @@ int keops_hip_decay_attention_run(const keops_hip_decay_attention* a, int device
   if (const char* why = check(a)) return keops_seq_fail(-1, why);
   const size_t need = keops_hip_decay_attention_bytes(a);
   if (need > (size_t)(a->states_bytes > 0 ? a->states_bytes : 0) || (need > 0 && !a->states)) return keops_seq_fail(-1, "decay attention: workspace too small");
+  if (a->states_given && need != (size_t)a->states_bytes) return keops_seq_fail(-1, "decay attention: the states given are not of this call's segments");
   if (a->states_given && need > 0 && a->state_out) return keops_seq_fail(-1, "decay attention: no final state where the states are given");
   SeqDevice on(device);
   hipStream_t st = (hipStream_t)hip_stream;

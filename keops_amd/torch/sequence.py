@@ -360,7 +360,6 @@ class _DecayWalk:
         if not self.empty:
             a.q = a.k = a.v = a.out = a.log_decay = 16  # placeholders for the library's own checks
             self.states = binder.lib().keops_hip_decay_attention_bytes(ctypes.byref(a)) // 4
-            a.states_bytes = 4 * self.states
         self.args = bytes(a)
 
     def __call__(self, q, k, v, log_decay, lengths, state, want_state=False, states=None):
@@ -373,7 +372,7 @@ class _DecayWalk:
             states = torch.empty(self.states, dtype=torch.float32, device=self.device)
         a = binder.DecayAttention.from_buffer_copy(self.args)
         a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-        a.log_decay, a.states = log_decay.data_ptr(), states.data_ptr()
+        a.log_decay, a.states, a.states_bytes = log_decay.data_ptr(), states.data_ptr(), states.nbytes
         if lengths is not None:
             a.lengths = lengths.data_ptr()
         if state is not None:

@@ -65,6 +65,12 @@ def test_long_sequence_in_segments():
     _check(q, k, v, ld, state, torch.tensor([1500, 700], dtype=torch.int32, device="cuda"), go, gs)
 
 
+@pytest.mark.parametrize("dtype,b,h,kv,t,d,dv", [(FP32, 8, 24, 8, 265, 40, 128), (BF16, 1, 4, 4, 2100, 128, 64), (FP16, 2, 3, 1, 1000, 16, 72)])
+def test_training_in_segments_with_different_dims(dtype, b, h, kv, t, d, dv):
+    q, k, v, ld, state, go, gs = _make(dtype, b, h, kv, t, d, dv)
+    _check(q, k, v, ld, state, None, go, gs)
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 def test_dims_and_strides_that_are_copied_first(dtype):
     gen = torch.Generator(device="cuda").manual_seed(4)

@@ -131,6 +131,30 @@ def test_decay_workspaces():
     assert lib.keops_hip_decay_attention_run(ctypes.byref(a), 0, None) != 0 and "final state" in binder.last_error()
 
 
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_decay_states_serve_the_walks_with_exchanged_dims(dtype):
+    """A training step's walks share the states before the segments, so both must cut the sequences alike."""
+    lib = binder.lib()
+    for units in (1, 2, 24, 192, 400):
+        for tokens in (64, 65, 265, 1000, 9000):
+            for d, dv in ((40, 128), (64, 72), (8, 64), (128, 128), (72, 8)):
+                need = []
+                for x, y in ((d, dv), (dv, d)):
+                    a = binder.DecayAttention(dtype=dtype, batch=1, heads=units, q_heads=units, k_heads=units, v_heads=units, dim=x, dim_v=y, tokens=tokens)
+                    for name in ("q", "k", "v", "out", "log_decay"):
+                        setattr(a, name, 16)
+                    need.append(lib.keops_hip_decay_attention_bytes(ctypes.byref(a)))
+                assert need[0] == need[1], (units, tokens, d, dv)
+    a.tokens, a.states, a.states_given = 9000, 16, 1
+    need = lib.keops_hip_decay_attention_bytes(ctypes.byref(a))
+    for size in (need + 16, need - 16):  # states of other segments
+        a.states_bytes = size
+        assert lib.keops_hip_decay_attention_run(ctypes.byref(a), 0, None) != 0
+    assert "too small" in binder.last_error()
+    a.states_bytes = need + 16
+    assert lib.keops_hip_decay_attention_run(ctypes.byref(a), 0, None) != 0 and "segments" in binder.last_error()
+
+
 def test_step_and_logprob_arguments_that_the_library_refuses():
     lib = binder.lib()
     two = (ctypes.c_int64 * 2)(64, 64)
