@@ -237,7 +237,12 @@ typedef struct keops_hip_decay_attention {
      (dim_v, 1), or (1, dim) for their transposes); no final state then. */
   float* states;
   int64_t states_bytes, states_stride[2];
-  int32_t states_given, reserved_states;
+  int32_t states_given;
+  /* joined_heads > 0 (with out_float32): the outputs' sums over neighbouring heads, rounded to the dtype once, as
+     (batch, joined_heads, tokens, dim_v): the gradient of a head that heads / joined_heads heads share */
+  int32_t joined_heads;
+  void* joined;
+  int64_t joined_stride[3];
 } keops_hip_decay_attention;
 
 size_t keops_hip_decay_attention_bytes(const keops_hip_decay_attention* a);

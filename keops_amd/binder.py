@@ -37,7 +37,7 @@ class DecayAttention(ctypes.Structure):
         + [(n, _P) for n in ("q", "k", "v", "out")] + [(n + "_stride", _I64 * 3) for n in ("q", "k", "v", "out")]
         + [(n, _P) for n in ("log_decay", "lengths", "state_in", "state_out")]
         + [("state_in_stride", _I64 * 2), ("state_out_stride", _I64 * 2), ("states", _P), ("states_bytes", _I64),
-           ("states_stride", _I64 * 2), ("states_given", _I32), ("reserved_states", _I32)]
+           ("states_stride", _I64 * 2), ("states_given", _I32), ("joined_heads", _I32), ("joined", _P), ("joined_stride", _I64 * 3)]
     )
 
 

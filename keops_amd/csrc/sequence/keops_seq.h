@@ -298,6 +298,10 @@ template <class T> __device__ inline void store4(T* dst, float a, float b, float
 // Host side: message behind keops_hip_last_error() (defined in keops_hip.cpp); returns `code`.
 int keops_seq_fail(int code, const char* message);
 
+inline bool rows_aligned(const void* p, const int64_t* stride, size_t size) {  // rows that start at multiples of 16 bytes
+  return !p || ((uintptr_t)p % 16 == 0 && stride[0] * size % 16 == 0 && stride[1] * size % 16 == 0 && stride[2] * size % 16 == 0);
+}
+
 struct SeqDevice {  // makes `device` current, and gives the caller's back
   int before = -1, now;
   explicit SeqDevice(int device) : now(device) {

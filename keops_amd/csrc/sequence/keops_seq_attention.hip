@@ -963,6 +963,13 @@ __global__ void __launch_bounds__(256) attention_grad_bias(const float* part, fl
 
 int padded_dim(int dim) { return dim <= 32 ? 32 : (dim <= 64 ? 64 : (dim <= 96 ? 96 : 128)); }
 
+bool aligned(const Args* a) {
+  const size_t size = a->dtype == 2 ? 4 : 2;
+  return rows_aligned(a->q, a->q_stride, size) && rows_aligned(a->k, a->k_stride, size) && rows_aligned(a->v, a->v_stride, size) &&
+         rows_aligned(a->out, a->out_stride, size) && rows_aligned(a->grad_out, a->grad_out_stride, size) &&
+         rows_aligned(a->grad_q, a->grad_q_stride, size) && rows_aligned(a->grad_k, a->grad_k_stride, size) && rows_aligned(a->grad_v, a->grad_v_stride, size);
+}
+
 const char* check(const Args* a) {
   if (!a) return "bucket attention: null arguments";
   if (a->dtype < 0 || a->dtype > 2) return "bucket attention: dtype must be 0 (bfloat16), 1 (float16) or 2 (float32)";
@@ -974,6 +981,7 @@ const char* check(const Args* a) {
   if (a->start < -(1 << 29) || a->start > (1 << 29)) return "bucket attention: query_start out of range";
   for (const int64_t* x : {a->q_stride, a->k_stride, a->v_stride, a->grad_out_stride})
     if (x[2] < 0 || x[2] > kMaxRowStride) return "bucket attention: rows too far apart";
+  if (!aligned(a)) return "bucket attention: a row does not start at a multiple of 16 bytes";
   if (!a->q || !a->out || !a->bias || !a->bucket_of || (a->keys > 0 && (!a->k || !a->v))) return "bucket attention: null data";
   const int64_t units = (int64_t)a->batch * a->heads;
   if (units * ((a->queries + 127) / 128) > 0x7fffffff || units * ((a->keys + 127) / 128) > 0x7fffffff) return "bucket attention: too many workgroups";

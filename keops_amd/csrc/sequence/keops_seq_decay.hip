@@ -310,6 +310,21 @@ __global__ void __launch_bounds__(2 * DV, (Vec<Tc>::terms == 1 && DK <= DV ? 2 :
   }
 }
 
+// sums over the heads that share one, in their order, four components to a thread
+template <class Tin> __global__ void __launch_bounds__(256) decay_join(const Args A) {
+  const int quads = A.dim_v / 4, J = A.joined_heads, group = A.heads / J;
+  const long long total = (long long)A.batch * J * A.tokens * quads;
+  for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long long)gridDim.x * 256) {
+    const int c = 4 * (int)(e % quads);
+    const long long row = e / quads, t = row % A.tokens, unit = row / A.tokens;
+    const int b = (int)(unit / J), j = (int)(unit % J);
+    const float* p = (const float*)A.out + b * A.out_stride[0] + (long long)j * group * A.out_stride[1] + t * A.out_stride[2] + c;
+    f32x4 x = *reinterpret_cast<const f32x4*>(p);
+    for (int h = 1; h < group; h++) x += *reinterpret_cast<const f32x4*>(p + h * A.out_stride[1]);
+    store4<Tin>((Tin*)A.joined + b * A.joined_stride[0] + j * A.joined_stride[1] + t * A.joined_stride[2] + c, x[0], x[1], x[2], x[3]);
+  }
+}
+
 // ---- one token ----------------------------------------------------------------------------------------------------------------
 //
 // One read and one write of the state, float32.  A workgroup has `slice` columns of one head's state, 16 bytes of a row to a
@@ -377,6 +392,13 @@ __global__ void __launch_bounds__(256) decay_step(int heads, int group, int dim,
 
 // ---- host -----------------------------------------------------------------------------------------------------------------------
 
+bool aligned(const Args* a) {
+  const size_t size = a->dtype == 2 ? 4 : 2;
+  return rows_aligned(a->q, a->q_stride, size) && rows_aligned(a->k, a->k_stride, size) && rows_aligned(a->v, a->v_stride, size) &&
+         rows_aligned(a->out, a->out_stride, a->out_float32 ? 4 : size) && (!a->joined_heads || rows_aligned(a->joined, a->joined_stride, size)) &&
+         (uintptr_t)a->state_in % 16 == 0 && (uintptr_t)a->states % 16 == 0;
+}
+
 const char* check(const Args* a) {
   if (!a) return "decay attention: null arguments";
   if (a->dtype < 0 || a->dtype > 2) return "decay attention: dtype must be 0 (bfloat16), 1 (float16) or 2 (float32)";
@@ -386,8 +408,11 @@ const char* check(const Args* a) {
   if (a->dim < ve || a->dim > 128 || a->dim % ve || a->dim_v < ve || a->dim_v > 128 || a->dim_v % ve)
     return "decay attention: dim and dim_v must be multiples of 16 bytes, at most 128";
   if (a->tokens < 0 || a->tokens > (1 << 29)) return "decay attention: tokens out of range";
+  if (a->joined_heads < 0 || (a->joined_heads > 0 && (!a->out_float32 || a->heads % a->joined_heads || (a->tokens > 0 && !a->joined))))
+    return "decay attention: joined outputs need float32 outputs, heads that are a multiple of theirs and a place";
   for (const int64_t* x : {a->q_stride, a->k_stride, a->v_stride, a->out_stride})
     if (x[2] < 0 || x[2] > kMaxRowStride) return "decay attention: rows too far apart";
+  if (!aligned(a)) return "decay attention: a row does not start at a multiple of 16 bytes";
   if (!a->log_decay || (a->tokens > 0 && (!a->q || !a->k || !a->v || !a->out))) return "decay attention: null data";
   if ((int64_t)a->batch * a->heads > 65535) return "decay attention: more than 65535 sequences times heads";
   return nullptr;
@@ -428,6 +453,8 @@ template <class Tin, class Tc, int DK, int DV, bool REV> int run(const Args& a, 
   const auto outputs = segments > 1 ? decay_outputs<Tin, Tc, DK, DV, REV, true> : decay_outputs<Tin, Tc, DK, DV, REV, false>;
   if (int e = prepare_lds(outputs, all)) return e;
   outputs<<<units * segments, 2 * DV, all, st>>>(a, segments, seg_tokens, work);
+  const int64_t joins = a.joined_heads ? ((int64_t)a.batch * a.joined_heads * a.tokens * (a.dim_v / 4) + 255) / 256 : 0;
+  if (joins > 0) decay_join<Tin><<<(unsigned)(joins < 65536 ? joins : 65536), 256, 0, st>>>(a);
   return seq_launched("decay attention: launch");
 }
 

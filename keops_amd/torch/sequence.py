@@ -53,6 +53,8 @@ def _check_whole(what, name, t, shape, device):
         raise ValueError(f"[KeOps] {what}: {name} must be of shape {tuple(shape)}, got {tuple(t.shape)}.")
     if t.dtype is torch.int32 and t.is_contiguous():
         return t
+    if t.dtype is torch.int64:  # (whole numbers that int32 does not hold mean the same as its ends)
+        t = t.clamp(-2**31, 2**31 - 1)
     return t.to(torch.int32).contiguous()
 
 
@@ -91,8 +93,8 @@ def _ptr(t):
 
 
 def _stride(shape, stride):
-    """Strides of batch, head and row as the library takes them (a single row has none)."""
-    return stride[0], stride[1], stride[2] if shape[2] > 1 else 0
+    """Strides of batch, head and row as the library takes them (a single one has none)."""
+    return tuple(s if n > 1 else 0 for n, s in zip(shape[:3], stride)) if 0 not in shape else (0, 0, 0)
 
 
 def _geometry(t):
@@ -174,6 +176,8 @@ class PositionBuckets:
         """The tables on a device: bucket of each distance, distances by bucket, begin of each bucket."""
         device = torch.device(device)
         if device not in self._device:
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("[KeOps] PositionBuckets: first use on a device inside of a graph capture; call .on(device) before it.")
             self._device[device] = tuple(t.to(device) for t in self._host)
         return self._device[device]
 
@@ -301,13 +305,16 @@ def bucket_attention(q, k, v, bias, buckets, *, causal=False, key_lengths=None, 
             2**29.  For one new token against a cache that already holds its key: ``key_lengths - 1``.
         scale: default ``dim ** -0.5``.
 
-    A bias of -6e4 or less (``-inf``, the lowest value of a type) hides its pairs.  A query that sees no key has output 0 and gives no gradient.  Keys that are only hidden by ``causal`` are read with their
-    tile: a value that is not finite there can reach earlier queries.
+    A bias of -6e4 or less (``-inf``, the lowest value of a type) hides its pairs.  A query that sees no key has output 0 and gives
+    no gradient.  Keys that are only hidden by ``causal`` are read with their tile: a value that is not finite there can reach
+    earlier queries.
 
     Returns (batch, heads, queries, dim) in the type and order of dimensions of q.  Differentiable with respect to q, k, v and
     bias.  Up to 32 queries x shared heads use a form of their own that splits the keys over the chip (token generation).
     """
     start = query_start if type(query_start) is int else None
+    if scale is not None and type(scale) is not float:
+        scale = float(scale)  # (a tensor's value, not the tensor, is what a plan is for)
     plan = key = None
     try:
         key = (_geometry(q), _geometry(k), _geometry(v), _geometry(bias), bool(causal), start, scale)
@@ -317,7 +324,7 @@ def bucket_attention(q, k, v, bias, buckets, *, causal=False, key_lengths=None, 
     if plan is None:
         _check_bucket(q, k, v, bias, buckets, query_start)
         d = q.shape[3]
-        number = d ** -0.5 if scale is None else float(scale)
+        number = d ** -0.5 if scale is None else scale
         align = 16 // q.element_size()
         if d % align or not all(map(_strides_fit, (q, k, v))) or bias.dtype != torch.float32 or not bias.is_contiguous():
             out = bucket_attention(_rows(_pad(q, align)), _rows(_pad(k, align)), _rows(_pad(v, align)), bias.float().contiguous(), buckets,
@@ -342,7 +349,7 @@ class _DecayWalk:
     the tensors alone.  q, k, v, out: (shape, strides)."""
 
     def __init__(self, dtype, device, heads, q, k, v, out, out_dtype, *, reverse=False, product_scale=1.0, query_scale=1.0,
-                 update_scale=1.0, transposed=False, given=False):
+                 update_scale=1.0, transposed=False, given=False, joined=None):
         (b, _, t, d), dv = q[0], v[0][3]
         self.device, self.index, self.out_dtype, self.given = device, device.index, out_dtype, given
         self.out, self.state_shape = out, (b, heads, d, dv)
@@ -356,6 +363,9 @@ class _DecayWalk:
         a.state_out_stride[:] = (dv, 1)
         a.states_stride[:] = (1, d) if transposed and given else (dv, 1)
         a.states_given = int(given)
+        self.joined, self.dtype = joined, dtype
+        if joined is not None:
+            a.joined_heads, a.joined_stride[:], a.joined = joined[0][1], _stride(*joined), 16
         self.empty = b == 0 or heads == 0
         if not self.empty:
             a.q = a.k = a.v = a.out = a.log_decay = 16  # placeholders for the library's own checks
@@ -364,10 +374,11 @@ class _DecayWalk:
 
     def __call__(self, q, k, v, log_decay, lengths, state, want_state=False, states=None):
         """Outputs, the final state (or None) and the workspace; ``states``: the workspace of the walk that left the states."""
+        if self.empty:
+            out = torch.empty_strided(*(self.joined or self.out), dtype=self.dtype, device=self.device).zero_()
+            return out, torch.empty(self.state_shape, dtype=torch.float32, device=self.device) if want_state else None, None
         out = torch.empty_strided(*self.out, dtype=self.out_dtype, device=self.device)
         last = torch.empty(self.state_shape, dtype=torch.float32, device=self.device) if want_state else None
-        if self.empty:
-            return out, last, None
         if states is None:
             states = torch.empty(self.states, dtype=torch.float32, device=self.device)
         a = binder.DecayAttention.from_buffer_copy(self.args)
@@ -379,6 +390,9 @@ class _DecayWalk:
             a.state_in = state.data_ptr()
         if want_state:
             a.state_out = last.data_ptr()
+        if self.joined is not None:
+            per_head, out = out, torch.empty_strided(*self.joined, dtype=self.dtype, device=self.device)
+            a.joined = out.data_ptr()
         rc = binder.lib().keops_hip_decay_attention_run(ctypes.byref(a), self.index, _raw_stream(self.index))
         if rc:
             binder.check(rc, "keops_hip_decay_attention_run")
@@ -412,29 +426,21 @@ class _DecayPlan:
         walks = self.gradients.get(grad_strides)
         if walks is None:
             g = (self.out[0], grad_strides)
-            per_head = self.heads == self.shared
 
             def like(name):
-                shape, strides = self.like[name]
-                if per_head:
-                    return (shape, strides), self.dtype
+                if self.heads == self.shared:
+                    return {"out": self.like[name], "out_dtype": self.dtype}
+                shape, _ = self.like[name]
                 shape = torch.Size((shape[0], self.heads, *shape[2:]))
-                return (shape, torch.empty(shape, device="meta").stride()), torch.float32
+                return {"out": (shape, torch.empty(shape, device="meta").stride()), "out_dtype": torch.float32, "joined": self.like[name]}
 
             walks = _keep(self.gradients, grad_strides, (
                 self.walk(g, self.v, self.k, self.like["q"], self.dtype, query_scale=self.scale, transposed=True, given=True),
-                self.walk(self.k, self.q, g, *like("v"), reverse=True, update_scale=self.scale),
-                self.walk(self.v, g, self.q, *like("k"), reverse=True, update_scale=self.scale, transposed=True),
-                self.walk(self.v, g, self.q, *like("k"), reverse=True, update_scale=self.scale, transposed=True, given=True),
+                self.walk(self.k, self.q, g, **like("v"), reverse=True, update_scale=self.scale),
+                self.walk(self.v, g, self.q, **like("k"), reverse=True, update_scale=self.scale, transposed=True),
+                self.walk(self.v, g, self.q, **like("k"), reverse=True, update_scale=self.scale, transposed=True, given=True),
             ))
         return walks
-
-    def join(self, x):
-        """Per head -> per shared head."""
-        if self.heads == self.shared:
-            return x
-        b, h, t, d = x.shape
-        return x.view(b, self.shared, h // self.shared, t, d).sum(2).to(self.dtype)
 
 
 class _DecayAttention(torch.autograd.Function):
@@ -454,7 +460,9 @@ class _DecayAttention(torch.autograd.Function):
         q, k, v, state, log_decay, lengths, states = ctx.saved_tensors
         plan = ctx.plan
         grad = torch.zeros(plan.out[0], dtype=q.dtype, device=q.device) if grad is None else _rows(grad)
-        grad_last = None if grad_last is None else grad_last.contiguous()
+        if grad_last is not None:
+            grad_last = grad_last.contiguous()
+            grad_last = grad_last.clone() if grad_last.data_ptr() & 15 else grad_last
         to_q, to_v, to_k, to_k_given = plan.backward(grad.stride())
         want_q, want_k, want_v, want_state = ctx.needs_input_grad[:4]
         dq = dk = dv = ds = None
@@ -462,13 +470,11 @@ class _DecayAttention(torch.autograd.Function):
             dq = to_q(grad, v, k, log_decay, lengths, state, states=states)[0]
         if want_v or want_state:
             dv, ds, back = to_v(k, q, grad, log_decay, lengths, grad_last, want_state)
-            dv = plan.join(dv)
         if want_k:
             if dv is None:
                 dk = to_k(v, grad, q, log_decay, lengths, grad_last)[0]
             else:
                 dk = to_k_given(v, grad, q, log_decay, lengths, grad_last, states=back)[0]
-            dk = plan.join(dk)
         return dq, dk, dv, ds, None, None, None
 
 
@@ -523,6 +529,8 @@ def decay_attention(q, k, v, log_decay, *, initial_state=None, lengths=None, sca
     which :func:`decay_attention_step` or another call goes on.  Differentiable with respect to q, k, v and initial_state, through
     both results.  Tokens are worked on in chunks of 64; a value that is not finite can reach earlier tokens of its chunk.
     """
+    if scale is not None and type(scale) is not float:
+        scale = float(scale)  # (a tensor's value, not the tensor, is what a plan is for)
     plan = key = None
     try:
         key = (_geometry(q), _geometry(k), _geometry(v), _geometry(initial_state), _geometry(log_decay), scale)
@@ -534,7 +542,7 @@ def decay_attention(q, k, v, log_decay, *, initial_state=None, lengths=None, sca
         if q.shape[2] > 1 << 29:
             raise ValueError("[KeOps] decay_attention: at most 2**29 tokens.")
         d, dv = q.shape[3], v.shape[3]
-        number = d ** -0.5 if scale is None else float(scale)
+        number = d ** -0.5 if scale is None else scale
         align = 16 // q.element_size()
         if (d % align or dv % align or not all(map(_strides_fit, (q, k, v))) or not log_decay.is_contiguous()
                 or (initial_state is not None and not initial_state.is_contiguous())):
@@ -569,6 +577,8 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
 
     Returns (batch, heads, dim_v) in the type of q.  No gradients.
     """
+    if scale is not None and type(scale) is not float:
+        scale = float(scale)  # (a tensor's value, not the tensor, is what a plan is for)
     key = plan = None
     try:
         key = (_geometry(q), _geometry(k), _geometry(v), _geometry(state), _geometry(log_decay), scale)
@@ -589,7 +599,7 @@ def decay_attention_step(q, k, v, log_decay, state, *, scale=None):
         b, h, d = q.shape
         pair = ctypes.c_int64 * 2
         plan = _keep(_step_plans, key, (
-            (_DTYPES[q.dtype], b, h, k.shape[1], d, v.shape[2], d ** -0.5 if scale is None else float(scale)),
+            (_DTYPES[q.dtype], b, h, k.shape[1], d, v.shape[2], d ** -0.5 if scale is None else scale),
             pair(*q.stride()[:2]), pair(*k.stride()[:2]), pair(*v.stride()[:2]), (b, h, v.shape[2]), q.device.index))
     if state.data_ptr() & 15:
         raise ValueError("[KeOps] decay_attention_step: state must be aligned to 16 bytes, it is overwritten.")
@@ -621,7 +631,7 @@ _logprob_bytes = {}  # workspace by type, rows, vocabulary and alternatives
 
 def _logprobs_forward(logits, tokens, top, ignore_index):
     (rows, vocab), device = logits.shape, logits.device
-    logprob, entropy, lse = torch.empty((3, rows), dtype=torch.float32, device=device).unbind(0)
+    logprob, entropy, lse = (torch.empty(rows, dtype=torch.float32, device=device) for _ in range(3))
     top_logprob = torch.empty((rows, top), dtype=torch.float32, device=device)
     top_index = torch.empty((rows, top), dtype=torch.int64, device=device)
     if rows:

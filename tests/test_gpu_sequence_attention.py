@@ -242,6 +242,24 @@ def test_graph_streams_and_repeats():
         assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_single_ones_may_have_any_stride_and_numbers_any_type():
+    from keops_amd.torch import PositionBuckets, bucket_attention
+
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    base = torch.randn(150 * 64 + 8, device="cuda", generator=gen).bfloat16()
+    q, k = base.as_strided((1, 1, 70, 64), (5, 3, 64, 1)), base.as_strided((1, 1, 150, 64), (9, 1, 64, 1), 8)
+    bias, b = torch.randn(1, 32, device="cuda", generator=gen), PositionBuckets()
+    dense = bucket_attention(q.contiguous(), k.contiguous(), k.contiguous(), bias, b, scale=0.5)
+    far = torch.tensor([2 ** 40], device="cuda")  # more keys than there are
+    assert torch.equal(bucket_attention(q, k, k, bias, b, scale=0.5, key_lengths=far), dense)
+    scale = torch.tensor(1.0)
+    bucket_attention(q, k, k, bias, b, scale=scale)
+    scale.mul_(0.5)
+    assert torch.equal(bucket_attention(q, k, k, bias, b, scale=scale), dense)
+    # no keys, cut out of others
+    assert (bucket_attention(q, k[:, :, 3:3, :], k[:, :, 3:3, :], bias, b) == 0).all()
+
+
 def test_refusals_on_the_device():
     from keops_amd.torch import PositionBuckets, bucket_attention
 

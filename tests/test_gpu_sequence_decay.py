@@ -83,6 +83,43 @@ def test_dims_and_strides_that_are_copied_first(dtype):
     _check(r(2, 2, 70, 16), k, v, ld, None, None, r(2, 2, 70, 1).expand(2, 2, 70, 16), None)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+def test_gradients_of_shared_heads(dtype):
+    """Joined over the heads that share, in the order of dimensions of the inputs; lengths behind which the gradient is zeros."""
+    q, k, v, ld, state, go, gs = _make(dtype, 2, 12, 3, 150, 24, 40)
+    lengths = torch.tensor([150, 31], device="cuda")
+    _check(q, k, v, ld, state, lengths, go, gs)
+    from keops_amd.torch import decay_attention
+
+    k.requires_grad_(True)
+    v.requires_grad_(True)
+    dk, dv = torch.autograd.grad(decay_attention(q, k, v, ld, lengths=lengths)[0], (k, v), go)
+    assert dk.stride() == k.stride() and dv.stride() == v.stride()
+    assert (dk[1, :, 31:] == 0).all() and (dv[1, :, 31:] == 0).all()
+    # no heads: nothing to add up
+    none = decay_attention(q[:, :0], k, v, ld[:0])[0]
+    dk, dv = torch.autograd.grad(none, (k, v), go[:, :0])
+    assert (dk == 0).all() and (dv == 0).all()
+
+
+def test_single_ones_may_have_any_stride_and_numbers_any_type():
+    from keops_amd.torch import decay_attention, decay_attention_step
+
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    base = torch.randn(2 * 130 * 64 + 6, device="cuda", generator=gen).bfloat16()
+    q = base.as_strided((1, 1, 130, 64), (5, 3, 64, 1))
+    k = base.as_strided((1, 1, 130, 64), (130 * 64 + 1, 7, 64, 1), 8)
+    ld, state, go = torch.tensor([-0.2], device="cuda"), torch.zeros(1, 1, 64, 64, device="cuda"), torch.randn(1, 1, 130, 64, device="cuda").bfloat16()
+    _check(q, k, k, ld, None, torch.tensor([2 ** 40], device="cuda"), go, None)
+    # a scale that is a tensor counts by its value at the call
+    scale = torch.tensor(0.5)
+    a = decay_attention(q, k, k, ld, scale=scale)[0]
+    step = decay_attention_step(q[:, :, 0], k[:, :, 0], k[:, :, 0], ld, state.clone(), scale=scale)
+    scale.mul_(2)
+    assert torch.equal(decay_attention(q, k, k, ld, scale=scale)[0], 2 * a)
+    assert torch.equal(decay_attention_step(q[:, :, 0], k[:, :, 0], k[:, :, 0], ld, state.clone(), scale=scale), 2 * step)
+
+
 def test_decays_at_the_ends_of_their_range():
     q, k, v, _, state, go, gs = _make(FP32, 1, 3, 1, 140, 32, 32)
     ld = torch.tensor([0.0, -math.inf, -60.0], device="cuda")

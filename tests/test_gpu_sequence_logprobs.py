@@ -176,6 +176,20 @@ def test_graph_and_streams():
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_results_may_be_changed_in_place():
+    """The log probabilities are a tensor of their own: masking them in place leaves what the gradient needs."""
+    from keops_amd.torch import token_logprobs
+
+    x = torch.randn(6, 500, device="cuda", requires_grad=True)
+    tokens, mask = torch.arange(6, device="cuda"), torch.tensor([1.0, 0, 1, 1, 0, 1], device="cuda")
+    r = token_logprobs(x, tokens)
+    (want,) = torch.autograd.grad((r.logprob * mask).sum(), x)
+    r = token_logprobs(x, tokens)
+    r.logprob.mul_(mask)
+    (got,) = torch.autograd.grad(r.logprob.sum(), x)
+    assert torch.equal(got, want)
+
+
 def test_refusals_on_the_device():
     from keops_amd.torch import token_logprobs
 

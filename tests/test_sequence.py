@@ -155,6 +155,42 @@ def test_decay_states_serve_the_walks_with_exchanged_dims(dtype):
     assert lib.keops_hip_decay_attention_run(ctypes.byref(a), 0, None) != 0 and "segments" in binder.last_error()
 
 
+def test_rows_off_16_bytes_are_refused_by_the_library():
+    lib = binder.lib()
+    for changes in (dict(q=24), dict(k_stride=(0, 0, 4)), dict(out_stride=(4, 0, 64)), dict(v_stride=(0, 2, 64)), dict(state_in=8)):
+        a = binder.DecayAttention(dtype=0, batch=1, heads=1, q_heads=1, k_heads=1, v_heads=1, dim=64, dim_v=64, tokens=8)
+        b = binder.BucketAttention(dtype=0, batch=1, heads=1, kv_heads=1, dim=64, queries=8, keys=8, buckets=3, reach=1)
+        for x in (a, b):
+            for name in ("q", "k", "v", "out", "log_decay", "bias", "bucket_of"):
+                if hasattr(x, name):
+                    setattr(x, name, 16)
+            for name, value in changes.items():
+                if not hasattr(x, name):
+                    break
+                setattr(x, name, (ctypes.c_int64 * 3)(*value) if isinstance(value, tuple) else value)
+            else:
+                rc = (lib.keops_hip_decay_attention_run(ctypes.byref(a), 0, None) if x is a
+                      else lib.keops_hip_bucket_attention_forward(ctypes.byref(b), None, 0, 0, None))
+                assert rc != 0 and "16 bytes" in binder.last_error(), changes
+
+
+@pytest.mark.parametrize("changes", [dict(joined_heads=2), dict(joined_heads=3, out_float32=1, joined=16), dict(joined_heads=2, out_float32=1),
+                                     dict(joined_heads=-1, out_float32=1, joined=16)])
+def test_joined_outputs_that_the_library_refuses(changes):
+    a = binder.DecayAttention(dtype=0, batch=1, heads=4, q_heads=4, k_heads=4, v_heads=4, dim=64, dim_v=64, tokens=8)
+    for name in ("q", "k", "v", "out", "log_decay"):
+        setattr(a, name, 16)
+    for name, value in changes.items():
+        setattr(a, name, value)
+    assert binder.lib().keops_hip_decay_attention_run(ctypes.byref(a), 0, None) != 0 and "joined" in binder.last_error()
+
+
+def test_first_use_of_buckets_inside_of_a_capture_is_refused(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="capture"):
+        PositionBuckets().on("cuda:0")
+
+
 def test_step_and_logprob_arguments_that_the_library_refuses():
     lib = binder.lib()
     two = (ctypes.c_int64 * 2)(64, 64)
