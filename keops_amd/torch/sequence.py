@@ -199,15 +199,15 @@ class _BucketPlan:
         a.grad_k_stride[:], a.grad_v_stride[:] = _stride(k.shape, self.k_strides), _stride(v.shape, self.v_strides)
         a.bucket_of, a.bucket_order, a.bucket_begin = (t.data_ptr() for t in self.tables)
         self.empty = q.numel() == 0
-        self.args = bytes(a)
+        self.args, self.grad_args = bytes(a), {}
         if not self.empty:  # the library's own checks, on placeholders that it does not follow
             lib = binder.lib()
             a.q = a.k = a.v = a.out = a.bias = a.grad_bias = 16
             self.forward_bytes = lib.keops_hip_bucket_attention_forward_bytes(ctypes.byref(a))
             self.backward_bytes = lib.keops_hip_bucket_attention_backward_bytes(ctypes.byref(a))  # at most this much without grad_bias
 
-    def fill(self, q, k, v, bias, key_lengths, query_start):
-        a = binder.BucketAttention.from_buffer_copy(self.args)
+    def fill(self, args, q, k, v, bias, key_lengths, query_start):
+        a = binder.BucketAttention.from_buffer_copy(args)
         a.q, a.k, a.v, a.bias = q.data_ptr(), k.data_ptr(), v.data_ptr(), bias.data_ptr()
         if key_lengths is not None:
             a.key_lengths = key_lengths.data_ptr()
@@ -225,12 +225,35 @@ class _BucketPlan:
         out = torch.empty_strided(q.shape, self.out_strides, dtype=q.dtype, device=q.device)
         lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
         if not self.empty:
-            a = self.fill(q, k, v, bias, key_lengths, query_start)
+            a = self.fill(self.args, q, k, v, bias, key_lengths, query_start)
             a.out = out.data_ptr()
             if want_lse:
                 a.lse = lse.data_ptr()
             self.run("keops_hip_bucket_attention_forward", a, self.forward_bytes, q.device)
         return out, lse
+
+    def backward(self, grad, q, k, v, bias, out, lse, key_lengths, query_start, want_q, want_bias):
+        args = self.grad_args.get(grad.stride())
+        if args is None or grad.data_ptr() & 15:  # the first of these strides, or such that are copied
+            grad = _rows(grad)
+            a = binder.BucketAttention.from_buffer_copy(self.args)
+            a.grad_out_stride[:] = _stride(grad.shape, grad.stride())
+            args = _keep(self.grad_args, grad.stride(), bytes(a))
+        new, delta = torch.empty_strided, torch.empty_like(lse)
+        dk = new(k.shape, self.k_strides, dtype=k.dtype, device=k.device)
+        dv = new(v.shape, self.v_strides, dtype=v.dtype, device=v.device)
+        a = self.fill(args, q, k, v, bias, key_lengths, query_start)
+        a.out, a.lse, a.delta, a.grad_out = out.data_ptr(), lse.data_ptr(), delta.data_ptr(), grad.data_ptr()
+        a.grad_k, a.grad_v = dk.data_ptr(), dv.data_ptr()
+        dq = db = None
+        if want_q:
+            dq = new(q.shape, self.out_strides, dtype=q.dtype, device=q.device)
+            a.grad_q = dq.data_ptr()
+        if want_bias:
+            db = torch.empty_like(bias)
+            a.grad_bias = db.data_ptr()
+        self.run("keops_hip_bucket_attention_backward", a, self.backward_bytes, q.device)
+        return dq, dk, dv, db
 
 
 class _BucketAttention(torch.autograd.Function):
@@ -248,18 +271,8 @@ class _BucketAttention(torch.autograd.Function):
         plan = ctx.plan
         if plan.empty:
             return (*(torch.zeros_like(t) for t in (q, k, v, bias)), None, None, None)
-        grad = _rows(grad)
-        new = lambda t, strides: torch.empty_strided(t.shape, strides, dtype=t.dtype, device=t.device)
-        dq = new(q, plan.out_strides) if ctx.needs_input_grad[0] else None
-        dk, dv = new(k, plan.k_strides), new(v, plan.v_strides)
-        db = torch.empty_like(bias) if ctx.needs_input_grad[3] else None
-        delta = torch.empty_like(lse)
-        a = plan.fill(q, k, v, bias, key_lengths, query_start)
-        a.out, a.lse, a.delta = out.data_ptr(), lse.data_ptr(), delta.data_ptr()
-        a.grad_out, a.grad_out_stride[:] = grad.data_ptr(), _stride(grad.shape, grad.stride())
-        a.grad_q, a.grad_k, a.grad_v, a.grad_bias = _ptr(dq), dk.data_ptr(), dv.data_ptr(), _ptr(db)
-        plan.run("keops_hip_bucket_attention_backward", a, plan.backward_bytes, q.device)
-        return dq, dk, dv, db, None, None, None
+        return (*plan.backward(grad, q, k, v, bias, out, lse, key_lengths, query_start, ctx.needs_input_grad[0], ctx.needs_input_grad[3]),
+                None, None, None)
 
 
 def _check_bucket(q, k, v, bias, buckets, query_start):
@@ -379,11 +392,13 @@ class _DecayWalk:
             return out, torch.empty(self.state_shape, dtype=torch.float32, device=self.device) if want_state else None, None
         out = torch.empty_strided(*self.out, dtype=self.out_dtype, device=self.device)
         last = torch.empty(self.state_shape, dtype=torch.float32, device=self.device) if want_state else None
-        if states is None:
-            states = torch.empty(self.states, dtype=torch.float32, device=self.device)
         a = binder.DecayAttention.from_buffer_copy(self.args)
+        if self.states:  # (sequences in one piece have none)
+            if states is None:
+                states = torch.empty(self.states, dtype=torch.float32, device=self.device)
+            a.states, a.states_bytes = states.data_ptr(), states.nbytes
         a.q, a.k, a.v, a.out = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
-        a.log_decay, a.states, a.states_bytes = log_decay.data_ptr(), states.data_ptr(), states.nbytes
+        a.log_decay = log_decay.data_ptr()
         if lengths is not None:
             a.lengths = lengths.data_ptr()
         if state is not None:
@@ -459,7 +474,10 @@ class _DecayAttention(torch.autograd.Function):
         # that of k from those of v's
         q, k, v, state, log_decay, lengths, states = ctx.saved_tensors
         plan = ctx.plan
-        grad = torch.zeros(plan.out[0], dtype=q.dtype, device=q.device) if grad is None else _rows(grad)
+        if grad is None:
+            grad = torch.zeros(plan.out[0], dtype=q.dtype, device=q.device)
+        elif grad.stride() not in plan.gradients or grad.data_ptr() & 15:  # (strides that have walks fit)
+            grad = _rows(grad)
         if grad_last is not None:
             grad_last = grad_last.contiguous()
             grad_last = grad_last.clone() if grad_last.data_ptr() & 15 else grad_last
