@@ -30,18 +30,12 @@ __device__ inline Span span_of(const Args& A, int b) {
   return s;
 }
 
-// Unit (sequence and key/value head) and block within it of a workgroup.  With a multiple of 8 units, the blocks of one unit run
-// on one XCD (workgroups go to the XCDs in turn), which then holds the unit's keys and values in its own L2.  Block by block over
-// the units: with a causal bound the blocks are of very different length, and the longest of all units come first.
-__device__ inline void block_of(unsigned w, int per_unit, int units, int& unit, int& block) {
-  if (units % 8 == 0) {
-    const int xcd = w & 7, slot = w >> 3, here = units / 8;
-    unit = (slot % here) * 8 + xcd;
-    block = slot / here;
-  } else {
-    unit = w % units;
-    block = w / units;
-  }
+// Unit (sequence and key/value head) and block within it of a workgroup: block by block over the units.  With a causal bound the
+// blocks are of very different length, and the longest of all units come first.  Workgroups go to the 8 XCDs in turn, so with a
+// multiple of 8 units the blocks of one unit share an XCD's L2.
+__device__ inline void block_of(unsigned w, int units, int& unit, int& block) {
+  unit = w % units;
+  block = w / units;
 }
 
 // A bias of -6e4 or less (the lowest fp16 is -65504; masks of the type's lowest value) hides its pairs as -inf does: next to such a
@@ -57,9 +51,12 @@ __device__ inline void fill_table(float* table, const Args& A, int h, int tid, i
 template <class T> __device__ inline const T* rows_of(const void* p, const int64_t* s, int b, int h) { return (const T*)p + (long long)b * s[0] + (long long)h * s[1]; }
 template <class T> __device__ inline T* rows_of(void* p, const int64_t* s, int b, int h) { return (T*)p + (long long)b * s[0] + (long long)h * s[1]; }
 
-// keys of a staged tile: 32 where 64 would not leave the rows in flight, the logits and the sums in 256 registers
+// Keys of a staged tile: 32 where 64 would not leave the rows in flight, the logits and the sums in 256 registers.  Forward pass of
+// 4x8x4096^2, 64 components, 64 keys 115 us and 32 keys 127; 8x16384^2, 128 components, 64 keys 1557 us (spilled) and 32 keys 672.
 template <class Tc, int DP> constexpr int key_tile() { return Vec<Tc>::terms == 1 && DP <= 64 ? 64 : 32; }
-template <class Tc> constexpr int query_tile() { return Vec<Tc>::terms == 1 ? 64 : 32; }  // queries of one, where keys are in registers
+// Queries of one, where keys are in registers: 64 against 32, training of 4x8x4096^2, 64 components, 436 and 448 us; 2x8x4096^2, 128
+// components, 568 and 582.  (Four tiles of 64 rows of three terms would not fit in LDS.)
+template <class Tc> constexpr int query_tile() { return Vec<Tc>::terms == 1 ? 64 : 32; }
 
 // wavefronts a SIMD: wide split rows need more than 256 registers
 template <class Tc, int DP> constexpr int waves(int widest = 64) { return Vec<Tc>::terms > 1 && DP > widest ? 1 : 2; }
@@ -136,6 +133,12 @@ __device__ inline long long share_of(const Args& A, int unit, int splits, int sp
 // Logits are formed less the reference point, so probabilities are exp2 of one multiply-add.  The point moves only when a logit
 // exceeds it by more than 8 (probabilities up to 2^8 lose nothing: the sum is kept in float32 and 16-bit operands have the same
 // relative step there).
+//
+// 8 x 16384^2 causal bf16, 128 components: 672 us, 0.82 Pflop/s (a library product of 8192^3 reaches 1.21); 4x8 x 4096^2, 64
+// components: 115 us, 0.60.  Of a SIMD's cycles the matrix instructions take 35 % (64 components: 28 %), vector instructions 39 %
+// (51 %): they hardly run side by side, and the exponential, which costs as much as four multiplications, is the largest part.
+// Not kept: products a tile ahead of the softmax (162 us for 111), three wavefronts a SIMD (127 with tiles of 32 keys, which two
+// take as well), places in LDS formed anew in each turn (752 us for 655), priorities around the products (680 for 673).
 template <class Tin, class Tc, int DP>
 __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_forward(const Args A, int splits, float* part) {
   constexpr int KT = key_tile<Tc, DP>(), SUB = KT / 32, ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32;
@@ -148,7 +151,7 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_forward(cons
   int lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int group = A.heads / A.kv_heads, M = (int)A.queries, nqb = (M + 127) / 128;
   int unit, block;
-  block_of(blockIdx.x, group * nqb * splits, A.batch * A.kv_heads, unit, block);
+  block_of(blockIdx.x, A.batch * A.kv_heads, unit, block);
   const int split = block % splits;
   block /= splits;
   const int b = unit / A.kv_heads, kvh = unit % A.kv_heads, h = kvh * group + block % group, qb = nqb - 1 - block / group;
@@ -303,7 +306,8 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_forward(cons
 // At most 32 rows (queries times heads that share a key/value head): every wavefront holds them all and takes every fourth tile
 // of 32 keys of its share of the sequence; keys go from memory to registers as operands, values through the wavefront's own
 // piece of LDS for the transposing read.  Shares of a long sequence go to different workgroups, which leave their sums for
-// attention_join.
+// attention_join.  Bound by reading keys and values: 131072 keys of 2 heads, 128 components, 134 MB in 26 us (5.2 TB/s; a copy
+// reaches 4.9), 32x8 ragged caches of up to 2048 keys, 64 components, 22 us with the join.
 template <class Tin, class Tc, int DP>
 __global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_rows(const Args A, int splits, float* part) {
   constexpr int ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32, VE = 16 / (int)sizeof(Tin), PER_ROW = DP / VE, NV = 32 * PER_ROW / 64;
@@ -557,6 +561,8 @@ template <class Tin> __global__ void __launch_bounds__(256) attention_join_keys(
 // exact sum is zero: a delta off by 2^-9 of itself would be most of a far bucket's gradient in a long row.  So dS is formed with
 // <dO_i, o_i>, and the row sums of that dS, which are what delta is off by, are added to the delta that the gradient of keys,
 // values and biases uses.
+//
+// 4x8 x 4096^2 causal bf16, 64 components: 150 us, 0.69 Pflop/s; of a SIMD's cycles matrix instructions take 30 %, vector ones 41 %.
 template <class Tin, class Tc, int DP>
 __global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_grad_q(const Args A, int splits, float* part) {
   constexpr int KT = key_tile<Tc, DP>(), SUB = KT / 32, ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32;
@@ -569,7 +575,7 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_grad_q(con
   int lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int group = A.heads / A.kv_heads, M = (int)A.queries, nqb = (M + 127) / 128;
   int unit, block;
-  block_of(blockIdx.x, group * nqb * splits, A.batch * A.kv_heads, unit, block);
+  block_of(blockIdx.x, A.batch * A.kv_heads, unit, block);
   const int split = block % splits;
   block /= splits;
   const int b = unit / A.kv_heads, kvh = unit % A.kv_heads, h = kvh * group + block % group, qb = nqb - 1 - block / group;
@@ -707,6 +713,9 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_grad_q(con
 // add to one sum a side; a 32 x 32 tile within it is summed along its 63 diagonals (each distance is one: lanes are rotated by the
 // register's row, so that equal distances meet in a lane) into a table by distance that belongs to the wavefront, and the tables
 // become sums by bucket when the head is done.
+//
+// 4x8 x 4096^2 causal bf16, 64 components: 222 us, 0.62 Pflop/s; of a SIMD's cycles matrix instructions take 27 %, vector ones 39 %;
+// the sums and operands of 32 keys take 247 registers, which allows two wavefronts a SIMD.
 template <class Tin, class Tc, int DP>
 __global__ void __launch_bounds__(256, (Vec<Tc>::terms == 1 && DP <= 64 ? 2 : 1)) attention_grad_kv(const Args A, float* part, int splits, float* share) {
   constexpr int QT = query_tile<Tc>(), ST = tile_stride<Tc, DP>(), NS = DP / 16, ND = DP / 32, SUB = QT / 32;
@@ -720,7 +729,7 @@ __global__ void __launch_bounds__(256, (Vec<Tc>::terms == 1 && DP <= 64 ? 2 : 1)
   int lane = tid & 63, half = lane >> 5, col = lane & 31;
   const int group = A.heads / A.kv_heads, M = (int)A.queries, N = (int)A.keys, nkb = (N + 127) / 128;
   int unit, kblock;
-  block_of(blockIdx.x, nkb * splits, A.batch * A.kv_heads, unit, kblock);
+  block_of(blockIdx.x, A.batch * A.kv_heads, unit, kblock);
   const int split = kblock % splits;
   kblock /= splits;
   const int b = unit / A.kv_heads, kvh = unit % A.kv_heads;
@@ -988,12 +997,16 @@ const char* check(const Args* a) {
   return nullptr;
 }
 
+// The form for few rows against the one for tiles of 128 queries, us: 32x8 caches of up to 2048 keys 25 and 37, 131072 keys for 16
+// rows 37 and 344, 4 queries of 32 heads that share 4, 8192 keys, 18 and 53.
 bool few_rows(const Args* a) { return a->queries * (a->heads / a->kv_heads) <= 32; }
 
-// Shares of the keys for few rows: enough workgroups for four on every CU, at least 256 keys to a share (two tiles a wavefront).
+// Shares of the keys for few rows: two workgroups on every CU, at least 256 keys to a share (two tiles a wavefront).  32x8 caches of
+// up to 2048 keys with 256, 512, 1024 and 2048 workgroups: 24.5, 22.4, 24.9 and 31.6 us.  32 rows of 4 sequences, 8192 keys, 64
+// components, with at least 128, 256 and 512 keys: 24.0, 18.3, 17.1 us; of one sequence, 128 components: 18.1, 19.0, 22.5.
 int splits_of(const Args* a) {
   const int64_t units = (int64_t)a->batch * a->kv_heads;
-  int64_t s = 1024 / units, most = a->keys / 256;
+  int64_t s = 512 / units, most = a->keys / 256;
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
 }
@@ -1008,7 +1021,9 @@ template <class K> int prepare_lds(K kernel, size_t bytes) {
 }
 
 // Workgroups of one block, for `blocks` blocks that walk over `rows` rows: two workgroups on every CU, but shares of at least 256
-// rows (128 of float32, whose steps take three times as long), or the join costs more than it gives.
+// rows (128 of float32, whose steps take three times as long), or the join costs more than it gives.  Training of 2x8(2)x2048^2, 64
+// components, for 256, 512 and 1024 workgroups: 216, 183, 197 us; 2x8x4096^2, 128 components: 568, 568, 595.  At least 128, 256 and
+// 512 rows: a forward pass of 8x300x2000 25, 19, 21 us; at least 64, 128 and 256 of float32, training of 3x6x517x777: 158, 147, 181.
 int shares_of(int64_t blocks, int64_t rows, int dtype) {
   int64_t s = blocks < 1 ? 1 : 512 / blocks, most = rows / (dtype == 2 ? 128 : 256);
   s = s < most ? s : most;

@@ -6,6 +6,9 @@
 // Chunks of 64 tokens: within a chunk the masked product (q k^T) o g^(i-j) times v, across chunks the state, so a token costs
 // 4 dim dim_v flop and 64 (dim + dim_v) more.  The state stays in the registers of the wavefronts, each of which has 32 of its
 // columns, as a C tile (keops_seq.h) that serves as an operand as it is.
+//
+// What bounds it is traffic: q, k, v and the outputs once, k and v a second time for the segments' states, and these.  16 x 16384
+// tokens, 128 components, bf16: 132 us for 540 MB; training of 4x8x4096, 64 components: 145 us for 520 MB in 8 launches.
 #include "../../../include/keops_hip.h"
 #include "keops_seq.h"
 
@@ -67,7 +70,8 @@ __device__ inline void update_state(f32x16 (&S)[DK / 32], const lds_t<Tc>* kt, c
 // Few sequences and heads do not fill the chip, so a long sequence is cut into segments: their own states first (this kernel),
 // then decay_scan carries them on, then decay_outputs starts every segment from its state.
 // A wavefront has 32 columns and half of the rows of a state.  The decayed values, which every row needs, are formed once, on their
-// way to LDS, as three bf16 terms each (all 24 bits: these states are results).
+// way to LDS, as three bf16 terms each (all 24 bits: these states are results).  16 x 16384 tokens, 128 components: 45 us, 3.7 TB/s
+// (58 us with all rows and their own decayed values in each wavefront).
 template <class Tin, class Tc, int DK, int DV, bool REV>
 __global__ void __launch_bounds__(4 * DV, 2) decay_states(const Args A, int segments, int seg_tokens, float* states) {
   constexpr int C = chunk<Tc>(), NT = 4 * DV, SK = tile_stride<Tc, DK>(), SV = tile_stride<Split<3>, DV>(), I = DK / 64;
@@ -127,7 +131,7 @@ __global__ void __launch_bounds__(4 * DV, 2) decay_states(const Args A, int segm
     }
 }
 
-// states before the segments in place of the segments' own, and the final state
+// States before the segments in place of the segments' own, and the final state.  16 heads of 32 states of 128 x 128: 17 us, 3.9 TB/s.
 __global__ void __launch_bounds__(256) decay_scan(const Args A, int segments, int seg_tokens, float* states) {
   const int unit = blockIdx.y, b = unit / A.heads, h = unit % A.heads, size = A.dim * A.dim_v;
   const int e = blockIdx.x * 256 + threadIdx.x;
@@ -186,7 +190,9 @@ template <class Tc, int DK, int DV> constexpr size_t query_bytes() {
   return q > o ? q : o;
 }
 
-// CUT: sequences are cut into segments, whose states are known
+// CUT: sequences are cut into segments, whose states are known.  16 x 16384 tokens, 128 components: 78 us, 3.9 TB/s; 4x8x4096, 64
+// components: 23 us, 3.6 TB/s.  Two wavefronts for every 32 columns, each with half of the tokens and of the state's rows, which
+// makes four a SIMD of two, took 80 and 21 us (training at 128 components 251 for 245).
 template <class Tin, class Tc, int DK, int DV, bool REV, bool CUT>
 __global__ void __launch_bounds__(2 * DV, (Vec<Tc>::terms == 1 && DK <= DV ? 2 : 1)) decay_outputs(const Args A, int segments, int seg_tokens, const float* states) {
   constexpr int C = chunk<Tc>(), U = C / 32, NT = 2 * DV, NW = DV / 32, SK = tile_stride<Tc, DK>(), SV = tile_stride<Tc, DV>(), SP = tile_stride<Tc, C>();
@@ -310,7 +316,7 @@ __global__ void __launch_bounds__(2 * DV, (Vec<Tc>::terms == 1 && DK <= DV ? 2 :
   }
 }
 
-// sums over the heads that share one, in their order, four components to a thread
+// Sums over the heads that share one, in their order, four components to a thread (2 to 4 us for 3x6x777 tokens).
 template <class Tin> __global__ void __launch_bounds__(256) decay_join(const Args A) {
   const int quads = A.dim_v / 4, J = A.joined_heads, group = A.heads / J;
   const long long total = (long long)A.batch * J * A.tokens * quads;
@@ -328,7 +334,8 @@ template <class Tin> __global__ void __launch_bounds__(256) decay_join(const Arg
 // ---- one token ----------------------------------------------------------------------------------------------------------------
 //
 // One read and one write of the state, float32.  A workgroup has `slice` columns of one head's state, 16 bytes of a row to a
-// thread; the sum over the rows is joined in LDS.
+// thread; the sum over the rows is joined in LDS.  64 x 16 states of 128 x 128: 134 MB in 22.4 us (6 TB/s, part of it from the
+// cache behind HBM).
 struct Strides2 { long long batch, head; };
 
 template <class T>
@@ -418,7 +425,9 @@ const char* check(const Args* a) {
   return nullptr;
 }
 
-// Segments of a sequence: enough workgroups to fill the chip, whole chunks each.
+// Segments of a sequence: enough workgroups to fill the chip, whole chunks each; more of them carry more states.  A prompt of
+// 16 x 16384 tokens, 128 components, with 256, 512, 768 and 1024 workgroups: 191, 144, 154 and 168 us; training of 4x8x4096, 64
+// components, with 256, 512, 768, 1024 and 2048: 237, 167, 148, 148 and 166.
 void segments_of(const Args* a, int& segments, int& seg_tokens) {
   const int64_t units = (int64_t)a->batch * a->heads, chunks = (a->tokens + kChunk - 1) / kChunk;
   const int64_t fill = a->dim > 64 || a->dim_v > 64 ? 512 : 1024;  // (the same for exchanged dims: the states are shared)
@@ -470,7 +479,8 @@ template <class Tin, class Tc> int dispatch(const Args& a, hipStream_t st) {
 template <class T>
 int step(int batch, int heads, int group, int dim, int dim_v, float scale, const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v,
          const int64_t* vs, const float* log_decay, float* state, void* out, hipStream_t st) {
-  // narrow slices while whole heads would not give two workgroups to a CU
+  // Narrow slices while whole heads would not give two workgroups to a CU: 32 states of 128 x 128 4.1 us (whole heads: 5.1), 320 9.5
+  // (9.8), 1024 22.4 whole (slices: 23.1).
   const int units = batch * heads, slice = units >= 512 ? 128 : 32;
   decay_step<T><<<dim3(units, (dim_v + slice - 1) / slice), 256, 0, st>>>(heads, group, dim, dim_v, slice, scale, (const T*)q, Strides2{qs[0], qs[1]},
                                                                           (const T*)k, Strides2{ks[0], ks[1]}, (const T*)v, Strides2{vs[0], vs[1]}, log_decay,
