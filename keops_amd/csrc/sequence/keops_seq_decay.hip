@@ -8,7 +8,7 @@
 // columns, as a C tile (keops_seq.h) that serves as an operand as it is.
 //
 // What bounds it is traffic: q, k, v and the outputs once, k and v a second time for the segments' states, and these.  16 x 16384
-// tokens, 128 components, bf16: 132 us for 540 MB; training of 4x8x4096, 64 components: 145 us for 520 MB in 8 launches.
+// tokens, 128 components, bf16: 132 us for 540 MB; training of 4x8x4096, 64 components: 140 us for 500 MB in 8 launches.
 #include "../../../include/keops_hip.h"
 #include "keops_seq.h"
 
