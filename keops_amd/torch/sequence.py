@@ -167,6 +167,9 @@ class PositionBuckets:
         self._device = {}
         self._plans = {}  # of bucket_attention with these buckets, by the geometry of the tensors
 
+    def __reduce__(self):  # copies and pickles hold the map alone: device copies and plans (which hold their addresses) stay behind
+        return PositionBuckets.from_map, (self._host[0].tolist(), self.num_buckets)
+
     def __call__(self, relative_position):
         """Bucket of each entry of an integer tensor of relative positions ``key - query``."""
         table = self._host[0].to(device=relative_position.device, dtype=torch.int64)
@@ -187,9 +190,9 @@ class _BucketPlan:
     """Arguments of a call that depend on the geometry of its tensors alone, checked once."""
 
     def __init__(self, q, k, v, bias, buckets, causal, start, scale):
-        self.tables = buckets.on(q.device)
+        self.tables, self.options = buckets.on(q.device), (buckets, causal, start, scale)
         self.out_strides, self.k_strides, self.v_strides = _dense_strides(q), _dense_strides(k), _dense_strides(v)
-        self.index = q.device.index
+        self.index, self.saved_strides = q.device.index, (q.stride(), k.stride(), v.stride(), self.out_strides)
         a = binder.BucketAttention()
         a.dtype, a.batch, a.heads, a.kv_heads, a.dim = _DTYPES[q.dtype], q.shape[0], q.shape[1], k.shape[1], q.shape[3]
         a.queries, a.keys, a.causal, a.scale = q.shape[2], k.shape[2], int(causal), scale
@@ -271,6 +274,9 @@ class _BucketAttention(torch.autograd.Function):
         plan = ctx.plan
         if plan.empty:
             return (*(torch.zeros_like(t) for t in (q, k, v, bias)), None, None, None)
+        if (q.stride(), k.stride(), v.stride(), out.stride()) != plan.saved_strides:  # hooks on saved tensors may lay them out anew
+            q, k, v, out = (_rows(x.contiguous()) for x in (q, k, v, out))
+            plan = _BucketPlan(q, k, v, bias, *plan.options)
         return (*plan.backward(grad, q, k, v, bias, out, lse, key_lengths, query_start, ctx.needs_input_grad[0], ctx.needs_input_grad[3]),
                 None, None, None)
 
@@ -420,6 +426,7 @@ class _DecayPlan:
     def __init__(self, q, k, v, scale):
         self.dtype, self.device, self.scale, self.heads, self.shared = q.dtype, q.device, scale, q.shape[1], k.shape[1]
         self.q, self.k, self.v = ((x.shape, x.stride()) for x in (q, k, v))
+        self.saved_strides = (q.stride(), k.stride(), v.stride())
         shape = (*q.shape[:3], v.shape[3])
         if q.shape[3] == v.shape[3]:
             strides = _dense_strides(q)
@@ -474,6 +481,9 @@ class _DecayAttention(torch.autograd.Function):
         # that of k from those of v's
         q, k, v, state, log_decay, lengths, states = ctx.saved_tensors
         plan = ctx.plan
+        if (q.stride(), k.stride(), v.stride()) != plan.saved_strides:  # hooks on saved tensors may lay them out anew
+            q, k, v = (_rows(x.contiguous()) for x in (q, k, v))
+            plan = _DecayPlan(q, k, v, plan.scale)
         if grad is None:
             grad = torch.zeros(plan.out[0], dtype=q.dtype, device=q.device)
         elif grad.stride() not in plan.gradients or grad.data_ptr() & 15:  # (strides that have walks fit)

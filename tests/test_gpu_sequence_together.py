@@ -1,5 +1,7 @@
 """The sequence operators as a model uses them: a layer of softmax attention with position buckets, a layer of linear attention with
 decays, logits, log probabilities and entropies; trained on a padded batch, then generating one token at a time from its caches."""
+import contextlib
+
 import pytest
 import torch
 
@@ -125,3 +127,25 @@ def test_generation_from_caches_is_the_whole_sequence():
                 one = token_logprobs(_model(w, tokens[:, t:t + 1], None, attend_one, carry_one), targets[:, t:t + 1], top=2)
                 for a, b in ((one.logprob, whole.logprob), (one.entropy, whole.entropy), (one.top_logprob, whole.top_logprob)):
                     assert (a[:, 0] - b[:, t]).abs().max() < tol * max(1.0, float(b.abs().max())), (dtype, t)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_saved_tensors_that_hooks_lay_out_anew(dtype):
+    """Saved tensors that travel to the host and back come back contiguous, whatever the strides of the inputs were."""
+    from keops_amd.torch import PositionBuckets, bucket_attention, decay_attention, token_logprobs
+
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=gen).to(dtype)
+    q, k = r(2, 150, 4, 64)[..., :32].transpose(1, 2), r(2, 150, 2, 32).transpose(1, 2)  # rows of a wider tensor; another order
+    v = r(1, 2, 150, 32).expand(2, 2, 150, 32)
+    bias, b = torch.randn(4, 32, device="cuda", generator=gen), PositionBuckets()
+    ld, x, tokens, go = -torch.rand(4, device="cuda", generator=gen), r(20, 600)[:, 40:], torch.arange(20, device="cuda"), r(2, 4, 150, 32)
+
+    def gradients(offload):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v, bias, x)]
+        with torch.autograd.graph.save_on_cpu() if offload else contextlib.nullcontext():
+            outs = (bucket_attention(*leaves[:4], b, causal=True), decay_attention(*leaves[:3], ld)[0], token_logprobs(leaves[4], tokens, top=3).logprob)
+        return torch.autograd.grad(outs, leaves, (go, go, torch.ones(20, device="cuda")))
+
+    for want, got in zip(gradients(False), gradients(True)):
+        assert torch.equal(want, got)

@@ -1,7 +1,9 @@
 """Sequence operators on the CPU: buckets of relative positions, what the entry points refuse, and the 64-bit references that the
 device tests use (against torch's autograd and against differences)."""
+import copy
 import ctypes
 import math
+import pickle
 
 import pytest
 import torch
@@ -183,6 +185,15 @@ def test_joined_outputs_that_the_library_refuses(changes):
     for name, value in changes.items():
         setattr(a, name, value)
     assert binder.lib().keops_hip_decay_attention_run(ctypes.byref(a), 0, None) != 0 and "joined" in binder.last_error()
+
+
+def test_copies_and_pickles_of_buckets_hold_the_map_alone():
+    """A plan holds the addresses of the tables of the object that made it: no copy may take it along."""
+    b = PositionBuckets(16, 40, False)
+    b._plans["geometry"], b._device[torch.device("cpu")] = "plan", b._host
+    for c in (copy.copy(b), copy.deepcopy(b), pickle.loads(pickle.dumps(b))):
+        assert c is not b and not c._plans and not c._device
+        assert (c.num_buckets, c.reach) == (b.num_buckets, b.reach) and all(map(torch.equal, c._host, b._host))
 
 
 def test_first_use_of_buckets_inside_of_a_capture_is_refused(monkeypatch):
