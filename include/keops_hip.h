@@ -204,6 +204,8 @@ typedef struct keops_hip_bucket_attention {
   int64_t grad_out_stride[3], grad_q_stride[3], grad_k_stride[3], grad_v_stride[3];
   float* delta;                   /* (batch, heads, queries), written */
   float* grad_bias;               /* (heads, buckets) or NULL */
+  void* out_rest;                 /* what the rounding of out to 16 bits leaves, laid out like it: written by the forward pass, read by
+                                     the backward pass; NULL: none */
 } keops_hip_bucket_attention;
 
 size_t keops_hip_bucket_attention_forward_bytes(const keops_hip_bucket_attention* a);

@@ -24,7 +24,7 @@ class BucketAttention(ctypes.Structure):
         + [(n, _P) for n in ("q", "k", "v", "out")] + [(n + "_stride", _I64 * 3) for n in ("q", "k", "v", "out")]
         + [(n, _P) for n in ("lse", "bias", "bucket_of", "bucket_order", "bucket_begin", "key_lengths", "query_start", "grad_out",
                              "grad_q", "grad_k", "grad_v")]
-        + [(n + "_stride", _I64 * 3) for n in ("grad_out", "grad_q", "grad_k", "grad_v")] + [("delta", _P), ("grad_bias", _P)]
+        + [(n + "_stride", _I64 * 3) for n in ("grad_out", "grad_q", "grad_k", "grad_v")] + [("delta", _P), ("grad_bias", _P), ("out_rest", _P)]
     )
 
 

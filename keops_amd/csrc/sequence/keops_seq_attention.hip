@@ -51,6 +51,14 @@ __device__ inline void fill_table(float* table, const Args& A, int h, int tid, i
 template <class T> __device__ inline const T* rows_of(const void* p, const int64_t* s, int b, int h) { return (const T*)p + (long long)b * s[0] + (long long)h * s[1]; }
 template <class T> __device__ inline T* rows_of(void* p, const int64_t* s, int b, int h) { return (T*)p + (long long)b * s[0] + (long long)h * s[1]; }
 
+// outputs, and what their rounding leaves
+template <class Tin> __device__ inline void put_out(const Args& A, int b, int h, int row, int d, float x) {
+  const Tin v = (Tin)x;
+  rows_of<Tin>(A.out, A.out_stride, b, h)[(long long)row * A.out_stride[2] + d] = v;
+  if (A.out_rest) rows_of<Tin>(A.out_rest, A.out_stride, b, h)[(long long)row * A.out_stride[2] + d] = (Tin)(x - (float)v);
+}
+template <class Tin> __device__ inline float left_of(float x) { return x - (float)(Tin)x; }
+
 // Keys of a staged tile: 32 where 64 would not leave the rows in flight, the logits and the sums in 256 registers.  Forward pass of
 // 4x8x4096^2, 64 components, 64 keys 115 us and 32 keys 127; 8x16384^2, 128 components, 64 keys 1557 us (spilled) and 32 keys 672.
 template <class Tc, int DP> constexpr int key_tile() { return Vec<Tc>::terms == 1 && DP <= 64 ? 64 : 32; }
@@ -296,6 +304,18 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>())) attention_forward(cons
         const int d = 32 * i + 8 * g + 4 * half;
         if (d < A.dim) store4<Tin>(o + d, acc[i][4 * g] * inv, acc[i][4 * g + 1] * inv, acc[i][4 * g + 2] * inv, acc[i][4 * g + 3] * inv);
       }
+    if (A.out_rest) {
+      Tin* rest = rows_of<Tin>(A.out_rest, A.out_stride, b, h) + (long long)row * A.out_stride[2];
+#pragma unroll
+      for (int i = 0; i < ND; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+          const int d = 32 * i + 8 * g + 4 * half;
+          if (d < A.dim)
+            store4<Tin>(rest + d, left_of<Tin>(acc[i][4 * g] * inv), left_of<Tin>(acc[i][4 * g + 1] * inv), left_of<Tin>(acc[i][4 * g + 2] * inv),
+                        left_of<Tin>(acc[i][4 * g + 3] * inv));
+        }
+    }
     // base-2 log of the row's sum; a row that sees nothing gets +inf, with which its probabilities are zeros later
     if (A.lse && half == 0) A.lse[((long long)b * A.heads + h) * M + row] = l == 0.f ? kInf : m + __builtin_amdgcn_logf(l);
   }
@@ -443,7 +463,7 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_rows(const
     }
     const int hr = kvh * group + r / M, qr = r % M;
     if (splits == 1) {
-      if (d < A.dim) rows_of<Tin>(A.out, A.out_stride, b, hr)[(long long)qr * A.out_stride[2] + d] = (Tin)(ll == 0.f ? 0.f : o / ll);
+      if (d < A.dim) put_out<Tin>(A, b, hr, qr, d, ll == 0.f ? 0.f : o / ll);
       if (A.lse && d == 0) A.lse[((long long)b * A.heads + hr) * M + qr] = ll == 0.f ? kInf : mm + __builtin_amdgcn_logf(ll);
     } else {
       float* p = part + ((long long)blockIdx.x * rows + r) * (DP + 2);
@@ -493,7 +513,7 @@ template <class Tin> __global__ void __launch_bounds__(512) attention_join(const
   __syncthreads();
   if (tid < A.dim) {
     o = (sums[0][d] + sums[1][d]) + (sums[2][d] + sums[3][d]);
-    rows_of<Tin>(A.out, A.out_stride, b, h)[(long long)qi * A.out_stride[2] + d] = (Tin)(ll == 0.f ? 0.f : o / ll);
+    put_out<Tin>(A, b, h, qi, d, ll == 0.f ? 0.f : o / ll);
   }
   if (A.lse && tid == 0) A.lse[((long long)b * A.heads + h) * M + qi] = ll == 0.f ? kInf : mm + __builtin_amdgcn_logf(ll);
 }
@@ -530,7 +550,11 @@ template <class Tin, bool GRAD> __global__ void __launch_bounds__(256) attention
       for (int j = 0; j < 4; j++) o[j] = fmaf(a, x[j], o[j]);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    store4<Tin>(rows_of<Tin>(A.out, A.out_stride, b, h) + (long long)q * A.out_stride[2] + c, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    const long long at = (long long)q * A.out_stride[2] + c;
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] *= inv;
+    store4<Tin>(rows_of<Tin>(A.out, A.out_stride, b, h) + at, o[0], o[1], o[2], o[3]);
+    if (A.out_rest) store4<Tin>(rows_of<Tin>(A.out_rest, A.out_stride, b, h) + at, left_of<Tin>(o[0]), left_of<Tin>(o[1]), left_of<Tin>(o[2]), left_of<Tin>(o[3]));
     if (A.lse && c == 0) A.lse[((long long)b * A.heads + h) * A.queries + q] = l == 0.f ? kInf : mm + __builtin_amdgcn_logf(l);
   }
 }
@@ -557,10 +581,11 @@ template <class Tin> __global__ void __launch_bounds__(256) attention_join_keys(
 // ---- gradient of the queries ------------------------------------------------------------------------------------------------
 //
 // P = exp2(z - lse), dP = dO V^T, dS = P (dP - delta), dq = scale dS K, laid out as in the forward pass.  delta_i = sum_j P_ij dP_ij
-// equals <dO_i, o_i>, but the stored output is rounded and came from rounded probabilities, and the bias gradient sums rows whose
-// exact sum is zero: a delta off by 2^-9 of itself would be most of a far bucket's gradient in a long row.  So dS is formed with
-// <dO_i, o_i>, and the row sums of that dS, which are what delta is off by, are added to the delta that the gradient of keys,
-// values and biases uses.
+// equals <dO_i, o_i>, but the output is rounded and came from rounded probabilities.  The forward pass of a training call leaves
+// what the output's rounding took (out_rest): without it delta adds half as much to the error of dq as the rounding of dS does (rows
+// with few keys; 2.6e-3 of dq for 2.3e-3, bf16).  The bias gradient sums rows whose exact sum is zero: a delta off by 2^-9 of itself would
+// be most of a far bucket's gradient in a long row.  So dS is formed with <dO_i, o_i>, and the row sums of that dS, which are what
+// delta is off by, are added to the delta that the gradient of keys, values and biases uses.
 //
 // 4x8 x 4096^2 causal bf16, 64 components: 150 us, 0.69 Pflop/s; of a SIMD's cycles matrix instructions take 30 %, vector ones 41 %.
 template <class Tin, class Tc, int DP>
@@ -592,13 +617,21 @@ __global__ void __launch_bounds__(256, (waves<Tc, DP>(32))) attention_grad_q(con
     const Tin* q = rows_of<Tin>(A.q, A.q_stride, b, h) + (long long)row * A.q_stride[2];
     const Tin* g = rows_of<Tin>(A.grad_out, A.grad_out_stride, b, h) + (long long)row * A.grad_out_stride[2];
     const Tin* o = rows_of<Tin>(A.out, A.out_stride, b, h) + (long long)row * A.out_stride[2];
+    const Tin* left = rows_of<Tin>(A.out_rest, A.out_stride, b, h) + (long long)row * A.out_stride[2];
+    const bool there = row < M, rest = there && A.out_rest;
 #pragma unroll
     for (int i = 0; i < NS; i++) {
-      qf[i] = frag_global<Tin, Tc>(q, row < M, 16 * i, half, A.dim);
-      gf[i] = frag_global<Tin, Tc>(g, row < M, 16 * i, half, A.dim);
+      qf[i] = frag_global<Tin, Tc>(q, there, 16 * i, half, A.dim);
+      gf[i] = frag_global<Tin, Tc>(g, there, 16 * i, half, A.dim);
       float gx[8], ox[8];
       to_float(gf[i], gx);
-      to_float(frag_global<Tin, Tc>(o, row < M, 16 * i, half, A.dim), ox);
+      to_float(frag_global<Tin, Tc>(o, there, 16 * i, half, A.dim), ox);
+      if constexpr (sizeof(Tin) == 2) {
+        float rx[8];
+        to_float(frag_global<Tin, Tc>(left, rest, 16 * i, half, A.dim), rx);
+#pragma unroll
+        for (int j = 0; j < 8; j++) ox[j] += rx[j];
+      }
 #pragma unroll
       for (int j = 0; j < 8; j++) delta = fmaf(gx[j], ox[j], delta);
     }
@@ -975,7 +1008,7 @@ int padded_dim(int dim) { return dim <= 32 ? 32 : (dim <= 64 ? 64 : (dim <= 96 ?
 bool aligned(const Args* a) {
   const size_t size = a->dtype == 2 ? 4 : 2;
   return rows_aligned(a->q, a->q_stride, size) && rows_aligned(a->k, a->k_stride, size) && rows_aligned(a->v, a->v_stride, size) &&
-         rows_aligned(a->out, a->out_stride, size) && rows_aligned(a->grad_out, a->grad_out_stride, size) &&
+         rows_aligned(a->out, a->out_stride, size) && rows_aligned(a->out_rest, a->out_stride, size) && rows_aligned(a->grad_out, a->grad_out_stride, size) &&
          rows_aligned(a->grad_q, a->grad_q_stride, size) && rows_aligned(a->grad_k, a->grad_k_stride, size) && rows_aligned(a->grad_v, a->grad_v_stride, size);
 }
 

@@ -226,16 +226,20 @@ class _BucketPlan:
 
     def forward(self, q, k, v, bias, key_lengths, query_start, want_lse):
         out = torch.empty_strided(q.shape, self.out_strides, dtype=q.dtype, device=q.device)
-        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if want_lse else None
+        lse = rest = None
         if not self.empty:
             a = self.fill(self.args, q, k, v, bias, key_lengths, query_start)
             a.out = out.data_ptr()
             if want_lse:
+                lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
                 a.lse = lse.data_ptr()
+                if q.dtype != torch.float32:
+                    rest = torch.empty_strided(q.shape, self.out_strides, dtype=q.dtype, device=q.device)
+                    a.out_rest = rest.data_ptr()
             self.run("keops_hip_bucket_attention_forward", a, self.forward_bytes, q.device)
-        return out, lse
+        return out, rest, lse
 
-    def backward(self, grad, q, k, v, bias, out, lse, key_lengths, query_start, want_q, want_bias):
+    def backward(self, grad, q, k, v, bias, out, rest, lse, key_lengths, query_start, want_q, want_bias):
         args = self.grad_args.get(grad.stride())
         if args is None or grad.data_ptr() & 15:  # the first of these strides, or such that are copied
             grad = _rows(grad)
@@ -248,6 +252,8 @@ class _BucketPlan:
         a = self.fill(args, q, k, v, bias, key_lengths, query_start)
         a.out, a.lse, a.delta, a.grad_out = out.data_ptr(), lse.data_ptr(), delta.data_ptr(), grad.data_ptr()
         a.grad_k, a.grad_v = dk.data_ptr(), dv.data_ptr()
+        if rest is not None:
+            a.out_rest = rest.data_ptr()
         dq = db = None
         if want_q:
             dq = new(q.shape, self.out_strides, dtype=q.dtype, device=q.device)
@@ -262,22 +268,24 @@ class _BucketPlan:
 class _BucketAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, plan, key_lengths, query_start):
-        out, lse = plan.forward(q, k, v, bias, key_lengths, query_start, True)
+        out, rest, lse = plan.forward(q, k, v, bias, key_lengths, query_start, True)
         ctx.plan = plan
-        ctx.save_for_backward(q, k, v, bias, out, lse, key_lengths, query_start)
+        ctx.save_for_backward(q, k, v, bias, out, rest, lse, key_lengths, query_start)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, k, v, bias, out, lse, key_lengths, query_start = ctx.saved_tensors
+        q, k, v, bias, out, rest, lse, key_lengths, query_start = ctx.saved_tensors
         plan = ctx.plan
         if plan.empty:
             return (*(torch.zeros_like(t) for t in (q, k, v, bias)), None, None, None)
-        if (q.stride(), k.stride(), v.stride(), out.stride()) != plan.saved_strides:  # hooks on saved tensors may lay them out anew
+        if (q.stride(), k.stride(), v.stride(), out.stride()) != plan.saved_strides or (rest is not None and rest.stride() != out.stride()):
+            # hooks on saved tensors may lay them out anew
             q, k, v, out = (_rows(x.contiguous()) for x in (q, k, v, out))
+            rest = None if rest is None else _rows(rest.contiguous())
             plan = _BucketPlan(q, k, v, bias, *plan.options)
-        return (*plan.backward(grad, q, k, v, bias, out, lse, key_lengths, query_start, ctx.needs_input_grad[0], ctx.needs_input_grad[3]),
+        return (*plan.backward(grad, q, k, v, bias, out, rest, lse, key_lengths, query_start, ctx.needs_input_grad[0], ctx.needs_input_grad[3]),
                 None, None, None)
 
 

@@ -242,6 +242,24 @@ def test_graph_streams_and_repeats():
         assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,n", [(64, 2), (1, 2), (70, 4000), (1, 4000), (33, 257)])
+def test_what_the_rounding_of_the_output_leaves(m, n, dtype):
+    """All logits equal, so outputs are means: a training call keeps a second term of them for the gradient's row sums.  Two terms are
+    off by half a step of half a step, the sum of n values by a step of float32 for each, and by the underflow of the second term."""
+    from keops_amd.torch import PositionBuckets, bucket_attention
+
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.zeros(2, 2, m, 48, device="cuda", dtype=dtype, requires_grad=True)
+    k, v = (torch.randn(2, 2, n, 48, device="cuda", generator=gen).to(dtype) for _ in range(2))
+    out = bucket_attention(q, k, v, torch.zeros(2, 32, device="cuda"), PositionBuckets())
+    rest = out.grad_fn.saved_tensors[5]
+    mean, size = v.double().mean(2, keepdim=True), v.double().abs().mean(2, keepdim=True)
+    half = torch.finfo(dtype).eps / 2
+    ref.assert_within(out.double() + rest.double(), mean.expand_as(out), (half ** 2 * mean.abs() + (n + 4) * 2.0 ** -23 * size + 2.0 ** -25).expand_as(out), "two terms")
+    assert rest.stride() == out.stride() and bool((rest != 0).any())
+
+
 def test_single_ones_may_have_any_stride_and_numbers_any_type():
     from keops_amd.torch import PositionBuckets, bucket_attention
 
