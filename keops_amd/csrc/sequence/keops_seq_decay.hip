@@ -19,7 +19,9 @@ namespace {
 typedef keops_hip_decay_attention Args;
 
 constexpr int kChunk = 64;  // tokens of a chunk
-template <class Tc> constexpr int chunk() { return Vec<Tc>::terms > 2 ? 32 : kChunk; }  // (tiles of three terms: what LDS holds)
+// With 32 tokens also for two terms: float16 training of 4x8x4096, 64 components, 164 us (64 tokens: 216), a prompt of 16 x 16384
+// tokens, 128 components, 190 (220): more workgroups fit in LDS.
+template <class Tc> constexpr int chunk() { return Vec<Tc>::terms > 1 ? 32 : kChunk; }
 
 // Decayed values as an operand for the state: all of a float32 where the state is a result (or becomes one over the segments
 // behind), 16 bits where it only serves outputs that are rounded to 8.  The state itself is float32; as an operand for those
@@ -166,10 +168,11 @@ __device__ inline void store_rows(T* out, long long stride, const f32x16 (&o)[U]
   constexpr int VE = 16 / (int)sizeof(T), PER_ROW = 32 / VE;
   T* const tile = (T*)strip;
   const int half = lane >> 5, col = lane & 31, row0 = lane / PER_ROW, c = 32 * wave + (lane % PER_ROW) * VE;
+  T* const place = tile + 128 * half + col;
 #pragma unroll
   for (int u = 0; u < U; u++) {
 #pragma unroll
-    for (int r = 0; r < 16; r++) tile[c_row(r, half) * 32 + col] = (T)o[u][r];
+    for (int r = 0; r < 16; r++) place[c_row(r, 0) * 32] = (T)o[u][r];
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -190,11 +193,13 @@ template <class Tc, int DK, int DV> constexpr size_t query_bytes() {
   return q > o ? q : o;
 }
 
+// Two terms: two wavefronts a SIMD, which leaves no sums in accumulation registers: with one, the compiler stored row 1 of a float32
+// tile 32 bytes behind row 0 instead of 128.
 // CUT: sequences are cut into segments, whose states are known.  16 x 16384 tokens, 128 components: 78 us, 3.9 TB/s; 4x8x4096, 64
 // components: 23 us, 3.6 TB/s.  Two wavefronts for every 32 columns, each with half of the tokens and of the state's rows, which
 // makes four a SIMD of two, took 80 and 21 us (training at 128 components 251 for 245).
 template <class Tin, class Tc, int DK, int DV, bool REV, bool CUT>
-__global__ void __launch_bounds__(2 * DV, (Vec<Tc>::terms == 1 && DK <= DV ? 2 : 1)) decay_outputs(const Args A, int segments, int seg_tokens, const float* states) {
+__global__ void __launch_bounds__(2 * DV, (Vec<Tc>::terms == 1 ? (DK <= DV ? 2 : 1) : Vec<Tc>::terms == 2 ? 2 : 1)) decay_outputs(const Args A, int segments, int seg_tokens, const float* states) {
   constexpr int C = chunk<Tc>(), U = C / 32, NT = 2 * DV, NW = DV / 32, SK = tile_stride<Tc, DK>(), SV = tile_stride<Tc, DV>(), SP = tile_stride<Tc, C>();
   extern __shared__ __align__(16) unsigned char smem[];
   lds_t<Tc>* const qt = (lds_t<Tc>*)smem;  // and, once the chunk's queries have been used, the outputs on their way
@@ -425,13 +430,14 @@ const char* check(const Args* a) {
   return nullptr;
 }
 
-// Segments of a sequence: enough workgroups to fill the chip, whole chunks each; more of them carry more states.  A prompt of
+// Segments of a sequence: as many workgroups as the chip takes at once, whole chunks each; more of them carry more states, and a few
+// more wait for a second turn (220 sequences times heads of 2094 tokens in 3 segments 722 us, in 2 636).  A prompt of
 // 16 x 16384 tokens, 128 components, with 256, 512, 768 and 1024 workgroups: 191, 144, 154 and 168 us; training of 4x8x4096, 64
 // components, with 256, 512, 768, 1024 and 2048: 237, 167, 148, 148 and 166.
 void segments_of(const Args* a, int& segments, int& seg_tokens) {
   const int64_t units = (int64_t)a->batch * a->heads, chunks = (a->tokens + kChunk - 1) / kChunk;
   const int64_t fill = a->dim > 64 || a->dim_v > 64 ? 512 : 1024;  // (the same for exchanged dims: the states are shared)
-  int64_t want = (fill + units - 1) / units;
+  int64_t want = fill / units;
   if (want > chunks) want = chunks;
   if (want < 1) want = 1;
   const int64_t per = chunks < 1 ? 1 : (chunks + want - 1) / want;

@@ -147,6 +147,7 @@ def test_decay_states_serve_the_walks_with_exchanged_dims(dtype):
                         setattr(a, name, 16)
                     need.append(lib.keops_hip_decay_attention_bytes(ctypes.byref(a)))
                 assert need[0] == need[1], (units, tokens, d, dv)
+    a.heads = a.q_heads = a.k_heads = a.v_heads = 24  # (few enough for segments)
     a.tokens, a.states, a.states_given = 9000, 16, 1
     need = lib.keops_hip_decay_attention_bytes(ctypes.byref(a))
     for size in (need + 16, need - 16):  # states of other segments
